@@ -489,6 +489,114 @@ typedef struct osam_aug_out {
  * follow the reference kernels' float steps in their order, under the same fast-math arithmetic. */
 int osam_augment(const osam_aug_batch* batch, int B, int S, const osam_aug_out* out, osam_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Token operators: a map of H×W pixels in NHWC is a matrix of H·W tokens × C channels, so a block that mixes
+ * tokens (norm → projections by 1×1 convs → attention) works on the model's activations in place.  No
+ * counterpart in the reference.  Types of 16-bit tensors and of gradients: */
+enum { OSAM_F16 = 0, OSAM_BF16 = 1, OSAM_F32 = 2 };
+
+/* RMS norm over the C channels of each row, with the residual's addition in front:
+ *   h = x + res (res NULL: h = x);  sum ← h (sum NULL: not written);  rstd = 1/√(Σ h²/C + eps)
+ *   y = h·rstd·w
+ * in fp32, each output rounded once.  x, res, sum, y are rows of C 16-bit values (dtype), ld* elements from row
+ * to row (a channel slice of a wider buffer: ld = its channels); C a multiple of 8, 8 ≤ C ≤ 8192, ld multiples
+ * of 8, ld ≥ C, 16-byte aligned.  w fp32 [C]; rstd fp32 [rows] or NULL.  sum may be x or res itself, y may be x
+ * where sum is not. */
+int osam_rms_fwd(int dtype, const void* x, int64_t ldx, const void* res, int64_t ldres, const float* w, int64_t rows,
+                 int C, float eps, void* sum, int64_t ldsum, void* y, int64_t ldy, float* rstd, osam_stream_t stream);
+/* The same with y in e4m3 and a scale per 128 channels (the last group may be shorter): qscale [rows][⌈C/128⌉] =
+ * max|y|/448 over the group, q = e4m3(y·448/max|y|), zeros where the group is all zero.  q: ldq bytes from row to
+ * row, 8-byte aligned. */
+int osam_rms_fwd_q8(int dtype, const void* x, int64_t ldx, const void* res, int64_t ldres, const float* w,
+                    int64_t rows, int C, float eps, void* sum, int64_t ldsum, void* q, int64_t ldq, float* qscale,
+                    float* rstd, osam_stream_t stream);
+/* Backward of osam_rms_fwd: with h (sum, or x where there was no residual) and rstd of the forward,
+ *   dx = rstd·(w·dy − ĥ·Σ(w·dy·ĥ)/C) + dsum   (ĥ = h·rstd; dsum: the gradient that reaches h by the residual
+ *   path, or NULL);  dw[c] = Σ_rows dy·ĥ  (written, not accumulated).
+ * dx is the gradient of x and of res alike.  dx may be dy or dsum.  The sums over rows are added in a fixed order.
+ * Workspace: osam_rms_bwd_workspace_size(C) bytes, 16-byte aligned, any contents. */
+size_t osam_rms_bwd_workspace_size(int C);
+int osam_rms_bwd(int dtype, const void* dy, int64_t lddy, const void* h, int64_t ldh, const float* w,
+                 const float* rstd, const void* dsum, int64_t lddsum, int64_t rows, int C, void* dx, int64_t lddx,
+                 float* dw, void* ws, size_t ws_bytes, osam_stream_t stream);
+
+/* AdamW over many tensors in one launch.  For every element, in fp32:
+ *   g' = g·mul;  m = β1·m + (1−β1)·g';  v = β2·v + (1−β2)·g'²
+ *   p = p·(1 − lr·weight_decay) − lr/(1−β1ᵗ)·m/(√v/√(1−β2ᵗ) + eps)   (tensors with decay = 0: no decay)
+ * and, where a tensor has one, its 16-bit copy ← p.  mul = grad_scale, or with max_norm > 0
+ * grad_scale·min(1, max_norm/(norm + 1e-6)), norm = grad_scale·√Σ g² over all tensors (written to *norm); a norm
+ * that is not finite (an fp16 overflow, say) leaves parameters, copies and states untouched.
+ * bits = 32: m and v are fp32 arrays of state_elems elements, zero at the start; each tensor's part begins at the next
+ * multiple of 64.  bits = 8: m and v are e4m3 arrays (parts begin at multiples of 256) with a scale per 256
+ * elements in m_scale / v_scale [state_elems / 256]: m = e4m3·scale, and √v = e4m3·scale; all zero at the start.
+ * The plan writes a table of the tensors into the caller's device buffer once; the tensors' addresses are fixed
+ * from then on.  Steps of one plan run in stream order (they share the table's scratch).
+ *   osam_adamw_sizes    bytes of the table and elements of the states
+ *   osam_adamw_create   fills `table` (256-byte aligned, kept by the caller) on `stream`
+ *   osam_adamw_step     t counts from 1; m, v 16-byte aligned */
+typedef struct osam_adamw_tensor {
+  float* p;        /* parameters, fp32 */
+  const void* g;   /* gradients of grad_type */
+  void* copy;      /* 16-bit copy of the parameters (copy_type), or NULL */
+  int64_t n;
+  int grad_type;   /* OSAM_F32, OSAM_F16, OSAM_BF16 */
+  int copy_type;   /* OSAM_F16, OSAM_BF16 */
+  int decay;       /* 0: no weight decay (norm gains, biases) */
+} osam_adamw_tensor;
+typedef struct osam_adamw osam_adamw;
+int osam_adamw_sizes(const osam_adamw_tensor* tensors, int n, int bits, size_t* table_bytes, int64_t* state_elems);
+int osam_adamw_create(const osam_adamw_tensor* tensors, int n, int bits, void* table, size_t table_bytes,
+                      osam_stream_t stream, osam_adamw** out);
+int osam_adamw_step(const osam_adamw* a, void* m, void* v, float* m_scale, float* v_scale, int64_t t, double lr,
+                    double beta1, double beta2, double eps, double weight_decay, double grad_scale, double max_norm,
+                    float* norm, osam_stream_t stream);
+int osam_adamw_destroy(osam_adamw* a);
+
+/* Attention with capped scores, a distance bias and document, prefix or causal masks, forward and backward; the
+ * same call serves single tokens over a long cache (few query rows: the keys are split over the GPU and joined).
+ *   s_ij = cap·tanh(scale·q_i·k_j/cap)  (cap > 0)   or   scale·q_i·k_j  (cap = 0)
+ *   x_ij = s_ij − slopes[head]·dist(i, j)           (slopes NULL: no bias; they get no gradient)
+ *   o_i = Σ_j p_ij v_j,  p_ij = exp(x_ij − lse_i),  over the keys that i sees
+ * n_b = lens[b] (clamped to 0 … len_k; lens NULL: len_k) keys are in use; query i stands at position
+ * i + n_b − len_q, key j at j.  dist = |pos_i − j|, or with grid_w > 0, tokens laid row by row on a map grid_w
+ * wide, |y_i − y_j| + |x_i − x_j|.  i sees j < n_b when, by `mask`, OSAM_ATTN_NONE: always; CAUSAL: j ≤ pos_i;
+ * PREFIX: j ≤ pos_i or j < prefix[b]; and with documents (doc_q [batch][len_q] and doc_k [batch][len_k], both or
+ * neither) doc_q[i] = doc_k[j] ≥ 0: a token with a negative id sees nothing and is seen by none.  A query that
+ * sees nothing gets o = 0, lse = −∞ and gives no gradient.  Contents of K and V rows past n_b or of tokens without
+ * a document do not matter (NaN included).
+ * Query head h reads key head h / (heads_q / heads_k).  Tensors are dtype (OSAM_F16 / OSAM_BF16), [batch][token]
+ * [head][dim] by element strides with dim contiguous; strides multiples of 8 and not 0 (where the extent is
+ * above 1), 16-byte aligned; dim a multiple of 8, 8 … 128.  With documents len_q and len_k ≤ 1048576.
+ * lse [batch][heads_q][len_q] fp32 (natural log), or NULL in the forward.  Scores, softmax statistics and sums
+ * are fp32; P (and dS in the backward) are rounded to dtype as operands of the second products.  No atomics:
+ * results do not depend on scheduling.
+ * Workspace osam_attn_workspace_size(desc) bytes (both directions), 256-byte aligned, any contents. */
+enum { OSAM_ATTN_NONE = 0, OSAM_ATTN_CAUSAL = 1, OSAM_ATTN_PREFIX = 2 };
+typedef struct osam_attn_desc {
+  int dtype, batch, len_q, len_k, heads_q, heads_k, dim;
+  int mask;             /* OSAM_ATTN_* */
+  float scale, cap;     /* scale > 0; cap 0: uncapped */
+  int grid_w;           /* 0: distance along the sequence */
+  const float* slopes;  /* [heads_q], device */
+  const int* lens;      /* [batch], device */
+  const int* prefix;    /* [batch], device; needed by OSAM_ATTN_PREFIX */
+  const int* doc_q;     /* device */
+  const int* doc_k;
+} osam_attn_desc;
+typedef struct osam_view {  /* element strides of batch, token and head */
+  void* p;
+  int64_t sb, st, sh;
+} osam_view;
+size_t osam_attn_workspace_size(const osam_attn_desc* a);
+int osam_attn_fwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v, osam_view o, float* lse, void* ws,
+                  size_t ws_bytes, osam_stream_t stream);
+/* dq, dk, dv (written) from the gradient dO of o:  dp_ij = do_i·v_j,  ds_ij = p_ij·(dp_ij − do_i·o_i),
+ * dq_i = scale·Σ_j ds_ij·(1 − t_ij²)·k_j (t = tanh of the capped score; 0 uncapped), dk likewise, dv_j = Σ_i
+ * p_ij do_i; the gradients of a shared key head are the sums over its query heads. */
+int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v, osam_view o, const float* lse,
+                  osam_view dout, osam_view dq, osam_view dk, osam_view dv, void* ws, size_t ws_bytes,
+                  osam_stream_t stream);
+
 /* Human-readable description of the last error returned on this host thread. */
 const char* osam_last_error(void);
 

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, byref, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, byref, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libosam.so")
@@ -64,6 +64,28 @@ class AugOut(ctypes.Structure):
     """osam_aug_out — ≙ AugOut + GtBatch (reference src/augment.cuh:11-17, src/loss.cuh:25-30)."""
     _fields_ = [("img", c_void_p), ("n_gt", c_void_p), ("box", c_void_p), ("mask", c_void_p), ("ignore", c_void_p),
                 ("gt_inst", c_void_p), ("G", c_int), ("Hp", c_int), ("Wp", c_int)]
+
+
+F16, BF16, F32 = range(3)
+ATTN_NONE, ATTN_CAUSAL, ATTN_PREFIX = range(3)
+
+
+class View(ctypes.Structure):
+    """osam_view — a [batch][token][head][dim] tensor by element strides."""
+    _fields_ = [("p", c_void_p), ("sb", c_int64), ("st", c_int64), ("sh", c_int64)]
+
+
+class AttnDesc(ctypes.Structure):
+    """osam_attn_desc."""
+    _fields_ = [(n, c_int) for n in ("dtype", "batch", "len_q", "len_k", "heads_q", "heads_k", "dim", "mask")] + \
+               [("scale", c_float), ("cap", c_float), ("grid_w", c_int)] + \
+               [(n, c_void_p) for n in ("slopes", "lens", "prefix", "doc_q", "doc_k")]
+
+
+class AdamWTensor(ctypes.Structure):
+    """osam_adamw_tensor."""
+    _fields_ = [("p", c_void_p), ("g", c_void_p), ("copy", c_void_p), ("n", c_int64), ("grad_type", c_int),
+                ("copy_type", c_int), ("decay", c_int)]
 
 
 # symbol → (restype, argtypes); every entry point of include/osam.h
@@ -144,6 +166,22 @@ _SIGS = {
     "osam_dp_backward": (c_int, [c_void_p, c_void_p]),
     "osam_dp_wait": (c_int, [c_void_p, c_int]),
     "osam_dp_destroy": (c_int, [c_void_p]),
+    "osam_rms_fwd": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_float, c_void_p,
+                             c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "osam_rms_fwd_q8": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_float,
+                                c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    "osam_rms_bwd_workspace_size": (c_size_t, [c_int]),
+    "osam_rms_bwd": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
+                             c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "osam_adamw_sizes": (c_int, [POINTER(AdamWTensor), c_int, c_int, POINTER(c_size_t), POINTER(c_int64)]),
+    "osam_adamw_create": (c_int, [POINTER(AdamWTensor), c_int, c_int, c_void_p, c_size_t, c_void_p, POINTER(c_void_p)]),
+    "osam_adamw_step": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_double, c_double, c_double,
+                                c_double, c_double, c_double, c_double, c_void_p, c_void_p]),
+    "osam_adamw_destroy": (c_int, [c_void_p]),
+    "osam_attn_workspace_size": (c_size_t, [POINTER(AttnDesc)]),
+    "osam_attn_fwd": (c_int, [POINTER(AttnDesc), View, View, View, View, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "osam_attn_bwd": (c_int, [POINTER(AttnDesc), View, View, View, View, c_void_p, View, View, View, View, c_void_p,
+                              c_size_t, c_void_p]),
     "osam_device_error": (c_int, []),
     "osam_device_error_peek": (c_int, []),
     "osam_selftest_wait_timeout": (c_int, [ctypes.c_ulonglong, c_void_p]),

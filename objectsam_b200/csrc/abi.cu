@@ -103,9 +103,9 @@ static PFN_encodeTiled_t encode_fn() {
   return fn;
 }
 
-// fp16 tensor map: dims[0] innermost, strides in bytes for dims 1..rank-1.
-static int make_map(CUtensorMap* tm, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_b,
-                    const uint32_t* box, int row_bytes) {
+// fp16 (or bf16) tensor map: dims[0] innermost, strides in bytes for dims 1..rank-1.
+int make_map(CUtensorMap* tm, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_b,
+             const uint32_t* box, int row_bytes, bool bf16) {
   PFN_encodeTiled_t fn = encode_fn();
   if (!fn) return fail(OSAM_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   if (reinterpret_cast<uintptr_t>(base) & 15) return fail(OSAM_ERR_INVALID, "operand not 16-byte aligned");
@@ -124,7 +124,7 @@ static int make_map(CUtensorMap* tm, const void* base, int rank, const uint64_t*
   const CUtensorMapSwizzle sw = row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
                                 : row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
                                                   : CU_TENSOR_MAP_SWIZZLE_NONE;
-  CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), gd, gs, bx, es,
+  CUresult r = fn(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), gd, gs, bx, es,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(OSAM_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d)", (int)r);

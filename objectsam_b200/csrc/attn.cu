@@ -1,0 +1,385 @@
+// Attention: the C entry points, argument checks and workspace layout, and the small kernels around the two main
+// ones (attn_fwd.cuh, attn_bwd.cuh): document summaries, the join of split keys, the backward's row terms.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "attn_bwd.cuh"
+
+namespace osam {
+namespace {
+
+// Per 64-token block: smallest and largest document id, and whether a token has none.  One warp per block; the
+// query blocks first, then the key blocks (`both`: the same array serves as both).
+__global__ void __launch_bounds__(256) k_attn_docs(const int* doc_q, const int* doc_k, int B, int Lq, int Lk, AtDocs* sq,
+                                                   AtDocs* sk) {
+  const int nq = (Lq + kAtDocBlock - 1) / kAtDocBlock, nk = (Lk + kAtDocBlock - 1) / kAtDocBlock;
+  const int w = (blockIdx.x * 256 + threadIdx.x) / 32, lane = threadIdx.x % 32;
+  const bool is_q = w < B * nq;
+  const int i = is_q ? w : w - B * nq, nb = is_q ? nq : nk, L = is_q ? Lq : Lk;
+  if (i >= B * nb) return;
+  const int b = i / nb, t0 = (i - b * nb) * kAtDocBlock;
+  const int* d = (is_q ? doc_q : doc_k) + (long long)b * L;
+  AtDocs s{INT_MAX, -1, 0, 0};
+#pragma unroll
+  for (int k = 0; k < kAtDocBlock; k += 32) {
+    const int t = t0 + k + lane;
+    if (t >= L) continue;
+    const int id = d[t];
+    if (id < 0) {
+      s.pad = 1;
+    } else {
+      s.lo = min(s.lo, id);
+      s.hi = max(s.hi, id);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s.lo = min(s.lo, __shfl_xor_sync(0xffffffffu, s.lo, o));
+    s.hi = max(s.hi, __shfl_xor_sync(0xffffffffu, s.hi, o));
+    s.pad |= __shfl_xor_sync(0xffffffffu, s.pad, o);
+  }
+  if (lane == 0) (is_q ? sq : sk)[i] = s;
+}
+
+// Joins the key splits: one warp per output row.  o = Σ 2^(m_s − M) o_s / Σ 2^(m_s − M) l_s over the splits, in
+// split order.
+template <typename T>
+__global__ void __launch_bounds__(256) k_attn_join(const float* part, const float2* stats, int splits, long long nrows,
+                                                   int Hq, int Lq, int D, AtView o, float* lse) {
+  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / 32;
+  const int lane = threadIdx.x % 32;
+  grid_dep_wait();
+  if (row >= nrows) return;
+  float M = -INFINITY;
+  for (int s = lane; s < splits; s += 32) M = fmaxf(M, stats[s * nrows + row].x);
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int s = 0; s < splits; s++) {
+    const float2 st = stats[s * nrows + row];
+    if (st.y == 0.f) continue;  // no key in this split
+    const float w = at_ex2(st.x - M);
+    l = fmaf(w, st.y, l);
+    if (lane * 4 < D) {
+      const float4 v = *reinterpret_cast<const float4*>(part + (s * nrows + row) * D + lane * 4);
+      acc.x = fmaf(w, v.x, acc.x);
+      acc.y = fmaf(w, v.y, acc.y);
+      acc.z = fmaf(w, v.z, acc.z);
+      acc.w = fmaf(w, v.w, acc.w);
+    }
+  }
+  const long long bh = row / Lq;
+  const int i = int(row - bh * Lq), h = int(bh % Hq);
+  const long long b = bh / Hq;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  if (lane * 4 < D) {
+    T* p = static_cast<T*>(o.p) + b * o.sb + i * o.st + h * o.sh + lane * 4;
+    *reinterpret_cast<uint2*>(p) =
+        make_uint2(Half16<T>::pack(acc.x * inv, acc.y * inv), Half16<T>::pack(acc.z * inv, acc.w * inv));
+  }
+  if (lane == 0 && lse) lse[row] = l == 0.f ? -INFINITY : (M + at_lg2(l)) * kAtLn2;
+}
+
+// Row terms of the backward pass, per 64-query block (padded to whole blocks): (lse·log2 e, δ = do·o) — (+∞, 0) for
+// queries that see nothing and for the padding, whose P is then 0 — and the block's largest |dO|.  One CTA per
+// block, 16 lanes per row (a 16-byte vector each).
+template <typename T>
+__global__ void __launch_bounds__(256) k_attn_rows(const AtView o, const AtView dout, const float* lse, int Hq, int Lq,
+                                                   int D, float2* rows, float* peak) {
+  __shared__ float top[8];
+  const int nb = (Lq + kAbCols - 1) / kAbCols;
+  const int blk = blockIdx.x % nb, h = (blockIdx.x / nb) % Hq, b = blockIdx.x / nb / Hq;
+  const int c = threadIdx.x % 16;
+  const long long bh = (long long)b * Hq + h;
+  float big = 0.f;
+#pragma unroll
+  for (int k = 0; k < kAbCols; k += 16) {
+    const int r = k + threadIdx.x / 16, i = blk * kAbCols + r;
+    const float L = i < Lq ? lse[bh * Lq + i] : -INFINITY;
+    const bool live = L != -INFINITY;
+    float d = 0.f;
+    if (live && c * 8 < D) {
+      float a[8], g[8];
+      unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(o.p) + b * o.sb + i * o.st + h * o.sh + c * 8), a);
+      unpack8<T>(
+          *reinterpret_cast<const uint4*>(static_cast<const T*>(dout.p) + b * dout.sb + i * dout.st + h * dout.sh + c * 8), g);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        d = fmaf(a[e], g[e], d);
+        big = fmaxf(big, fabsf(g[e]));
+      }
+    }
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
+    if (c == 0) rows[(bh * nb + blk) * kAbCols + r] = make_float2(live ? L * kAtLog2e : INFINITY, live ? d : 0.f);
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
+  if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = big;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; w++) big = fmaxf(big, top[w]);
+    peak[bh * nb + blk] = big;
+  }
+}
+
+int at_fail(int code, const char* what) {
+  set_last_error("attention: %s", what);
+  return code;
+}
+int at_cuda(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return OSAM_OK;
+  set_last_error("attention: %s: %s", what, cudaGetErrorString(e));
+  return OSAM_ERR_CUDA;
+}
+
+int at_check(const osam_attn_desc* a) {
+  if (!a) return at_fail(OSAM_ERR_INVALID, "null description");
+  if (a->dtype != OSAM_F16 && a->dtype != OSAM_BF16) return at_fail(OSAM_ERR_INVALID, "dtype is OSAM_F16 or OSAM_BF16");
+  if (a->batch < 0 || a->len_q < 0 || a->len_k < 0 || a->heads_q < 1 || a->heads_k < 1 || a->heads_q % a->heads_k)
+    return at_fail(OSAM_ERR_INVALID, "lengths ≥ 0 and heads_q a multiple of heads_k");
+  if (a->dim < 8 || a->dim > 128 || a->dim % 8) return at_fail(OSAM_ERR_INVALID, "dim is a multiple of 8 up to 128");
+  if (!(a->scale > 0.f) || std::isinf(a->scale)) return at_fail(OSAM_ERR_INVALID, "scale is positive and finite");
+  if (!(a->cap >= 0.f) || std::isinf(a->cap)) return at_fail(OSAM_ERR_INVALID, "cap is 0 or positive and finite");
+  if (a->mask != OSAM_ATTN_NONE && a->mask != OSAM_ATTN_CAUSAL && a->mask != OSAM_ATTN_PREFIX)
+    return at_fail(OSAM_ERR_INVALID, "unknown mask");
+  if (a->mask == OSAM_ATTN_PREFIX && !a->prefix) return at_fail(OSAM_ERR_INVALID, "a prefix mask needs prefix lengths");
+  if ((a->doc_q == nullptr) != (a->doc_k == nullptr)) return at_fail(OSAM_ERR_INVALID, "doc_q and doc_k come together");
+  if (a->grid_w < 0) return at_fail(OSAM_ERR_INVALID, "grid_w is not negative");
+  const long long most = 1LL << 30;
+  if ((long long)a->len_q * (a->heads_q / a->heads_k) > most || a->len_k > most ||
+      (long long)a->batch * a->heads_q * ((a->len_q + 63) / 64) > most ||
+      (long long)a->batch * a->heads_k * ((a->len_k + 63) / 64) > most)
+    return at_fail(OSAM_ERR_INVALID, "too many tokens");
+  if (a->doc_q && (a->len_q > 1048576 || a->len_k > 1048576))
+    return at_fail(OSAM_ERR_INVALID, "with documents at most 1048576 tokens");
+  return OSAM_OK;
+}
+
+int at_view_check(const osam_view& v, int batch, int len, int heads, const char* name) {
+  if (!v.p || (reinterpret_cast<uintptr_t>(v.p) & 15)) {
+    set_last_error("attention: %s is null or not 16-byte aligned", name);
+    return OSAM_ERR_INVALID;
+  }
+  const int64_t s[3] = {v.sb, v.st, v.sh};
+  const int n[3] = {batch, len, heads};
+  for (int i = 0; i < 3; i++)
+    if (n[i] > 1 && (s[i] <= 0 || s[i] % 8 || s[i] >= (1LL << 38))) {
+      set_last_error("attention: %s has a stride that is not a positive multiple of 8 elements", name);
+      return OSAM_ERR_INVALID;
+    }
+  return OSAM_OK;
+}
+
+AtView at_view(const osam_view& v) { return AtView{v.p, v.sb, v.st, v.sh}; }
+
+// (dim, token, head, batch) map with boxes of 64 dims × `rows` tokens.
+int at_map(CUtensorMap* tm, const osam_view& v, int batch, int len, int heads, int dim, int rows, bool bf16) {
+  const uint64_t dims[4] = {(uint64_t)dim, (uint64_t)len, (uint64_t)heads, (uint64_t)batch};
+  const uint64_t st[3] = {len > 1 ? (uint64_t)v.st * 2 : 16, heads > 1 ? (uint64_t)v.sh * 2 : 16,
+                          batch > 1 ? (uint64_t)v.sb * 2 : 16};
+  const uint32_t box[4] = {64, (uint32_t)rows, 1, 1};
+  return make_map(tm, v.p, 4, dims, st, box, 128, bf16);
+}
+
+// How the keys are split: nothing to gain once the query tiles fill the GPU.
+struct AtSplit {
+  int splits, tiles;
+};
+AtSplit at_split(const osam_attn_desc& a) {
+  const int tiles = (a.len_k + 127) / 128;
+  const long long ctas = (((long long)a.len_q * (a.heads_q / a.heads_k) + 127) / 128) * a.batch * a.heads_k;
+  AtSplit s{1, std::max(tiles, 1)};
+  if (ctas == 0 || tiles < 4 || ctas >= 2 * kAtSms) return s;
+  const int want = (int)std::min<long long>((4LL * kAtSms + ctas - 1) / ctas, tiles / 2);
+  s.tiles = (tiles + want - 1) / want;
+  s.splits = (tiles + s.tiles - 1) / s.tiles;
+  return s;
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Workspace: document summaries | split outputs and statistics (forward) or row terms (backward).
+struct AtLayout {
+  size_t sum_q = 0, sum_k = 0, part = 0, stats = 0, rows = 0, peak = 0, bytes = 0;
+};
+AtLayout at_layout(const osam_attn_desc& a) {
+  AtLayout L;
+  size_t at = 0;
+  if (a.doc_q) {
+    L.sum_q = at;
+    at += up256((size_t)a.batch * ((a.len_q + 63) / 64) * sizeof(AtDocs));
+    L.sum_k = at;
+    at += up256((size_t)a.batch * ((a.len_k + 63) / 64) * sizeof(AtDocs));
+  }
+  const size_t rows = (size_t)a.batch * a.heads_q * a.len_q;
+  const AtSplit s = at_split(a);
+  L.part = L.rows = at;
+  size_t fwd = at;
+  if (s.splits > 1) {
+    fwd += up256(rows * s.splits * a.dim * sizeof(float));
+    L.stats = fwd;
+    fwd += up256(rows * s.splits * sizeof(float2));
+  }
+  const size_t blocks = (size_t)a.batch * a.heads_q * ((a.len_q + kAbCols - 1) / kAbCols);
+  L.peak = at + up256(blocks * kAbCols * sizeof(float2));
+  L.bytes = std::max(fwd, L.peak + up256(blocks * sizeof(float)));
+  return L;
+}
+
+int at_dev(const osam_attn_desc& a, const AtLayout& W, char* ws, AttnDev* A, cudaStream_t st) {
+  A->B = a.batch; A->Lq = a.len_q; A->Lk = a.len_k; A->Hq = a.heads_q; A->Hk = a.heads_k;
+  A->G = a.heads_q / a.heads_k; A->D = a.dim;
+  A->mask = a.mask; A->scale = a.scale; A->cap = a.cap;
+  A->grid_w = a.grid_w;
+  A->f_w.set(a.grid_w);
+  A->lens = a.lens; A->prefix = a.prefix; A->doc_q = a.doc_q; A->doc_k = a.doc_k; A->slopes = a.slopes;
+  A->err = device_error_word();
+  if (!A->err) return at_fail(OSAM_ERR_CUDA, "no device error word");
+  if (a.doc_q) {
+    AtDocs* sq = reinterpret_cast<AtDocs*>(ws + W.sum_q);
+    AtDocs* sk = reinterpret_cast<AtDocs*>(ws + W.sum_k);
+    A->sum_q = sq;
+    A->sum_k = sk;
+    const long long warps = (long long)a.batch * ((a.len_q + 63) / 64 + (a.len_k + 63) / 64);
+    k_attn_docs<<<(unsigned)((warps + 7) / 8), 256, 0, st>>>(a.doc_q, a.doc_k, a.batch, a.len_q, a.len_k, sq, sk);
+    return at_cuda(cudaGetLastError(), "document summaries");
+  }
+  return OSAM_OK;
+}
+
+cudaError_t launch_dependent(const void* k, unsigned grid, unsigned threads, void** args, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelExC(&cfg, k, args);
+}
+
+}  // namespace
+}  // namespace osam
+
+using namespace osam;
+
+extern "C" {
+
+size_t osam_attn_workspace_size(const osam_attn_desc* a) { return at_check(a) == OSAM_OK ? at_layout(*a).bytes : 0; }
+
+int osam_attn_fwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v, osam_view o, float* lse, void* ws,
+                  size_t ws_bytes, osam_stream_t stream) {
+  int rc = at_check(a);
+  if (rc != OSAM_OK) return rc;
+  if (a->batch == 0 || a->len_q == 0) return OSAM_OK;
+  if ((rc = at_view_check(q, a->batch, a->len_q, a->heads_q, "q")) != OSAM_OK ||
+      (rc = at_view_check(o, a->batch, a->len_q, a->heads_q, "o")) != OSAM_OK)
+    return rc;
+  if (a->len_k > 0 && ((rc = at_view_check(k, a->batch, a->len_k, a->heads_k, "k")) != OSAM_OK ||
+                       (rc = at_view_check(v, a->batch, a->len_k, a->heads_k, "v")) != OSAM_OK))
+    return rc;
+  const AtLayout W = at_layout(*a);
+  if (W.bytes && (!ws || ws_bytes < W.bytes || (reinterpret_cast<uintptr_t>(ws) & 255)))
+    return at_fail(OSAM_ERR_INVALID, "workspace (osam_attn_workspace_size, 256-byte aligned)");
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  char* w = static_cast<char*>(ws);
+  const AtSplit s = at_split(*a);
+  AttnFwdLaunch L{};
+  if ((rc = at_dev(*a, W, w, &L.d, st)) != OSAM_OK) return rc;
+  const bool bf16 = a->dtype == OSAM_BF16;
+  // without keys every query is empty: no tile is visited, so the maps only have to be valid
+  const osam_view& kk = a->len_k > 0 ? k : q;
+  const osam_view& vv = a->len_k > 0 ? v : q;
+  if ((rc = at_map(&L.tk, kk, a->batch, std::max(a->len_k, 1), a->heads_k, a->dim, 128, bf16)) != OSAM_OK ||
+      (rc = at_map(&L.tv, vv, a->batch, std::max(a->len_k, 1), a->heads_k, a->dim, 128, bf16)) != OSAM_OK)
+    return rc;
+  L.q = at_view(q);
+  L.o = at_view(o);
+  L.lse = lse;
+  L.splits = s.splits;
+  L.tiles_per_split = s.tiles;
+  L.part = reinterpret_cast<float*>(w + W.part);
+  L.stats = reinterpret_cast<float2*>(w + W.stats);
+  cudaError_t e = bf16 ? launch_attn_fwd<__nv_bfloat16>(L, st) : launch_attn_fwd<__half>(L, st);
+  if (e != cudaSuccess || s.splits == 1) return at_cuda(e, "forward launch");
+  long long nrows = (long long)a->batch * a->heads_q * a->len_q;
+  const float* part = L.part;
+  const float2* stats = L.stats;
+  int splits = s.splits, Hq = a->heads_q, Lq = a->len_q, D = a->dim;
+  void* args[] = {&part, &stats, &splits, &nrows, &Hq, &Lq, &D, &L.o, &lse};
+  const void* join = bf16 ? (const void*)k_attn_join<__nv_bfloat16> : (const void*)k_attn_join<__half>;
+  return at_cuda(launch_dependent(join, (unsigned)((nrows + 7) / 8), 256, args, st), "join launch");
+}
+
+int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v, osam_view o, const float* lse,
+                  osam_view dout, osam_view dq, osam_view dk, osam_view dv, void* ws, size_t ws_bytes,
+                  osam_stream_t stream) {
+  int rc = at_check(a);
+  if (rc != OSAM_OK) return rc;
+  if (a->batch == 0 || (a->len_q == 0 && a->len_k == 0)) return OSAM_OK;
+  if (a->len_q > 0) {
+    const osam_view* t[] = {&q, &o, &dout, &dq};
+    const char* name[] = {"q", "o", "dout", "dq"};
+    for (int i = 0; i < 4; i++)
+      if ((rc = at_view_check(*t[i], a->batch, a->len_q, a->heads_q, name[i])) != OSAM_OK) return rc;
+    if (!lse) return at_fail(OSAM_ERR_INVALID, "the backward pass needs the forward's lse");
+  }
+  if (a->len_k > 0) {
+    const osam_view* t[] = {&k, &v, &dk, &dv};
+    const char* name[] = {"k", "v", "dk", "dv"};
+    for (int i = 0; i < 4; i++)
+      if ((rc = at_view_check(*t[i], a->batch, a->len_k, a->heads_k, name[i])) != OSAM_OK) return rc;
+  }
+  const AtLayout W = at_layout(*a);
+  if (W.bytes && (!ws || ws_bytes < W.bytes || (reinterpret_cast<uintptr_t>(ws) & 255)))
+    return at_fail(OSAM_ERR_INVALID, "workspace (osam_attn_workspace_size, 256-byte aligned)");
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  char* w = static_cast<char*>(ws);
+  const bool bf16 = a->dtype == OSAM_BF16;
+  AttnBwdLaunch L{};
+  if ((rc = at_dev(*a, W, w, &L.d, st)) != OSAM_OK) return rc;
+  float2* rows = reinterpret_cast<float2*>(w + W.rows);
+  float* peak = reinterpret_cast<float*>(w + W.peak);
+  const int blocks = a->batch * a->heads_q * ((a->len_q + kAbCols - 1) / kAbCols);
+  if (blocks > 0) {
+    if (bf16)
+      k_attn_rows<__nv_bfloat16><<<blocks, 256, 0, st>>>(at_view(o), at_view(dout), lse, a->heads_q, a->len_q, a->dim, rows, peak);
+    else
+      k_attn_rows<__half><<<blocks, 256, 0, st>>>(at_view(o), at_view(dout), lse, a->heads_q, a->len_q, a->dim, rows, peak);
+    if ((rc = at_cuda(cudaGetLastError(), "row terms")) != OSAM_OK) return rc;
+  }
+  L.rows = rows;
+  L.peak = peak;
+  // a side of length 0 is never visited: its maps only have to be valid
+  const bool eq = a->len_q == 0, ek = a->len_k == 0;
+  const osam_view &vq = eq ? k : q, &vdo = eq ? k : dout, &vk = ek ? q : k, &vv = ek ? q : v;
+  const int lq = eq ? 1 : a->len_q, lk = ek ? 1 : a->len_k, hq = eq ? a->heads_k : a->heads_q;
+  auto map = [&](CUtensorMap* m, const osam_view& t, bool query, int box) {
+    return at_map(m, t, a->batch, query ? lq : lk, query ? hq : a->heads_k, a->dim, box, bf16);
+  };
+  if (!ek) {
+    if ((rc = map(&L.stat1, vk, false, kAbRows)) != OSAM_OK || (rc = map(&L.stat2, vv, false, kAbRows)) != OSAM_OK ||
+        (rc = map(&L.strm1, vq, true, kAbCols)) != OSAM_OK || (rc = map(&L.strm2, vdo, true, kAbCols)) != OSAM_OK)
+      return rc;
+    L.out1 = at_view(dk);
+    L.out2 = at_view(dv);
+    const cudaError_t e = bf16 ? launch_attn_bwd<__nv_bfloat16, true>(L, st) : launch_attn_bwd<__half, true>(L, st);
+    if (e != cudaSuccess) return at_cuda(e, "backward launch (dK, dV)");
+  }
+  if (!eq) {
+    if ((rc = map(&L.stat1, vq, true, kAbRows)) != OSAM_OK || (rc = map(&L.stat2, vdo, true, kAbRows)) != OSAM_OK ||
+        (rc = map(&L.strm1, vk, false, kAbCols)) != OSAM_OK || (rc = map(&L.strm2, vv, false, kAbCols)) != OSAM_OK)
+      return rc;
+    L.out1 = at_view(dq);
+    const cudaError_t e = bf16 ? launch_attn_bwd<__nv_bfloat16, false>(L, st) : launch_attn_bwd<__half, false>(L, st);
+    if (e != cudaSuccess) return at_cuda(e, "backward launch (dQ)");
+  }
+  return OSAM_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,479 @@
+// Attention backward (see attn.cuh): one kernel in two forms.  Each CTA keeps 128 rows of one side in shared memory
+// and streams 64-row tiles of the other:
+//   DKV: 128 keys of a key head stay (K, V), the queries of every head of the group stream (Q, dO):
+//        dV += Pᵀ·dO, dK += dSᵀ·Q — the sum over a shared key head's query heads is this accumulation
+//   DQ : 128 queries of one head stay (Q, dO), the keys stream (K, V):  dQ += dS·K
+// Two passes compute S and dP twice (7 products instead of 5) but every sum is taken by one CTA in one order: no
+// atomics, no fp32 copy of dQ, results that do not depend on scheduling.
+//
+// Per tile, rows = the stationary side (TMEM lanes), columns = the streamed side:
+//   X = stat1·strm1ᵀ (scores), Y = stat2·strm2ᵀ (dP), both fp32 in TMEM
+//   one thread per row: p = 2^(x − lse), ds = p·(dp − δ)·(1 − t²), both back to TMEM in 16 bits over X and Y
+//   acc2 += P·strm2 (DKV), acc1 += dS·strm1, P and dS as TMEM operands
+// fp16 keeps its precision over long rows and small gradients by powers of two: P is held times 2^8 and dS times
+// 2^8·F with F = 2^−e, e the exponent of the largest |dO| (of the key head's group for DKV, of the row's block for
+// DQ), both taken back in fp32 at the end; bf16 needs neither.
+// Warps: 4 per buffer of (X, Y) for the element-wise part, then the TMA producer and the MMA issuer.  Up to 64 head
+// dims one buffer and 256 TMEM columns, two CTAs per SM; above, two buffers in one CTA with all 512 columns: the
+// tensor cores work on one while the other is in the element-wise part.
+#pragma once
+#include "attn.cuh"
+
+namespace osam {
+
+constexpr int kAbRows = 128, kAbCols = 64;
+
+struct AttnBwdLaunch {
+  AttnDev d;
+  CUtensorMap stat1, stat2, strm1, strm2;
+  AtView out1, out2;      // dK, dV (DKV); dQ (DQ)
+  const float2* rows;     // [B][Hq][⌈Lq/64⌉·64] (lse·log2 e, or +∞ where the query is empty; δ)
+  const float* peak;      // [B][Hq][⌈Lq/64⌉] max |dO| of the block
+};
+template <typename T, bool DKV>
+cudaError_t launch_attn_bwd(const AttnBwdLaunch& L, cudaStream_t st);
+
+template <int DP>
+struct AbCfg {
+  static constexpr int PANELS = DP / 64;
+  static constexpr int NB = DP == 64 ? 1 : 2;   // (X, Y) buffers = warpgroups
+  static constexpr int CTAS = DP == 64 ? 2 : 1; // per SM
+  static constexpr int STAGES = 4;
+  static constexpr int STAT = PANELS * kAbRows * 128;  // bytes of one stationary operand
+  static constexpr int STRM = PANELS * kAbCols * 128;  // bytes of one streamed operand
+  static constexpr int ROWS = kAbCols * 8;             // (lse, δ) of a query tile
+  static constexpr int SMEM = 1024 + 2 * STAT + STAGES * (2 * STRM + ROWS);
+  static constexpr int TMEM = DP == 64 ? 256 : 512;
+  static constexpr int COL_ACC1 = 128 * NB, COL_ACC2 = COL_ACC1 + DP;
+  static constexpr int THREADS = 128 * NB + 64;
+};
+
+// Visits (head of the group, tile) pairs, heads outermost.
+struct AbIter {
+  int g, t;
+  __device__ __forceinline__ void start(const AtTiles& T) {
+    g = 0;
+    t = T.first();
+  }
+  __device__ __forceinline__ bool more(const AtTiles& T, int heads) const { return g < heads && t < T.end; }
+  __device__ __forceinline__ void step(const AtTiles& T) {
+    t = T.next(t + 1);
+    if (t >= T.end) {
+      g++;
+      t = T.first();
+    }
+  }
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <typename T, int DP, bool DKV, bool CAP, int BIAS>
+__global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
+    k_attn_bwd(const __grid_constant__ AttnBwdLaunch P) {
+  using Cfg = AbCfg<DP>;
+  constexpr bool BF16 = Half16<T>::kBf16;
+  constexpr int NB = Cfg::NB;
+  extern __shared__ uint8_t ab_raw[];
+  __shared__ __align__(8) uint64_t stat_full, full[Cfg::STAGES], empty[Cfg::STAGES], xy_full[NB], ds_full[NB], acc_done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t live[kAtDocWords], mix[kAtDocWords], pad[kAtDocWords];
+  __shared__ __align__(16) int col_doc[NB][2][kAbCols];
+  __shared__ __align__(16) float2 col_cell[NB][BIAS == 2 ? 2 : 1][kAbCols];
+
+  const AttnDev& A = P.d;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  uint8_t* smem = ab_raw + ((1024 - (smem_u32(ab_raw) & 1023)) & 1023);
+  uint8_t* strm = smem + 2 * Cfg::STAT;
+  uint8_t* srows = strm + Cfg::STAGES * 2 * Cfg::STRM;
+
+  // ---- which tile (with a causal bound the longest first)
+  const int heads = DKV ? A.Hk : A.Hq, nt = ((DKV ? A.Lk : A.Lq) + kAbRows - 1) / kAbRows;
+  const int per = A.B * heads;
+  int rt, rest;
+  if (A.mask == OSAM_ATTN_NONE) {
+    rt = int(blockIdx.x) % nt;
+    rest = int(blockIdx.x) / nt;
+  } else {
+    rt = int(blockIdx.x) / per;
+    rest = int(blockIdx.x) % per;
+    if (!DKV) rt = nt - 1 - rt;
+  }
+  const int hd = rest % heads, b = rest / heads;
+  const int row0 = rt * kAbRows;
+  const int n = at_keys(A, b), off = n - A.Lq;
+  const int prefix = A.mask == OSAM_ATTN_PREFIX ? A.prefix[b] : 0;
+  const int nq64 = (A.Lq + kAbCols - 1) / kAbCols, nk64 = (A.Lk + kAbCols - 1) / kAbCols;
+  const bool causal = A.mask != OSAM_ATTN_NONE;
+  const int streams = DKV ? A.G : 1;  // query heads that stream past
+  AtTiles tiles;
+  int lim_min = 0;  // DQ: bound of the tile's first query
+  if (DKV) {  // queries from the first that sees key row0
+    tiles.begin = causal && prefix <= row0 ? max(0, row0 - off) / kAbCols : 0;
+    tiles.end = row0 < n ? nq64 : tiles.begin;
+    tiles.begin = min(tiles.begin, tiles.end);
+  } else {
+    const int last = min(row0 + kAbRows, A.Lq) - 1;
+    tiles.begin = 0;
+    tiles.end = (at_limit(A, n, prefix, off + last) + kAbCols - 1) / kAbCols;
+    lim_min = at_limit(A, n, prefix, off + row0);
+  }
+  const bool docs = A.doc_q != nullptr;
+  tiles.live = docs ? live : nullptr;
+
+  if (tid == 0) {
+    mbar_init(&stat_full, 1);
+    for (int i = 0; i < Cfg::STAGES; i++) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < NB; i++) {
+      mbar_init(&xy_full[i], 1);
+      mbar_init(&ds_full[i], 4);
+    }
+    mbar_init(&acc_done, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&P.stat1);
+    tma_prefetch_desc(&P.stat2);
+    tma_prefetch_desc(&P.strm1);
+    tma_prefetch_desc(&P.strm2);
+  }
+  if (warp == 4 * NB + 1) {
+    tmem_alloc(&tmem_slot, Cfg::TMEM);
+    tmem_relinquish();
+  }
+  if (docs) {
+    const AtDocs* sq = A.sum_q + (long long)b * nq64;
+    const AtDocs* sk = A.sum_k + (long long)b * nk64;
+    const AtDocs own = at_docs(DKV ? sk : sq, rt * 2, 2, DKV ? nk64 : nq64);
+    at_doc_bits(own, DKV ? sq : sk, DKV ? nq64 : nk64, 1, tiles.begin, tiles.end, warp, Cfg::THREADS / 32, live, mix, pad);
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 4 * NB) {
+    if (lane == 0) {
+      AbIter x;
+      x.start(tiles);
+      const bool any = x.more(tiles, streams);
+      if (any) {
+        mbar_arrive_expect_tx(&stat_full, 2 * Cfg::STAT);
+        for (int p = 0; p < Cfg::PANELS; p++) {
+          tma_load_4d(smem + p * kAbRows * 128, &P.stat1, &stat_full, p * 64, row0, hd, b);
+          tma_load_4d(smem + Cfg::STAT + p * kAbRows * 128, &P.stat2, &stat_full, p * 64, row0, hd, b);
+        }
+      }
+      int it = 0;
+      for (; x.more(tiles, streams); x.step(tiles), it++) {
+        const int s = it % Cfg::STAGES;
+        if (it >= Cfg::STAGES && !mbar_wait(&empty[s], ((it / Cfg::STAGES) & 1) ^ 1, A.err)) break;
+        uint8_t* d = strm + s * 2 * Cfg::STRM;
+        mbar_arrive_expect_tx(&full[s], 2 * Cfg::STRM + (DKV ? Cfg::ROWS : 0));
+        const int h = DKV ? hd * A.G + x.g : hd / A.G;
+        for (int p = 0; p < Cfg::PANELS; p++) {
+          tma_load_4d(d + p * kAbCols * 128, &P.strm1, &full[s], p * 64, x.t * kAbCols, h, b);
+          tma_load_4d(d + Cfg::STRM + p * kAbCols * 128, &P.strm2, &full[s], p * 64, x.t * kAbCols, h, b);
+        }
+        if (DKV)
+          bulk_load(srows + s * Cfg::ROWS, P.rows + (((long long)b * A.Hq + h) * nq64 + x.t) * kAbCols, Cfg::ROWS,
+                    &full[s]);
+      }
+      // no copy of this CTA may be in flight when it ends
+      if (any) mbar_wait(&stat_full, 0, A.err);
+      for (int i = max(0, it - Cfg::STAGES); i < it; i++) mbar_wait(&full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, A.err);
+    }
+    __syncwarp();
+  } else if (warp == 4 * NB + 1) {
+    if (lane == 0) {
+      const int ks = (A.D + 15) / 16;
+      const uint32_t id_x = at_idesc(BF16, 128, kAbCols, false), id_g = at_idesc(BF16, 128, 16 * ks, true);
+      const uint32_t a1 = smem_u32(smem), a2 = a1 + Cfg::STAT, sb = smem_u32(strm);
+      // X and Y of streamed tile `it`
+      auto scores = [&](int it) {
+        const uint32_t b1 = sb + (it % Cfg::STAGES) * 2 * Cfg::STRM, b2 = b1 + Cfg::STRM;
+        const uint32_t d = tmem + (it % NB) * 128;
+        for (int k = 0; k < ks; k++) {
+          const uint32_t oa = (k / 4) * kAbRows * 128 + (k % 4) * 32, ob = (k / 4) * kAbCols * 128 + (k % 4) * 32;
+          umma_f16(d, smem_desc_kmajor(a1 + oa, 128), smem_desc_kmajor(b1 + ob, 128), id_x, k > 0);
+        }
+        for (int k = 0; k < ks; k++) {
+          const uint32_t oa = (k / 4) * kAbRows * 128 + (k % 4) * 32, ob = (k / 4) * kAbCols * 128 + (k % 4) * 32;
+          umma_f16(d + 64, smem_desc_kmajor(a2 + oa, 128), smem_desc_kmajor(b2 + ob, 128), id_x, k > 0);
+        }
+        umma_commit(&xy_full[it % NB]);
+      };
+      AbIter ahead, x;  // `ahead` runs NB tiles in front
+      ahead.start(tiles);
+      x.start(tiles);
+      bool ok = !x.more(tiles, streams) || mbar_wait(&stat_full, 0, A.err);
+      int ia = 0;
+      for (; ok && ia < NB && ahead.more(tiles, streams); ahead.step(tiles), ia++) {
+        ok = mbar_wait(&full[ia % Cfg::STAGES], (ia / Cfg::STAGES) & 1, A.err);
+        if (!ok) break;
+        tc_fence_after();
+        scores(ia);
+      }
+      int it = 0;
+      for (; ok && x.more(tiles, streams); x.step(tiles), it++) {
+        const int s = it % Cfg::STAGES, buf = it % NB;
+        if (!(ok = mbar_wait(&ds_full[buf], (it / NB) & 1, A.err))) break;
+        tc_fence_after();
+        const uint32_t b1 = sb + s * 2 * Cfg::STRM, b2 = b1 + Cfg::STRM, d = tmem + buf * 128;
+        if (DKV) {
+#pragma unroll
+          for (int k = 0; k < kAbCols / 16; k++)
+            umma_f16_ts(tmem + Cfg::COL_ACC2, d + k * 8, at_desc_mn(b2 + k * 16 * 128, kAbCols * 128), id_g, (it | k) != 0);
+        }
+#pragma unroll
+        for (int k = 0; k < kAbCols / 16; k++)
+          umma_f16_ts(tmem + Cfg::COL_ACC1, d + 64 + k * 8, at_desc_mn(b1 + k * 16 * 128, kAbCols * 128), id_g,
+                      (it | k) != 0);
+        umma_commit(&empty[s]);
+        if (ahead.more(tiles, streams)) {
+          if (!(ok = mbar_wait(&full[ia % Cfg::STAGES], (ia / Cfg::STAGES) & 1, A.err))) break;
+          tc_fence_after();
+          scores(ia);
+          ahead.step(tiles);
+          ia++;
+        }
+      }
+      umma_commit(&acc_done);
+      if (!ok) mbar_wait(&acc_done, 0, A.err);  // the issued MMAs finish before TMEM is freed
+    }
+    __syncwarp();
+  } else {
+    const int wg = warp / 4, r = tid % 128;
+    const uint32_t lane_base = uint32_t((warp % 4) * 32) << 16;
+    const int row = row0 + r;
+    const bool valid = row < (DKV ? A.Lk : A.Lq);
+    // ---- what this thread's row is: a key (DKV) or a query (DQ)
+    const int pos = DKV ? row : off + row;
+    int my_doc = -2;
+    if (docs && valid) {
+      my_doc = (DKV ? A.doc_k : A.doc_q)[(long long)b * (DKV ? A.Lk : A.Lq) + row];
+      if (my_doc < 0) my_doc = -2;
+    }
+    // DKV: queries from `from` on see the key; DQ: keys below `lim` are seen
+    const int from = row >= n ? INT_MAX : (!causal || prefix > row ? 0 : row - off);
+    const int lim = !DKV && valid ? at_limit(A, n, prefix, pos) : 0;
+    const float2 cell = BIAS == 2 ? at_cell(A, pos) : make_float2(0.f, 0.f);
+    float F = 1.f;  // power of two that brings the largest |dO| to [1, 2)
+    if (!BF16) {
+      float peak = 0.f;
+      if (DKV) {
+        const float* pk = P.peak + ((long long)b * A.Hq + hd * A.G) * nq64;
+        for (int i = lane; i < A.G * nq64; i += 32) peak = fmaxf(peak, pk[i]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+      } else if (valid) {
+        peak = P.peak[((long long)b * A.Hq + hd) * nq64 + row / kAbCols];
+      }
+      const int e = (__float_as_int(peak) >> 23) & 255;
+      if (peak > 0.f && e < 255) F = __int_as_float(min(227, max(27, 254 - e)) << 23);  // at most 2^±100
+    }
+    constexpr float kUp = BF16 ? 0.f : 8.f;  // log2 of P's factor
+    float row_lse = 0.f, row_delta = 0.f;
+    if (!DKV) {
+      const float2 v = valid ? P.rows[((long long)b * A.Hq + hd) * nq64 * kAbCols + row] : make_float2(INFINITY, 0.f);
+      row_lse = kUp - v.x;
+      row_delta = -v.y;
+    }
+    const float cmul = CAP ? 2.f * A.scale * kAtLog2e / A.cap : A.scale * kAtLog2e, cap2 = A.cap * kAtLog2e;
+    float slope = 0.f;
+    int slope_of = -1;
+    AbIter x;
+    x.start(tiles);
+    bool ok = true;
+    int it = 0, tile = 0;
+    for (; x.more(tiles, streams); x.step(tiles), it++) {
+      if (NB > 1 && it % NB != wg) continue;
+      const int c0 = x.t * kAbCols;  // first column: query (DKV) or key (DQ)
+      const int h = DKV ? hd * A.G + x.g : hd;
+      if (BIAS && slope_of != h) {
+        slope = A.slopes[h] * kAtLog2e;
+        slope_of = h;
+      }
+      const bool by_doc = docs && at_bit(mix, x.t - tiles.begin);
+      const bool has_pad = docs && at_bit(pad, x.t - tiles.begin);
+      const bool by_lim = DKV ? row0 + kAbRows > n || (causal && prefix < row0 + kAbRows && c0 < row0 + kAbRows - 1 - off)
+                              : c0 + kAbCols > lim_min;
+      const int slot = tile & 1;
+      if (by_doc || BIAS == 2) {
+        if (r < kAbCols) {
+          if (docs) {
+            const int c = c0 + r, L = DKV ? A.Lq : n;
+            const int id = c < L ? (DKV ? A.doc_q : A.doc_k)[(long long)b * (DKV ? A.Lq : A.Lk) + c] : -1;
+            col_doc[wg][slot][r] = id < 0 ? -1 : id;
+          }
+          if (BIAS == 2) col_cell[wg][slot][r] = at_cell(A, DKV ? off + c0 + r : c0 + r);
+        }
+        named_bar_sync(1 + wg, 128);
+      }
+      if (!(ok = at_wait_warp(&xy_full[it % NB], (it / NB) & 1, A.err))) break;
+      tc_fence_after();
+      const int s = it % Cfg::STAGES;
+      const float4* rows2 = reinterpret_cast<const float4*>(srows + s * Cfg::ROWS);
+      if (DKV) {  // written by the bulk copy that this barrier counts
+        if (!(ok = at_wait_warp(&full[s], (it / Cfg::STAGES) & 1, A.err))) break;
+      }
+      const float rel = float(pos - (DKV ? off + c0 : c0));
+      const uint32_t xcol = tmem + lane_base + (it % NB) * 128;
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        float sv[32], dp[32];
+        tmem_ld32_nowait(xcol + half * 32, sv);
+        tmem_ld32_nowait(xcol + 64 + half * 32, dp);
+        tmem_wait_ld();
+        uint32_t pp[16], dd[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int c = half * 32 + 2 * i;
+          float2 v = make_float2(sv[2 * i], sv[2 * i + 1]);
+          float2 add, del;  // kUp − lse and −δ of the pair
+          if (DKV) {
+            const float4 q2 = rows2[c / 2];
+            add = make_float2(kUp - q2.x, kUp - q2.z);
+            del = make_float2(-q2.y, -q2.w);
+          } else {
+            add = make_float2(row_lse, row_lse);
+            del = make_float2(row_delta, row_delta);
+          }
+          float2 g = make_float2(1.f, 1.f);  // 1 − t²
+          if (CAP) {
+            const float2 rc = make_float2(at_rcp(1.f + at_ex2(v.x * cmul)), at_rcp(1.f + at_ex2(v.y * cmul)));
+            v = make_float2(fmaf(-2.f * cap2, rc.x, cap2), fmaf(-2.f * cap2, rc.y, cap2));
+            g = make_float2(4.f * rc.x * (1.f - rc.x), 4.f * rc.y * (1.f - rc.y));
+          }
+          if (BIAS) {
+            float2 far;
+            if (BIAS == 1) {
+              far = make_float2(fabsf(rel - float(c)), fabsf(rel - float(c + 1)));
+            } else {
+              const float4 k2 = reinterpret_cast<const float4*>(col_cell[wg][slot])[c / 2];
+              far = make_float2(fabsf(cell.x - k2.x) + fabsf(cell.y - k2.y), fabsf(cell.x - k2.z) + fabsf(cell.y - k2.w));
+            }
+            add = fma2(make_float2(-slope, -slope), far, add);
+          }
+          v = CAP ? add2(v, add) : fma2(v, make_float2(cmul, cmul), add);
+          float2 p = make_float2(at_ex2(v.x), at_ex2(v.y));
+          float2 d = add2(make_float2(dp[2 * i], dp[2 * i + 1]), del);
+          if (CAP) d = mul2(d, g);
+          d = mul2(d, BF16 ? p : mul2(p, make_float2(F, F)));
+          if (by_lim || by_doc) {
+            bool sx = DKV ? c0 + c >= from : c0 + c < lim, sy = DKV ? c0 + c + 1 >= from : c0 + c + 1 < lim;
+            if (by_doc) {
+              const int2 cd = reinterpret_cast<const int2*>(col_doc[wg][slot])[c / 2];
+              sx = sx && cd.x == my_doc;
+              sy = sy && cd.y == my_doc;
+            }
+            p.x = sx ? p.x : 0.f;
+            d.x = sx ? d.x : 0.f;
+            p.y = sy ? p.y : 0.f;
+            d.y = sy ? d.y : 0.f;
+          }
+          if (DKV) pp[i] = Half16<T>::pack(p.x, p.y);
+          if (!BF16) {
+            d.x = fminf(fmaxf(d.x, -65504.f), 65504.f);
+            d.y = fminf(fmaxf(d.y, -65504.f), 65504.f);
+          }
+          dd[i] = Half16<T>::pack(d.x, d.y);
+        }
+        if (DKV) tmem_st16(xcol + half * 16, pp);
+        tmem_st16(xcol + 64 + half * 16, dd);
+      }
+      // streamed rows that nothing sees hold anything, NaN included: 0·NaN must not enter the sums
+      if (has_pad || (!DKV && n < A.Lk && c0 + kAbCols > n)) {
+        const int c = c0 + r % kAbCols;
+        const bool dead = DKV ? c < A.Lq && A.doc_q[(long long)b * A.Lq + c] < 0
+                              : c >= n || (docs && A.doc_k[(long long)b * A.Lk + c] < 0);
+        if (dead) {
+          uint8_t* d = strm + s * 2 * Cfg::STRM + (r / kAbCols) * Cfg::STRM + (r % kAbCols) * 128;
+          for (int p = 0; p < Cfg::PANELS; p++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) *reinterpret_cast<uint4*>(d + p * kAbCols * 128 + k * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ds_full[it % NB]);
+      tile++;
+    }
+    const bool any = it > 0;
+    ok = ok && at_wait_warp(&acc_done, 0, A.err);
+    if (ok) {
+      tc_fence_after();
+      const float down = BF16 ? 1.f : 1.f / 256.f;
+      // NB = 1: the one warpgroup writes both; NB = 2: DKV one each, DQ half of the columns each
+      for (int which = 0; which < (DKV ? 2 : 1); which++) {
+        if (DKV && NB == 2 && which != wg) continue;
+        const AtView& v = which == 0 ? P.out1 : P.out2;
+        const float f = which == 0 ? A.scale * down / F : down;
+        const uint32_t acc = tmem + lane_base + (which == 0 ? Cfg::COL_ACC1 : Cfg::COL_ACC2);
+        T* o = static_cast<T*>(v.p) + b * v.sb + row * v.st + hd * v.sh;
+        const int lo = !DKV && NB == 2 ? wg * (DP / 2) : 0, hi = !DKV && NB == 2 ? lo + DP / 2 : DP;
+        for (int c = lo; c < hi && c < A.D; c += 16) {
+          float a[16];
+          if (any) tmem_ld16(acc + c, a);
+#pragma unroll
+          for (int i = 0; i < 16; i++) a[i] = any ? a[i] * f : 0.f;
+          if (!valid) continue;
+          const float lo8[8] = {a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7]};
+          const float hi8[8] = {a[8], a[9], a[10], a[11], a[12], a[13], a[14], a[15]};
+          *reinterpret_cast<uint4*>(o + c) = pack8<T>(lo8);
+          if (c + 8 < A.D) *reinterpret_cast<uint4*>(o + c + 8) = pack8<T>(hi8);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4 * NB + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::TMEM);
+  }
+}
+
+template <typename T, int DP, bool DKV, bool CAP, int BIAS>
+cudaError_t attn_bwd_one(const AttnBwdLaunch& L, int grid, cudaStream_t st) {
+  static bool set[64] = {};  // per device; a race only repeats the call
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  auto* k = k_attn_bwd<T, DP, DKV, CAP, BIAS>;
+  if (dev >= 64 || !set[dev]) {
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, AbCfg<DP>::SMEM);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) set[dev] = true;
+  }
+  k<<<grid, AbCfg<DP>::THREADS, AbCfg<DP>::SMEM, st>>>(L);
+  return cudaGetLastError();
+}
+
+template <typename T, int DP, bool DKV>
+cudaError_t attn_bwd_dp(const AttnBwdLaunch& L, int grid, cudaStream_t st) {
+  const int bias = !L.d.slopes ? 0 : L.d.grid_w > 0 ? 2 : 1;
+  if (L.d.cap > 0.f)
+    return bias == 0   ? attn_bwd_one<T, DP, DKV, true, 0>(L, grid, st)
+           : bias == 1 ? attn_bwd_one<T, DP, DKV, true, 1>(L, grid, st)
+                       : attn_bwd_one<T, DP, DKV, true, 2>(L, grid, st);
+  return bias == 0   ? attn_bwd_one<T, DP, DKV, false, 0>(L, grid, st)
+         : bias == 1 ? attn_bwd_one<T, DP, DKV, false, 1>(L, grid, st)
+                     : attn_bwd_one<T, DP, DKV, false, 2>(L, grid, st);
+}
+
+template <typename T, bool DKV>
+cudaError_t launch_attn_bwd(const AttnBwdLaunch& L, cudaStream_t st) {
+  const int nt = ((DKV ? L.d.Lk : L.d.Lq) + kAbRows - 1) / kAbRows;
+  const int grid = nt * L.d.B * (DKV ? L.d.Hk : L.d.Hq);
+  if (grid == 0) return cudaSuccess;
+  return L.d.D <= 64 ? attn_bwd_dp<T, 64, DKV>(L, grid, st) : attn_bwd_dp<T, 128, DKV>(L, grid, st);
+}
+
+}  // namespace osam

@@ -196,6 +196,10 @@ size_t sppf_bwd_smem_bytes(int H, int W);
 cudaError_t launch_conv_stem(const __half* x, const __half* w, const ConvDev& d, int BN, cudaStream_t st);
 cudaError_t launch_conv_stem_rgb(const ConvLaunch& L, cudaStream_t st);
 
+// Tensor map of a 16-bit tensor: dims[0] innermost, byte strides of dims 1…rank−1, rows of `row_bytes` (128 or 64)
+// swizzled in the matching mode.  Returns an OSAM_* code.
+int make_map(CUtensorMap* tm, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_b,
+             const uint32_t* box, int row_bytes, bool bf16 = false);
 int* device_error_word();       // the error word kernels report to (host-mapped after error_word_init)
 int error_word_init();           // allocates the host-mapped error word once per process (plan/model creation)
 int static_scratch_take_error();  // error recorded by the static-scratch entry point's kernels (and clear it)

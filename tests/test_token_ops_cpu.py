@@ -1,0 +1,154 @@
+"""The token operators without a GPU: their refusals (argument checks come before any device call), and the 64-bit
+restatement's gradients against differences."""
+import math
+
+import pytest
+import torch
+
+from objectsam_b200 import _lib
+from objectsam_b200._lib import AdamWTensor, AttnDesc, View, lib
+from oracle import token_ref
+
+INVALID = _lib.OSAM_ERR_INVALID
+
+
+def desc(**kw):
+    d = dict(dtype=_lib.F16, batch=1, len_q=4, len_k=4, heads_q=2, heads_k=2, dim=64, mask=_lib.ATTN_NONE, scale=0.125,
+             cap=0.0, grid_w=0)
+    d.update(kw)
+    return AttnDesc(**d)
+
+
+def fwd(d, *views):
+    import ctypes
+    views = list(views) or [View(4096, 4 * 128, 128, 64)] * 4
+    return lib().osam_attn_fwd(ctypes.byref(d), *views, None, None, 0, None)
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=_lib.F32), dict(dtype=7), dict(batch=-1), dict(len_q=-1), dict(len_k=-2),
+                                dict(heads_q=0), dict(heads_q=3), dict(heads_k=0), dict(dim=0), dict(dim=12), dict(dim=136),
+                                dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan),
+                                dict(cap=-1.0), dict(cap=math.nan), dict(cap=math.inf), dict(mask=3), dict(mask=-1),
+                                dict(mask=_lib.ATTN_PREFIX), dict(doc_q=4096), dict(doc_k=4096), dict(grid_w=-1),
+                                dict(len_q=1 << 30, heads_q=4), dict(len_k=(1 << 30) + 1),
+                                dict(len_k=1048577, doc_q=4096, doc_k=4096)])
+def test_attention_descriptions(kw):
+    import ctypes
+    d = desc(**kw)
+    assert fwd(d) == INVALID and lib().osam_last_error().startswith(b"attention: ")
+    assert lib().osam_attn_workspace_size(ctypes.byref(d)) == 0
+
+
+def test_attention_views():
+    good = View(4096, 512, 128, 64)
+    for bad in (View(None, 512, 128, 64), View(4104, 512, 128, 64), View(4096, 512, 124, 64), View(4096, 512, 0, 64),
+                View(4096, 512, -128, 64), View(4096, 512, 128, 1 << 40)):
+        for at in range(4):
+            assert fwd(desc(), *(bad if i == at else good for i in range(4))) == INVALID
+    assert fwd(desc(), good, good, good, good) == INVALID and b"workspace" in lib().osam_last_error()
+    # strides of extents of one are not looked at, and empty work is no error
+    one = View(4096, 3, 5, 7)
+    assert fwd(desc(len_q=1, len_k=1, heads_q=1, heads_k=1), one, one, one, one) == INVALID
+    assert b"workspace" in lib().osam_last_error()
+    assert fwd(desc(batch=0)) == fwd(desc(len_q=0)) == _lib.OSAM_OK
+
+
+def test_rms_refusals():
+    L = lib()
+
+    def call(dtype=_lib.F16, x=4096, ldx=64, res=None, ldres=0, w=4096, rows=3, C=64, total=None, ldt=0, y=8192, ldy=64):
+        return L.osam_rms_fwd(dtype, x, ldx, res, ldres, w, rows, C, 1e-5, total, ldt, y, ldy, None, None)
+
+    for kw in (dict(dtype=_lib.F32), dict(C=60), dict(C=0), dict(C=8200, ldx=8200, ldy=8200), dict(rows=-1), dict(x=None),
+               dict(x=4104), dict(ldx=56), dict(ldx=68), dict(w=None), dict(y=None), dict(ldy=8), dict(res=4100, ldres=64),
+               dict(res=4096, ldres=32), dict(total=4096, ldt=60)):
+        assert call(**kw) == INVALID, kw
+    assert call(rows=0) == _lib.OSAM_OK
+    assert L.osam_rms_fwd_q8(_lib.F16, 4096, 64, None, 0, 4096, 3, 64, 1e-5, None, 0, 8192, 64, None, None, None) == INVALID
+    assert L.osam_rms_fwd_q8(_lib.F16, 4096, 64, None, 0, 4096, 3, 64, 1e-5, None, 0, 8196, 64, 4096, None, None) == INVALID
+    assert L.osam_rms_bwd_workspace_size(12000) == 0 and L.osam_rms_bwd_workspace_size(64) > 0
+    assert L.osam_rms_bwd(_lib.F16, 4096, 64, 4096, 64, 4096, 4096, None, 0, 3, 64, 8192, 64, 4096, None, 0, None) == INVALID
+    assert L.osam_rms_bwd(_lib.F16, 4096, 64, 4096, 64, 4096, 4096, None, 0, 3, 64, 8192, 64, None, 4096, 1 << 30, None) == INVALID
+
+
+def test_adamw_refusals():
+    import ctypes
+    L = lib()
+    nbytes, elems = ctypes.c_size_t(), ctypes.c_int64()
+
+    def sizes(bits=32, **kw):
+        t = dict(p=4096, g=4096, copy=None, n=100, grad_type=_lib.F32, copy_type=_lib.F16, decay=1)
+        t.update(kw)
+        tab = (AdamWTensor * 2)(AdamWTensor(**t), AdamWTensor(4096, 4096, None, 65, _lib.F32, _lib.F16, 0))
+        return L.osam_adamw_sizes(tab, 2, bits, ctypes.byref(nbytes), ctypes.byref(elems))
+
+    assert sizes() == _lib.OSAM_OK and elems.value == 128 + 128
+    assert sizes(8) == _lib.OSAM_OK and elems.value == 256 + 256
+    for kw in (dict(bits=16), dict(n=-1), dict(p=None), dict(g=None), dict(p=4098), dict(g=4097), dict(grad_type=5),
+               dict(copy=4096, copy_type=_lib.F32), dict(copy=4097)):
+        assert sizes(**kw) == INVALID, kw
+    plan = ctypes.c_void_p()
+    tab = (AdamWTensor * 1)(AdamWTensor(4096, 4096, None, 65, _lib.F32, _lib.F16, 0))
+    assert L.osam_adamw_create(tab, 1, 32, None, 0, None, ctypes.byref(plan)) == INVALID and not plan
+    assert L.osam_adamw_step(None, 4096, 4096, None, None, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, 0.0, None, None) == INVALID
+    # a plan over no elements: the checks of a step need no device
+    none = (AdamWTensor * 1)(AdamWTensor(None, None, None, 0, _lib.F32, _lib.F16, 0))
+    assert L.osam_adamw_sizes(none, 1, 32, ctypes.byref(nbytes), ctypes.byref(elems)) == _lib.OSAM_OK and elems.value == 0
+
+
+def test_python_refusals():
+    from objectsam_b200 import norm
+    from objectsam_b200.attn import AttnGeom, AttnOp
+    from objectsam_b200.optim import AdamW
+    x = torch.zeros(4, 64, dtype=torch.float16)
+    with pytest.raises(ValueError):
+        norm.rms_norm_fwd(x, torch.ones(64), 1e-5, x)  # not on a GPU
+    with pytest.raises(ValueError):
+        norm.rms_norm_fwd(x.float(), torch.ones(64), 1e-5, x)
+    with pytest.raises(ValueError):
+        AttnOp().init(AttnGeom(1, 4, 4, 1, 1, 64, torch.float32))
+    with pytest.raises(ValueError):
+        AttnOp().init(AttnGeom(1, 4, 4, 1, 1, 64), mask="window")
+    with pytest.raises(ValueError):
+        AttnOp().init(AttnGeom(1, 4, 4, 1, 1, 64), slopes=torch.ones(2))
+    with pytest.raises(_lib.OsamError):
+        AttnOp().init(AttnGeom(1, 4, 4, 1, 1, 60))
+    with pytest.raises(ValueError):
+        AdamW([], [])
+    with pytest.raises(ValueError):
+        AdamW([torch.zeros(4)], [torch.zeros(4)])
+
+
+@pytest.mark.parametrize("cap,slope,mask", [(0.0, 0.0, "none"), (2.0, 0.3, "causal"), (3.0, 0.1, "prefix")])
+def test_reference_attention_gradients(cap, slope, mask):
+    """Σ gradient·d against central differences of the restated forward, both in 64 bits: the difference's error is
+    ε²/6 of the third derivative, about 1e-9 here."""
+    g = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    B, L, Hq, Hk, D = 2, 9, 4, 2, 5
+    q, k, v, do = r(B, L, Hq, D), r(B, L, Hk, D), r(B, L, Hk, D), r(B, L, Hq, D)
+    doc = torch.tensor([[0, 0, 0, 1, 1, -1, 1, 1, 0]] * B, dtype=torch.int32)
+    vis = token_ref.attn_visible(B, L, L, mask, prefix=[3, 7], doc_q=doc, doc_k=doc)
+    kw = dict(scale=0.4, cap=cap, slopes=torch.full((Hq,), slope), distance=token_ref.attn_distance(B, L, L, 3))
+    out = token_ref.attention(q, k, v, vis, do=do, **kw)
+    eps = 1e-5
+    for name, at in (("dq", 0), ("dk", 1), ("dv", 2)):
+        d = r(*out[name].shape)
+        loss = []
+        for s in (eps, -eps):
+            a = [q, k, v]
+            a[at] = a[at] + s * d
+            loss.append((token_ref.attention(*a, vis, **kw)["o"] * do).sum())
+        assert abs((loss[0] - loss[1]) / (2 * eps) - (out[name] * d).sum()) < 1e-7
+
+
+def test_reference_rms_gradients():
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    x, w, dy = r(5, 16), r(16), r(5, 16)
+    out = token_ref.rms_norm(x, w, 1e-5, dy=dy)
+    eps = 1e-5
+    dx, dw = r(5, 16), r(16)
+    up, down = token_ref.rms_norm(x + eps * dx, w + eps * dw, 1e-5)["y"], token_ref.rms_norm(x - eps * dx, w - eps * dw, 1e-5)["y"]
+    got = ((up - down) * dy).sum() / (2 * eps)
+    assert abs(got - (out["dx"] * dx).sum() - (out["dw"] * dw).sum()) < 1e-7
