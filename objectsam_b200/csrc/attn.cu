@@ -4,7 +4,7 @@
 #include <cmath>
 #include <cstring>
 
-#include "attn_bwd.cuh"
+#include "attn.cuh"
 
 namespace osam {
 namespace {
@@ -82,13 +82,14 @@ __global__ void __launch_bounds__(256) k_attn_join(const float* part, const floa
   if (lane == 0 && lse) lse[row] = l == 0.f ? -INFINITY : (M + at_lg2(l)) * kAtLn2;
 }
 
-// Row terms of the backward pass, per 64-query block (padded to whole blocks): (lse·log2 e, δ = do·o) — (+∞, 0) for
-// queries that see nothing and for the padding, whose P is then 0 — and the block's largest |dO|.  One CTA per
+// Row terms of the backward pass, per 64-query block (padded to whole blocks): (u − lse·log2 e, −δ), δ = do·o, u = log2
+// of the factor that the backward holds P times — (−∞, 0) for that see nothing and for the padding, whose P is then 0 — and the block's largest |dO|.  One CTA per
 // block, 16 lanes per row (a 16-byte vector each).
 template <typename T>
 __global__ void __launch_bounds__(256) k_attn_rows(const AtView o, const AtView dout, const float* lse, int Hq, int Lq,
                                                    int D, float2* rows, float* peak) {
   __shared__ float top[8];
+  constexpr float up = Half16<T>::kBf16 ? 0.f : kAbUp;
   const int nb = (Lq + kAbCols - 1) / kAbCols;
   const int blk = blockIdx.x % nb, h = (blockIdx.x / nb) % Hq, b = blockIdx.x / nb / Hq;
   const int c = threadIdx.x % 16;
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(256) k_attn_rows(const AtView o, const AtView 
     }
 #pragma unroll
     for (int s = 8; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
-    if (c == 0) rows[(bh * nb + blk) * kAbCols + r] = make_float2(live ? L * kAtLog2e : INFINITY, live ? d : 0.f);
+    if (c == 0) rows[(bh * nb + blk) * kAbCols + r] = make_float2(live ? up - L * kAtLog2e : -INFINITY, live ? -d : 0.f);
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
@@ -189,11 +190,11 @@ struct AtSplit {
   int splits, tiles;
 };
 AtSplit at_split(const osam_attn_desc& a) {
-  const int tiles = (a.len_k + 127) / 128;
+  const int keys = attn_fwd_tile_keys(a.dim), tiles = (a.len_k + keys - 1) / keys;
   const long long ctas = (((long long)a.len_q * (a.heads_q / a.heads_k) + 127) / 128) * a.batch * a.heads_k;
   AtSplit s{1, std::max(tiles, 1)};
-  if (ctas == 0 || tiles < 4 || ctas >= 2 * kAtSms) return s;
-  const int want = (int)std::min<long long>((4LL * kAtSms + ctas - 1) / ctas, tiles / 2);
+  if (ctas == 0 || a.len_k < 512 || ctas >= 2 * kAtSms) return s;
+  const int want = (int)std::min<long long>((4LL * kAtSms + ctas - 1) / ctas, a.len_k / 256);
   s.tiles = (tiles + want - 1) / want;
   s.splits = (tiles + s.tiles - 1) / s.tiles;
   return s;
@@ -292,11 +293,12 @@ int osam_attn_fwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   AttnFwdLaunch L{};
   if ((rc = at_dev(*a, W, w, &L.d, st)) != OSAM_OK) return rc;
   const bool bf16 = a->dtype == OSAM_BF16;
+  const int keys = attn_fwd_tile_keys(a->dim);
   // without keys every query is empty: no tile is visited, so the maps only have to be valid
   const osam_view& kk = a->len_k > 0 ? k : q;
   const osam_view& vv = a->len_k > 0 ? v : q;
-  if ((rc = at_map(&L.tk, kk, a->batch, std::max(a->len_k, 1), a->heads_k, a->dim, 128, bf16)) != OSAM_OK ||
-      (rc = at_map(&L.tv, vv, a->batch, std::max(a->len_k, 1), a->heads_k, a->dim, 128, bf16)) != OSAM_OK)
+  if ((rc = at_map(&L.tk, kk, a->batch, std::max(a->len_k, 1), a->heads_k, a->dim, keys, bf16)) != OSAM_OK ||
+      (rc = at_map(&L.tv, vv, a->batch, std::max(a->len_k, 1), a->heads_k, a->dim, keys, bf16)) != OSAM_OK)
     return rc;
   L.q = at_view(q);
   L.o = at_view(o);

@@ -80,6 +80,13 @@ __device__ __forceinline__ float at_rcp(float x) {
   return y;
 }
 
+// min that keeps a NaN.
+__device__ __forceinline__ float at_min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 // Two fp32 operations per instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   uint64_t d;
@@ -104,14 +111,132 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return *reinterpret_cast<float2*>(&d);
 }
 
-// D[tmem] (+)= A[tmem] · B[smem]: A's 128 rows are TMEM lanes, two 16-bit values of K per 32-bit column.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// The first n of 32 bits (n may lie outside 0 … 32).
+__device__ __forceinline__ uint32_t at_low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+// x where bit i of `vis` is set, `other` elsewhere, over 32 columns.
+__device__ __forceinline__ void at_mask32(float* x, uint32_t vis, float other) {
+#pragma unroll
+  for (int c = 0; c < 32; c++) x[c] = (vis >> c) & 1 ? x[c] : other;
+}
+// Which of 32 columns have document `doc`.
+__device__ __forceinline__ uint32_t at_doc_bits32(const int* cols, int doc) {
+  uint32_t v = 0;
+#pragma unroll
+  for (int c = 0; c < 32; c += 4) {
+    const int4 d = *reinterpret_cast<const int4*>(cols + c);
+    v |= (uint32_t(d.x == doc) << c) | (uint32_t(d.y == doc) << (c + 1)) | (uint32_t(d.z == doc) << (c + 2)) |
+         (uint32_t(d.w == doc) << (c + 3));
+  }
+  return v;
+}
+
+// 1 / (1 + 2^u) of four values with one reciprocal: 1/a = (1/abcd)·bcd.  u is held to 30, where 1 − tanh is below
+// fp32's resolution, so the product of four stays finite.  A NaN spreads to all four: hidden scores are replaced before.
+__device__ __forceinline__ void at_sigmoid4(float2 (&u)[2]) {
+  float2 a[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    a[i].x = at_ex2(at_min_nan(u[i].x, 30.f));
+    a[i].y = at_ex2(at_min_nan(u[i].y, 30.f));
+    a[i] = add2(a[i], make_float2(1.f, 1.f));
+  }
+  const float2 pr = mul2(make_float2(a[0].x, a[1].x), make_float2(a[0].y, a[1].y));
+  const float r = at_rcp(pr.x * pr.y);
+  const float2 half = mul2(make_float2(r, r), make_float2(pr.y, pr.x));  // 1 / (product of each pair)
+  u[0] = mul2(make_float2(half.x, half.x), make_float2(a[0].y, a[0].x));
+  u[1] = mul2(make_float2(half.y, half.y), make_float2(a[1].y, a[1].x));
+}
+
+// Scores in log2 units: s ← cap·tanh(scale·s/cap)·log2 e (CAP) or s·scale·log2 e, minus slope·dist.
+struct AtBias {
+  float mul;        // scale·log2 e, or with a cap 2·scale·log2 e / cap
+  float cap2;       // cap·log2 e
+  float slope;      // of the row's head, ·log2 e
+  float y, x;       // the row's position on the map times the slope; line: y only, relative to the chunk's first column
+};
+// Distances along the line of four consecutive columns, carried from one group of four to the next.
+struct AtLine {
+  float2 d[2], step;
+  __device__ __forceinline__ void start(const AtBias& P) {
+    d[0] = make_float2(P.y, P.y - P.slope);
+    d[1] = make_float2(P.y - 2.f * P.slope, P.y - 3.f * P.slope);
+    step = make_float2(-4.f * P.slope, -4.f * P.slope);
+  }
+  __device__ __forceinline__ void next() {
+    d[0] = add2(d[0], step);
+    d[1] = add2(d[1], step);
+  }
+};
+// Four consecutive columns; `line` holds their distances (line), ky / kx their cells (grid).  out: the scores plus
+// `add`; with CAP, sig = 1/(1 + 2^u), from which 1 − tanh² = 4·sig·(1 − sig).
+template <bool CAP, int BIAS>
+__device__ __forceinline__ void at_scores4(const AtBias& P, float2 (&s)[2], const float2 (&add)[2], AtLine& line,
+                                           const float4& ky, const float4& kx, float2 (&sig)[2]) {
+  const float2 mul = make_float2(P.mul, P.mul);
+  float2 b[2] = {add[0], add[1]};
+  if (BIAS == 1) {
+    b[0] = make_float2(b[0].x - fabsf(line.d[0].x), b[0].y - fabsf(line.d[0].y));
+    b[1] = make_float2(b[1].x - fabsf(line.d[1].x), b[1].y - fabsf(line.d[1].y));
+    line.next();
+  }
+  if (BIAS == 2) {
+    const float2 ns = make_float2(-P.slope, -P.slope), y = make_float2(P.y, P.y), x = make_float2(P.x, P.x);
+    const float2 y0 = fma2(ns, make_float2(ky.x, ky.y), y), y1 = fma2(ns, make_float2(ky.z, ky.w), y);
+    const float2 x0 = fma2(ns, make_float2(kx.x, kx.y), x), x1 = fma2(ns, make_float2(kx.z, kx.w), x);
+    b[0] = add2(b[0], make_float2(-fabsf(y0.x) - fabsf(x0.x), -fabsf(y0.y) - fabsf(x0.y)));
+    b[1] = add2(b[1], make_float2(-fabsf(y1.x) - fabsf(x1.x), -fabsf(y1.y) - fabsf(x1.y)));
+  }
+  if (CAP) {
+    sig[0] = mul2(s[0], mul);
+    sig[1] = mul2(s[1], mul);
+    at_sigmoid4(sig);
+    const float2 m2 = make_float2(-2.f * P.cap2, -2.f * P.cap2), c2 = make_float2(P.cap2, P.cap2);
+    s[0] = fma2(m2, sig[0], add2(c2, b[0]));
+    s[1] = fma2(m2, sig[1], add2(c2, b[1]));
+  } else {
+    s[0] = fma2(s[0], mul, b[0]);
+    s[1] = fma2(s[1], mul, b[1]);
+  }
+}
+
+// Barrier of the two warps that share rows, with the OR of a flag.
+__device__ __forceinline__ bool at_pair_any(int id, bool flag) {
+  uint32_t r;
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(r)
+      : "r"(uint32_t(flag)), "r"(id)
+      : "memory");
+  return r != 0;
+}
+
+// The MMA warp runs its loop with all lanes and one elected lane issues: with warp-uniform control flow the descriptors
+// stay in uniform registers, where the instruction reads them (issued from inside a one-lane branch, every MMA
+// first moved its operands over, about 100 cycles each: more than these small MMAs take).
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// A's 128 rows are TMEM lanes, two 16-bit values of K per 32-bit column.
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
       : "memory");
 }
 // kind::f16 instruction descriptor, fp32 D, K-major A; bf16 or fp16 operands; b_mn: MN-major B.
@@ -170,12 +295,13 @@ __device__ __forceinline__ bool at_wait_warp(uint64_t* bar, uint32_t parity, int
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
 }
 
-// Which tiles of the streamed side a CTA visits.  Without documents every tile of [begin, end); with them, the
-// tiles whose bit is set (built by at_doc_bits).
+// Which tiles of the streamed side a CTA visits: of [begin, end) all, or with documents those whose bit is set (built
+// by at_doc_bits).  The order is from `from` down to `begin`, then from + 1 up to end − 1: with `from` the tile of
+// the CTA's own positions, the keys nearest in distance come first, and with them a row's largest scores.
 struct AtTiles {
-  int begin, end;
+  int begin, end, from;
   const uint32_t* live;  // nullptr: all
-  __device__ __forceinline__ int next(int t) const {  // first visited tile ≥ t (end: none)
+  __device__ __forceinline__ int up(int t) const {  // first live tile ≥ t (end: none)
     if (!live || t >= end) return t;
     uint32_t w = live[(t - begin) >> 5] >> ((t - begin) & 31);
     while (!w) {
@@ -185,7 +311,32 @@ struct AtTiles {
     }
     return min(end, t + __ffs(w) - 1);
   }
-  __device__ __forceinline__ int first() const { return next(begin); }
+  __device__ __forceinline__ int down(int t) const {  // last live tile ≤ t (begin − 1: none)
+    if (!live || t < begin) return t;
+    uint32_t w = live[(t - begin) >> 5] << (31 - ((t - begin) & 31));
+    while (!w) {
+      t = begin + ((t - begin) >> 5) * 32 - 1;
+      if (t < begin) return begin - 1;
+      w = live[(t - begin) >> 5];
+    }
+    return t - __clz(w);
+  }
+  __device__ __forceinline__ int count() const {
+    if (!live) return max(0, end - begin);
+    int n = 0;
+    for (int w = 0; w * 32 < end - begin; w++) n += __popc(live[w]);
+    return n;
+  }
+  // `end` says that there is none (any more)
+  __device__ __forceinline__ int first() const {
+    const int t = down(from);
+    return t >= begin ? t : up(from + 1);
+  }
+  __device__ __forceinline__ int next(int t) const {
+    if (t > from) return up(t + 1);
+    t = down(t - 1);
+    return t >= begin ? t : up(from + 1);
+  }
 };
 __device__ __forceinline__ bool at_bit(const uint32_t* w, int i) { return (w[i >> 5] >> (i & 31)) & 1; }
 
@@ -232,7 +383,21 @@ struct AttnFwdLaunch {
   float* part;    // [split][B][Hq][Lq][D] unnormalised outputs
   float2* stats;  // [split][B][Hq][Lq] (reference maximum in log2 units, sum)
 };
+constexpr int attn_fwd_tile_keys(int dim) { return dim <= 64 ? 128 : 64; }  // keys of a tile (AfCfg::KEYS)
 template <typename T>
 cudaError_t launch_attn_fwd(const AttnFwdLaunch& L, cudaStream_t st);
+
+constexpr int kAbRows = 128, kAbCols = 64;
+constexpr float kAbUp = 8.f;  // fp16: P is held times 2^8
+
+struct AttnBwdLaunch {
+  AttnDev d;
+  CUtensorMap stat1, stat2, strm1, strm2;
+  AtView out1, out2;      // dK, dV (DKV); dQ (DQ)
+  const float2* rows;     // [B][Hq][⌈Lq/64⌉·64] (log2 of P's factor − lse·log2 e, −∞ where the query is empty; −δ)
+  const float* peak;      // [B][Hq][⌈Lq/64⌉] max |dO| of the block
+};
+template <typename T, bool DKV>
+cudaError_t launch_attn_bwd(const AttnBwdLaunch& L, cudaStream_t st);
 
 }  // namespace osam

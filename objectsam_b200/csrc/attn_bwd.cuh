@@ -8,35 +8,24 @@
 //
 // Per tile, rows = the stationary side (TMEM lanes), columns = the streamed side:
 //   X = stat1·strm1ᵀ (scores), Y = stat2·strm2ᵀ (dP), both fp32 in TMEM
-//   one thread per row: p = 2^(x − lse), ds = p·(dp − δ)·(1 − t²), both back to TMEM in 16 bits over X and Y
+//   two threads per row (32 columns each): p = 2^(x − lse), ds = p·(dp − δ)·(1 − t²), back to TMEM in 16 bits over
+//   X and Y
 //   acc2 += P·strm2 (DKV), acc1 += dS·strm1, P and dS as TMEM operands
 // fp16 keeps its precision over long rows and small gradients by powers of two: P is held times 2^8 and dS times
 // 2^8·F with F = 2^−e, e the exponent of the largest |dO| (of the key head's group for DKV, of the row's block for
 // DQ), both taken back in fp32 at the end; bf16 needs neither.
-// Warps: 4 per buffer of (X, Y) for the element-wise part, then the TMA producer and the MMA issuer.  Up to 64 head
-// dims one buffer and 256 TMEM columns, two CTAs per SM; above, two buffers in one CTA with all 512 columns: the
-// tensor cores work on one while the other is in the element-wise part.
+// Warps: 8 per buffer of (X, Y) for the element-wise part (warps w and w + 4 share rows), then the TMA producer and the
+// MMA issuer.  Up to 64 head dims one buffer and 256 TMEM columns, two CTAs per SM; above, two buffers in one CTA
+// with all 512 columns: the tensor cores work on one while the other is in the element-wise part.
 #pragma once
 #include "attn.cuh"
 
 namespace osam {
 
-constexpr int kAbRows = 128, kAbCols = 64;
-
-struct AttnBwdLaunch {
-  AttnDev d;
-  CUtensorMap stat1, stat2, strm1, strm2;
-  AtView out1, out2;      // dK, dV (DKV); dQ (DQ)
-  const float2* rows;     // [B][Hq][⌈Lq/64⌉·64] (lse·log2 e, or +∞ where the query is empty; δ)
-  const float* peak;      // [B][Hq][⌈Lq/64⌉] max |dO| of the block
-};
-template <typename T, bool DKV>
-cudaError_t launch_attn_bwd(const AttnBwdLaunch& L, cudaStream_t st);
-
 template <int DP>
 struct AbCfg {
   static constexpr int PANELS = DP / 64;
-  static constexpr int NB = DP == 64 ? 1 : 2;   // (X, Y) buffers = warpgroups
+  static constexpr int NB = DP == 64 ? 1 : 2;   // (X, Y) buffers, each with eight warps
   static constexpr int CTAS = DP == 64 ? 2 : 1; // per SM
   static constexpr int STAGES = 4;
   static constexpr int STAT = PANELS * kAbRows * 128;  // bytes of one stationary operand
@@ -45,7 +34,8 @@ struct AbCfg {
   static constexpr int SMEM = 1024 + 2 * STAT + STAGES * (2 * STRM + ROWS);
   static constexpr int TMEM = DP == 64 ? 256 : 512;
   static constexpr int COL_ACC1 = 128 * NB, COL_ACC2 = COL_ACC1 + DP;
-  static constexpr int THREADS = 128 * NB + 64;
+  static constexpr int SOFT = 256 * NB;  // element-wise threads
+  static constexpr int THREADS = SOFT + 64;
 };
 
 // Visits (head of the group, tile) pairs, heads outermost.
@@ -57,7 +47,7 @@ struct AbIter {
   }
   __device__ __forceinline__ bool more(const AtTiles& T, int heads) const { return g < heads && t < T.end; }
   __device__ __forceinline__ void step(const AtTiles& T) {
-    t = T.next(t + 1);
+    t = T.next(t);
     if (t >= T.end) {
       g++;
       t = T.first();
@@ -83,7 +73,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t live[kAtDocWords], mix[kAtDocWords], pad[kAtDocWords];
   __shared__ __align__(16) int col_doc[NB][2][kAbCols];
-  __shared__ __align__(16) float2 col_cell[NB][BIAS == 2 ? 2 : 1][kAbCols];
+  __shared__ __align__(16) float col_y[NB][BIAS == 2 ? 2 : 1][kAbCols], col_x[NB][BIAS == 2 ? 2 : 1][kAbCols];
 
   const AttnDev& A = P.d;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -122,6 +112,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     tiles.end = (at_limit(A, n, prefix, off + last) + kAbCols - 1) / kAbCols;
     lim_min = at_limit(A, n, prefix, off + row0);
   }
+  tiles.from = tiles.begin - 1;  // the order does not matter here: upwards
   const bool docs = A.doc_q != nullptr;
   tiles.live = docs ? live : nullptr;
 
@@ -133,7 +124,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     }
     for (int i = 0; i < NB; i++) {
       mbar_init(&xy_full[i], 1);
-      mbar_init(&ds_full[i], 4);
+      mbar_init(&ds_full[i], 8);
     }
     mbar_init(&acc_done, 1);
     fence_barrier_init();
@@ -142,7 +133,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     tma_prefetch_desc(&P.strm1);
     tma_prefetch_desc(&P.strm2);
   }
-  if (warp == 4 * NB + 1) {
+  if (warp == 8 * NB + 1) {
     tmem_alloc(&tmem_slot, Cfg::TMEM);
     tmem_relinquish();
   }
@@ -156,7 +147,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp == 4 * NB) {
+  if (warp == 8 * NB) {
     if (lane == 0) {
       AbIter x;
       x.start(tiles);
@@ -188,66 +179,60 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
       for (int i = max(0, it - Cfg::STAGES); i < it; i++) mbar_wait(&full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, A.err);
     }
     __syncwarp();
-  } else if (warp == 4 * NB + 1) {
-    if (lane == 0) {
-      const int ks = (A.D + 15) / 16;
-      const uint32_t id_x = at_idesc(BF16, 128, kAbCols, false), id_g = at_idesc(BF16, 128, 16 * ks, true);
-      const uint32_t a1 = smem_u32(smem), a2 = a1 + Cfg::STAT, sb = smem_u32(strm);
-      // X and Y of streamed tile `it`
-      auto scores = [&](int it) {
-        const uint32_t b1 = sb + (it % Cfg::STAGES) * 2 * Cfg::STRM, b2 = b1 + Cfg::STRM;
-        const uint32_t d = tmem + (it % NB) * 128;
-        for (int k = 0; k < ks; k++) {
-          const uint32_t oa = (k / 4) * kAbRows * 128 + (k % 4) * 32, ob = (k / 4) * kAbCols * 128 + (k % 4) * 32;
-          umma_f16(d, smem_desc_kmajor(a1 + oa, 128), smem_desc_kmajor(b1 + ob, 128), id_x, k > 0);
-        }
-        for (int k = 0; k < ks; k++) {
-          const uint32_t oa = (k / 4) * kAbRows * 128 + (k % 4) * 32, ob = (k / 4) * kAbCols * 128 + (k % 4) * 32;
-          umma_f16(d + 64, smem_desc_kmajor(a2 + oa, 128), smem_desc_kmajor(b2 + ob, 128), id_x, k > 0);
-        }
-        umma_commit(&xy_full[it % NB]);
-      };
-      AbIter ahead, x;  // `ahead` runs NB tiles in front
-      ahead.start(tiles);
-      x.start(tiles);
-      bool ok = !x.more(tiles, streams) || mbar_wait(&stat_full, 0, A.err);
-      int ia = 0;
-      for (; ok && ia < NB && ahead.more(tiles, streams); ahead.step(tiles), ia++) {
-        ok = mbar_wait(&full[ia % Cfg::STAGES], (ia / Cfg::STAGES) & 1, A.err);
-        if (!ok) break;
+  } else if (warp == 8 * NB + 1) {
+    const int ks = (A.D + 15) / 16;
+    const uint32_t id_x = at_idesc(BF16, 128, kAbCols, false), id_g = at_idesc(BF16, 128, 16 * ks, true);
+    const uint32_t a1 = smem_u32(smem), sb = smem_u32(strm);
+    const uint64_t da1 = smem_desc_kmajor(a1, 128), da2 = smem_desc_kmajor(a1 + Cfg::STAT, 128);
+    const uint64_t db = smem_desc_kmajor(sb, 128), dg = at_desc_mn(sb, kAbCols * 128);  // offsets: bytes / 16
+    const int count = __shfl_sync(0xffffffffu, tiles.count(), 0) * streams;
+    // X and Y of streamed tile `it`
+    auto scores = [&](int it) {
+      const uint64_t b1 = db + ((it % Cfg::STAGES) * 2 * Cfg::STRM >> 4), b2 = b1 + (Cfg::STRM >> 4);
+      const uint32_t d = tmem + (it % NB) * 128;
+#pragma unroll
+      for (int k = 0; k < DP / 16; k++)
+        if (k < ks)
+          mma_ss(d, da1 + (((k / 4) * kAbRows * 128 + (k % 4) * 32) >> 4),
+                 b1 + (((k / 4) * kAbCols * 128 + (k % 4) * 32) >> 4), id_x, k > 0);
+#pragma unroll
+      for (int k = 0; k < DP / 16; k++)
+        if (k < ks)
+          mma_ss(d + 64, da2 + (((k / 4) * kAbRows * 128 + (k % 4) * 32) >> 4),
+                 b2 + (((k / 4) * kAbCols * 128 + (k % 4) * 32) >> 4), id_x, k > 0);
+      mma_commit(&xy_full[it % NB]);
+    };
+    bool ok = count == 0 || at_wait_warp(&stat_full, 0, A.err);
+    for (int it = 0; ok && it < NB && it < count; it++) {
+      if (!(ok = at_wait_warp(&full[it % Cfg::STAGES], (it / Cfg::STAGES) & 1, A.err))) break;
+      tc_fence_after();
+      scores(it);
+    }
+    for (int it = 0; ok && it < count; it++) {
+      const int s = it % Cfg::STAGES, buf = it % NB, ia = it + NB;
+      if (!(ok = at_wait_warp(&ds_full[buf], (it / NB) & 1, A.err))) break;
+      tc_fence_after();
+      const uint64_t g1 = dg + (s * 2 * Cfg::STRM >> 4), g2 = g1 + (Cfg::STRM >> 4);
+      const uint32_t d = tmem + buf * 128;
+      if (DKV) {
+#pragma unroll
+        for (int k = 0; k < kAbCols / 16; k++)
+          mma_ts(tmem + Cfg::COL_ACC2, d + k / 2 * 32 + k % 2 * 8, g2 + (k * 16 * 128 >> 4), id_g, (it | k) != 0);
+      }
+#pragma unroll
+      for (int k = 0; k < kAbCols / 16; k++)
+        mma_ts(tmem + Cfg::COL_ACC1, d + 64 + k / 2 * 32 + k % 2 * 8, g1 + (k * 16 * 128 >> 4), id_g, (it | k) != 0);
+      mma_commit(&empty[s]);
+      if (ia < count) {
+        if (!(ok = at_wait_warp(&full[ia % Cfg::STAGES], (ia / Cfg::STAGES) & 1, A.err))) break;
         tc_fence_after();
         scores(ia);
       }
-      int it = 0;
-      for (; ok && x.more(tiles, streams); x.step(tiles), it++) {
-        const int s = it % Cfg::STAGES, buf = it % NB;
-        if (!(ok = mbar_wait(&ds_full[buf], (it / NB) & 1, A.err))) break;
-        tc_fence_after();
-        const uint32_t b1 = sb + s * 2 * Cfg::STRM, b2 = b1 + Cfg::STRM, d = tmem + buf * 128;
-        if (DKV) {
-#pragma unroll
-          for (int k = 0; k < kAbCols / 16; k++)
-            umma_f16_ts(tmem + Cfg::COL_ACC2, d + k * 8, at_desc_mn(b2 + k * 16 * 128, kAbCols * 128), id_g, (it | k) != 0);
-        }
-#pragma unroll
-        for (int k = 0; k < kAbCols / 16; k++)
-          umma_f16_ts(tmem + Cfg::COL_ACC1, d + 64 + k * 8, at_desc_mn(b1 + k * 16 * 128, kAbCols * 128), id_g,
-                      (it | k) != 0);
-        umma_commit(&empty[s]);
-        if (ahead.more(tiles, streams)) {
-          if (!(ok = mbar_wait(&full[ia % Cfg::STAGES], (ia / Cfg::STAGES) & 1, A.err))) break;
-          tc_fence_after();
-          scores(ia);
-          ahead.step(tiles);
-          ia++;
-        }
-      }
-      umma_commit(&acc_done);
-      if (!ok) mbar_wait(&acc_done, 0, A.err);  // the issued MMAs finish before TMEM is freed
     }
-    __syncwarp();
+    mma_commit(&acc_done);
+    if (!ok) at_wait_warp(&acc_done, 0, A.err);  // the issued MMAs finish before TMEM is freed
   } else {
-    const int wg = warp / 4, r = tid % 128;
+    const int buf = warp / 8, half = warp / 4 % 2, r = tid % 128;
     const uint32_t lane_base = uint32_t((warp % 4) * 32) << 16;
     const int row = row0 + r;
     const bool valid = row < (DKV ? A.Lk : A.Lq);
@@ -261,7 +246,6 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     // DKV: queries from `from` on see the key; DQ: keys below `lim` are seen
     const int from = row >= n ? INT_MAX : (!causal || prefix > row ? 0 : row - off);
     const int lim = !DKV && valid ? at_limit(A, n, prefix, pos) : 0;
-    const float2 cell = BIAS == 2 ? at_cell(A, pos) : make_float2(0.f, 0.f);
     float F = 1.f;  // power of two that brings the largest |dO| to [1, 2)
     if (!BF16) {
       float peak = 0.f;
@@ -276,27 +260,33 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
       const int e = (__float_as_int(peak) >> 23) & 255;
       if (peak > 0.f && e < 255) F = __int_as_float(min(227, max(27, 254 - e)) << 23);  // at most 2^±100
     }
-    constexpr float kUp = BF16 ? 0.f : 8.f;  // log2 of P's factor
     float row_lse = 0.f, row_delta = 0.f;
     if (!DKV) {
-      const float2 v = valid ? P.rows[((long long)b * A.Hq + hd) * nq64 * kAbCols + row] : make_float2(INFINITY, 0.f);
-      row_lse = kUp - v.x;
-      row_delta = -v.y;
+      const float2 v = valid ? P.rows[((long long)b * A.Hq + hd) * nq64 * kAbCols + row] : make_float2(-INFINITY, 0.f);
+      row_lse = v.x;
+      row_delta = v.y;
     }
-    const float cmul = CAP ? 2.f * A.scale * kAtLog2e / A.cap : A.scale * kAtLog2e, cap2 = A.cap * kAtLog2e;
-    float slope = 0.f;
+    AtBias bias;
+    bias.mul = CAP ? 2.f * A.scale * kAtLog2e / A.cap : A.scale * kAtLog2e;
+    bias.cap2 = A.cap * kAtLog2e;
+    bias.slope = bias.y = bias.x = 0.f;
     int slope_of = -1;
     AbIter x;
     x.start(tiles);
     bool ok = true;
     int it = 0, tile = 0;
     for (; x.more(tiles, streams); x.step(tiles), it++) {
-      if (NB > 1 && it % NB != wg) continue;
-      const int c0 = x.t * kAbCols;  // first column: query (DKV) or key (DQ)
+      if (NB > 1 && it % NB != buf) continue;
+      const int c0 = x.t * kAbCols, h0 = half * 32;  // first column: query (DKV) or key (DQ); this thread's first
       const int h = DKV ? hd * A.G + x.g : hd;
       if (BIAS && slope_of != h) {
-        slope = A.slopes[h] * kAtLog2e;
+        bias.slope = A.slopes[h] * kAtLog2e;
         slope_of = h;
+        if (BIAS == 2) {
+          const float2 cell = at_cell(A, pos);
+          bias.y = cell.x * bias.slope;
+          bias.x = cell.y * bias.slope;
+        }
       }
       const bool by_doc = docs && at_bit(mix, x.t - tiles.begin);
       const bool has_pad = docs && at_bit(pad, x.t - tiles.begin);
@@ -304,105 +294,102 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
                               : c0 + kAbCols > lim_min;
       const int slot = tile & 1;
       if (by_doc || BIAS == 2) {
-        if (r < kAbCols) {
+        if (half == 0 && r < kAbCols) {
           if (docs) {
             const int c = c0 + r, L = DKV ? A.Lq : n;
             const int id = c < L ? (DKV ? A.doc_q : A.doc_k)[(long long)b * (DKV ? A.Lq : A.Lk) + c] : -1;
-            col_doc[wg][slot][r] = id < 0 ? -1 : id;
+            col_doc[buf][slot][r] = id < 0 ? -1 : id;
           }
-          if (BIAS == 2) col_cell[wg][slot][r] = at_cell(A, DKV ? off + c0 + r : c0 + r);
+          if (BIAS == 2) {
+            const float2 cell = at_cell(A, DKV ? off + c0 + r : c0 + r);
+            col_y[buf][slot][r] = cell.x;
+            col_x[buf][slot][r] = cell.y;
+          }
         }
-        named_bar_sync(1 + wg, 128);
+        named_bar_sync(1 + buf, 256);
       }
-      if (!(ok = at_wait_warp(&xy_full[it % NB], (it / NB) & 1, A.err))) break;
+      if (!(ok = at_wait_warp(&xy_full[buf], (it / NB) & 1, A.err))) break;
       tc_fence_after();
       const int s = it % Cfg::STAGES;
-      const float4* rows2 = reinterpret_cast<const float4*>(srows + s * Cfg::ROWS);
+      const float4* rows2 = reinterpret_cast<const float4*>(srows + s * Cfg::ROWS + h0 * 8);
       if (DKV) {  // written by the bulk copy that this barrier counts
         if (!(ok = at_wait_warp(&full[s], (it / Cfg::STAGES) & 1, A.err))) break;
       }
-      const float rel = float(pos - (DKV ? off + c0 : c0));
-      const uint32_t xcol = tmem + lane_base + (it % NB) * 128;
+      if (BIAS == 1) bias.y = float(pos - (DKV ? off + c0 : c0) - h0) * bias.slope;
+      const uint32_t xcol = tmem + lane_base + buf * 128;
+      float sv[32], dp[32];
+      tmem_ld32_nowait(xcol + h0, sv);
+      tmem_ld32_nowait(xcol + 64 + h0, dp);
+      tmem_wait_ld();
+      uint32_t vis = 0xffffffffu;
+      if (by_lim || by_doc) {  // hidden: p = 0 and ds = 0 whatever the operands hold
+        vis = DKV ? (from == INT_MAX ? 0u : ~at_low_bits(from - c0 - h0)) : at_low_bits(lim - c0 - h0);
+        if (by_doc) vis &= at_doc_bits32(&col_doc[buf][slot][h0], my_doc);
+        at_mask32(sv, vis, CAP ? 0.f : -INFINITY);
+        at_mask32(dp, vis, 0.f);
+      }
+      AtLine line;
+      if (BIAS == 1) line.start(bias);
+      uint32_t pp[16], dd[16];
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        float sv[32], dp[32];
-        tmem_ld32_nowait(xcol + half * 32, sv);
-        tmem_ld32_nowait(xcol + 64 + half * 32, dp);
-        tmem_wait_ld();
-        uint32_t pp[16], dd[16];
+      for (int c = 0; c < 32; c += 4) {
+        float2 v[2] = {make_float2(sv[c], sv[c + 1]), make_float2(sv[c + 2], sv[c + 3])}, sig[2];
+        float2 add[2], del[2];  // −lse (with P's factor) and −δ
+        if (DKV) {
+          const float4 q0 = rows2[c / 2], q1 = rows2[c / 2 + 1];
+          add[0] = make_float2(q0.x, q0.z);
+          add[1] = make_float2(q1.x, q1.z);
+          del[0] = make_float2(q0.y, q0.w);
+          del[1] = make_float2(q1.y, q1.w);
+        } else {
+          add[0] = add[1] = make_float2(row_lse, row_lse);
+          del[0] = del[1] = make_float2(row_delta, row_delta);
+        }
+        if (CAP && (by_lim || by_doc)) {
+          add[0] = make_float2((vis >> c) & 1 ? add[0].x : -INFINITY, (vis >> (c + 1)) & 1 ? add[0].y : -INFINITY);
+          add[1] = make_float2((vis >> (c + 2)) & 1 ? add[1].x : -INFINITY, (vis >> (c + 3)) & 1 ? add[1].y : -INFINITY);
+        }
+        float4 ky = {}, kx = {};
+        if (BIAS == 2) {
+          ky = *reinterpret_cast<const float4*>(&col_y[buf][slot][h0 + c]);
+          kx = *reinterpret_cast<const float4*>(&col_x[buf][slot][h0 + c]);
+        }
+        at_scores4<CAP, BIAS>(bias, v, add, line, ky, kx, sig);
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int c = half * 32 + 2 * i;
-          float2 v = make_float2(sv[2 * i], sv[2 * i + 1]);
-          float2 add, del;  // kUp − lse and −δ of the pair
-          if (DKV) {
-            const float4 q2 = rows2[c / 2];
-            add = make_float2(kUp - q2.x, kUp - q2.z);
-            del = make_float2(-q2.y, -q2.w);
-          } else {
-            add = make_float2(row_lse, row_lse);
-            del = make_float2(row_delta, row_delta);
+        for (int i = 0; i < 2; i++) {
+          float2 p = make_float2(at_ex2(v[i].x), at_ex2(v[i].y));
+          float2 d = add2(make_float2(dp[c + 2 * i], dp[c + 2 * i + 1]), del[i]);
+          if (CAP) {  // 1 − t² = 4·sig·(1 − sig)
+            const float2 g = fma2(sig[i], make_float2(-4.f, -4.f), make_float2(4.f, 4.f));
+            d = mul2(d, mul2(g, sig[i]));
           }
-          float2 g = make_float2(1.f, 1.f);  // 1 − t²
-          if (CAP) {
-            const float2 rc = make_float2(at_rcp(1.f + at_ex2(v.x * cmul)), at_rcp(1.f + at_ex2(v.y * cmul)));
-            v = make_float2(fmaf(-2.f * cap2, rc.x, cap2), fmaf(-2.f * cap2, rc.y, cap2));
-            g = make_float2(4.f * rc.x * (1.f - rc.x), 4.f * rc.y * (1.f - rc.y));
-          }
-          if (BIAS) {
-            float2 far;
-            if (BIAS == 1) {
-              far = make_float2(fabsf(rel - float(c)), fabsf(rel - float(c + 1)));
-            } else {
-              const float4 k2 = reinterpret_cast<const float4*>(col_cell[wg][slot])[c / 2];
-              far = make_float2(fabsf(cell.x - k2.x) + fabsf(cell.y - k2.y), fabsf(cell.x - k2.z) + fabsf(cell.y - k2.w));
-            }
-            add = fma2(make_float2(-slope, -slope), far, add);
-          }
-          v = CAP ? add2(v, add) : fma2(v, make_float2(cmul, cmul), add);
-          float2 p = make_float2(at_ex2(v.x), at_ex2(v.y));
-          float2 d = add2(make_float2(dp[2 * i], dp[2 * i + 1]), del);
-          if (CAP) d = mul2(d, g);
           d = mul2(d, BF16 ? p : mul2(p, make_float2(F, F)));
-          if (by_lim || by_doc) {
-            bool sx = DKV ? c0 + c >= from : c0 + c < lim, sy = DKV ? c0 + c + 1 >= from : c0 + c + 1 < lim;
-            if (by_doc) {
-              const int2 cd = reinterpret_cast<const int2*>(col_doc[wg][slot])[c / 2];
-              sx = sx && cd.x == my_doc;
-              sy = sy && cd.y == my_doc;
-            }
-            p.x = sx ? p.x : 0.f;
-            d.x = sx ? d.x : 0.f;
-            p.y = sy ? p.y : 0.f;
-            d.y = sy ? d.y : 0.f;
-          }
-          if (DKV) pp[i] = Half16<T>::pack(p.x, p.y);
+          if (DKV) pp[c / 2 + i] = Half16<T>::pack(p.x, p.y);
           if (!BF16) {
             d.x = fminf(fmaxf(d.x, -65504.f), 65504.f);
             d.y = fminf(fmaxf(d.y, -65504.f), 65504.f);
           }
-          dd[i] = Half16<T>::pack(d.x, d.y);
+          dd[c / 2 + i] = Half16<T>::pack(d.x, d.y);
         }
-        if (DKV) tmem_st16(xcol + half * 16, pp);
-        tmem_st16(xcol + 64 + half * 16, dd);
       }
+      if (DKV) tmem_st16(xcol + h0, pp);  // over the scores that this thread has read
+      tmem_st16(xcol + 64 + h0, dd);
       // streamed rows that nothing sees hold anything, NaN included: 0·NaN must not enter the sums
       if (has_pad || (!DKV && n < A.Lk && c0 + kAbCols > n)) {
-        const int c = c0 + r % kAbCols;
+        const int c = c0 + r % kAbCols, panel = half;
         const bool dead = DKV ? c < A.Lq && A.doc_q[(long long)b * A.Lq + c] < 0
                               : c >= n || (docs && A.doc_k[(long long)b * A.Lk + c] < 0);
-        if (dead) {
-          uint8_t* d = strm + s * 2 * Cfg::STRM + (r / kAbCols) * Cfg::STRM + (r % kAbCols) * 128;
-          for (int p = 0; p < Cfg::PANELS; p++)
+        if (dead && panel < Cfg::PANELS) {
+          uint8_t* d = strm + s * 2 * Cfg::STRM + (r / kAbCols) * Cfg::STRM + panel * kAbCols * 128 + (r % kAbCols) * 128;
 #pragma unroll
-            for (int k = 0; k < 8; k++) *reinterpret_cast<uint4*>(d + p * kAbCols * 128 + k * 16) = make_uint4(0, 0, 0, 0);
+          for (int k = 0; k < 8; k++) *reinterpret_cast<uint4*>(d + k * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ds_full[it % NB]);
+      if (lane == 0) mbar_arrive(&ds_full[buf]);
       tile++;
     }
     const bool any = it > 0;
@@ -410,14 +397,15 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     if (ok) {
       tc_fence_after();
       const float down = BF16 ? 1.f : 1.f / 256.f;
-      // NB = 1: the one warpgroup writes both; NB = 2: DKV one each, DQ half of the columns each
-      for (int which = 0; which < (DKV ? 2 : 1); which++) {
-        if (DKV && NB == 2 && which != wg) continue;
+      // four warpgroups (two where NB = 1) share the outputs: by accumulator where there are two, then by columns
+      const int wgs = 2 * NB, me = warp / 4, outs = DKV ? 2 : 1, parts = wgs / outs;
+      const int which = me / parts;
+      {
         const AtView& v = which == 0 ? P.out1 : P.out2;
         const float f = which == 0 ? A.scale * down / F : down;
         const uint32_t acc = tmem + lane_base + (which == 0 ? Cfg::COL_ACC1 : Cfg::COL_ACC2);
         T* o = static_cast<T*>(v.p) + b * v.sb + row * v.st + hd * v.sh;
-        const int lo = !DKV && NB == 2 ? wg * (DP / 2) : 0, hi = !DKV && NB == 2 ? lo + DP / 2 : DP;
+        const int lo = me % parts * (DP / parts), hi = lo + DP / parts;
         for (int c = lo; c < hi && c < A.D; c += 16) {
           float a[16];
           if (any) tmem_ld16(acc + c, a);
@@ -434,7 +422,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 4 * NB + 1) {
+  if (warp == 8 * NB + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::TMEM);
   }

@@ -3,51 +3,57 @@
 // single token of many heads still fills rows.  Long caches with few rows are split over the keys: each split
 // writes its unnormalised output with its maximum and sum, and k_attn_join (attn.cu) adds them.
 //
-// Per 128-key tile:  S = Q·Kᵀ (tcgen05, fp32 in TMEM) → one thread per row reads its 128 scores from TMEM, applies
-// cap, bias and masks, keeps the running maximum and sum (no shuffles: a row is a lane) and writes P in 16 bits
-// back to TMEM → O += P·V with P as the TMEM operand.  O stays in TMEM; it is rescaled only when a row's maximum
-// grew by more than 2^8 (P ≤ 2^8 keeps its relative precision in 16 bits, the sum is fp32), which after the first
-// tiles is rare.
-// Warps 0–3: softmax (thread = row = TMEM lane), warp 4: TMA producer, warp 5: TMEM owner and MMA issuer.
-// TMEM, 256 columns a CTA (two CTAs per SM, whose softmax and MMA phases overlap): up to 64 head dims S | O | P with S
-// released as soon as it is in registers, so the next Q·Kᵀ runs under the softmax; above, S | O with P written over S.
+// Per key tile:  S = Q·Kᵀ (tcgen05, fp32 in TMEM) → two threads per row (half of the columns each) read its scores from
+// TMEM 32 at a time, apply cap, bias and masks, take p = 2^(x − m) against the row's reference maximum m and write
+// P in 16 bits back to TMEM → O += P·V with P as the TMEM operand.  A row is a TMEM lane, so its maximum and sum need no
+// shuffles.  m is taken from the first tile and kept while scores stay below m + 8 (P ≤ 2^8 keeps its relative
+// precision in 16 bits, the sum is fp32): scores turn into P in one pass, without waiting for the tile's maximum.
+// When a score does pass m + 8 (one flag barrier of the row's two warps a tile tells), m is raised, O and the sum are
+// rescaled and the tile's pass is taken again from S, which is kept until then.
+// Warps 0–7: softmax (warps w and w + 4 share rows), warp 8: TMA producer, warp 9: TMEM owner and MMA issuer.
+// TMEM, 256 columns a CTA: two CTAs per SM, whose softmax and MMA phases overlap.  Up to 64 head dims 128 keys a tile
+// (S 128 | O 64 | P 64), above 64 keys (S 64 | P 32 | O 128).
 #pragma once
 #include "attn.cuh"
 
 namespace osam {
 
-constexpr int kAfRows = 128, kAfKeys = 128;
-constexpr int kAfThreads = 192;
-constexpr int kAfPanel = kAfRows * 128;  // bytes of a 64-dim panel of 128 rows
-constexpr float kAfGrow = 8.f;           // log2 growth of a row's maximum that forces a rescale
+constexpr int kAfRows = 128;
+constexpr int kAfSoft = 256;    // softmax threads
+constexpr int kAfThreads = kAfSoft + 64;
+constexpr float kAfGrow = 8.f;  // log2 growth over a row's reference maximum that forces a rescale
 
 template <int DP>
 struct AfCfg {
   static constexpr int PANELS = DP / 64;
-  static constexpr int STAGES = DP == 64 ? 2 : 1;
-  static constexpr bool EARLY = DP == 64;  // P beside S
-  static constexpr int COL_S = 0, COL_O = 128, COL_P = EARLY ? 192 : 0;
-  static constexpr int TILE = PANELS * kAfPanel;
-  static constexpr int SMEM = 1024 + TILE * (1 + 2 * STAGES);
+  static constexpr int KEYS = DP == 64 ? 128 : 64;  // per tile
+  static constexpr int CHUNKS = KEYS / 64;          // of 32 columns, per thread
+  static constexpr int STAGES = 2;
+  static constexpr int COL_S = 0, COL_P = DP == 64 ? 192 : 64, COL_O = 128;
+  static constexpr int QPANEL = kAfRows * 128, KPANEL = KEYS * 128;  // bytes of a 64-dim panel
+  static constexpr int QTILE = PANELS * QPANEL, TILE = PANELS * KPANEL;
+  static constexpr int SMEM = 1024 + QTILE + 2 * STAGES * TILE;
 };
 
 template <typename T, int DP, bool CAP, int BIAS>
 __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constant__ AttnFwdLaunch P) {
   using Cfg = AfCfg<DP>;
   constexpr bool BF16 = Half16<T>::kBf16;
+  constexpr int KEYS = Cfg::KEYS;
   extern __shared__ uint8_t af_raw[];
   __shared__ __align__(8) uint64_t k_full[Cfg::STAGES], k_empty[Cfg::STAGES], v_full[Cfg::STAGES], v_empty[Cfg::STAGES];
-  __shared__ __align__(8) uint64_t s_full, s_free, p_full, pv_done, drain;
+  __shared__ __align__(8) uint64_t s_full, p_full, pv_done, drain;
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t live[kAtDocWords], mix[kAtDocWords], pad[kAtDocWords];
   __shared__ AtDocs own_docs[4];
-  __shared__ __align__(16) int col_doc[2][kAfKeys];
-  __shared__ __align__(16) float2 col_cell[BIAS == 2 ? 2 : 1][kAfKeys];
+  __shared__ __align__(16) int col_doc[2][KEYS];
+  __shared__ __align__(16) float col_y[BIAS == 2 ? 2 : 1][KEYS], col_x[BIAS == 2 ? 2 : 1][KEYS];
+  __shared__ float pair_top[2][kAfRows], pair_sum[2][kAfRows];  // what the two threads of a row tell each other
 
   const AttnDev& A = P.d;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   uint8_t* smem = af_raw + ((1024 - (smem_u32(af_raw) & 1023)) & 1023);
-  const uint32_t sq = smem_u32(smem), sk = sq + Cfg::TILE, sv = sk + Cfg::STAGES * Cfg::TILE;
+  const uint32_t sq = smem_u32(smem), sk = sq + Cfg::QTILE, sv = sk + Cfg::STAGES * Cfg::TILE;
 
   // ---- which tile: with a causal bound the longest rows first
   const int rows = A.Lq * A.G, nq = (rows + kAfRows - 1) / kAfRows;
@@ -63,13 +69,14 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   const int lim_max = at_limit(A, n, prefix, off + r_last / A.G), lim_min = at_limit(A, n, prefix, off + r0 / A.G);
   AtTiles tiles;
   tiles.begin = split * P.tiles_per_split;
-  tiles.end = max(tiles.begin, min((lim_max + kAfKeys - 1) / kAfKeys, tiles.begin + P.tiles_per_split));
+  tiles.end = max(tiles.begin, min((lim_max + KEYS - 1) / KEYS, tiles.begin + P.tiles_per_split));
+  tiles.from = min(max((off + r_last / A.G) / KEYS, tiles.begin), tiles.end - 1);
   const bool docs = A.doc_q != nullptr;
   tiles.live = docs ? live : nullptr;
 
   // ---- this thread's row
-  const int r = r0 + tid;
-  const bool valid = warp < 4 && r < rows;
+  const int r = r0 + tid % kAfRows;
+  const bool valid = warp < 8 && r < rows;
   const int qi = valid ? r / A.G : 0, head = hk * A.G + (valid ? r - qi * A.G : 0);
   int my_doc = -2;
   if (valid && docs) {
@@ -85,34 +92,33 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       mbar_init(&v_empty[i], 1);
     }
     mbar_init(&s_full, 1);
-    mbar_init(&s_free, 4);
-    mbar_init(&p_full, 4);
+    mbar_init(&p_full, 8);
     mbar_init(&pv_done, 1);
     mbar_init(&drain, 1);
     fence_barrier_init();
     tma_prefetch_desc(&P.tk);
     tma_prefetch_desc(&P.tv);
   }
-  if (warp == 5) {
+  if (warp == 9) {
     tmem_alloc(&tmem_slot, 256);
     tmem_relinquish();
   }
-  if (warp < 4) {
+  if (warp < 8) {
     // Q rows into the K-major swizzled panels; rows past the end and dims past D are zero
     constexpr int CH = DP / 8;
     const T* q = static_cast<const T*>(P.q.p) + b * P.q.sb;
 #pragma unroll 8
-    for (int c = tid; c < kAfRows * CH; c += 128) {
+    for (int c = tid; c < kAfRows * CH; c += kAfSoft) {
       const int row = c / CH, ch = c % CH, rr = r0 + row;
       uint4 u = make_uint4(0, 0, 0, 0);
       if (rr < rows && ch * 8 < A.D) {
         const int i = rr / A.G, h = hk * A.G + rr - i * A.G;
         u = *reinterpret_cast<const uint4*>(q + i * P.q.st + h * P.q.sh + ch * 8);
       }
-      *reinterpret_cast<uint4*>(smem + (ch / 8) * kAfPanel + at_sw128(row, ch % 8)) = u;
+      *reinterpret_cast<uint4*>(smem + (ch / 8) * Cfg::QPANEL + at_sw128(row, ch % 8)) = u;
     }
     fence_proxy_async_smem();
-    if (docs) {
+    if (docs && warp < 4) {
       AtDocs d{my_doc >= 0 ? my_doc : INT_MAX, my_doc, valid && my_doc < 0, 0};
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -132,32 +138,32 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       own.pad |= own_docs[w].pad;
     }
     const int nb = (A.Lk + kAtDocBlock - 1) / kAtDocBlock;
-    at_doc_bits(own, A.sum_k + (long long)b * nb, nb, kAfKeys / kAtDocBlock, tiles.begin, tiles.end, warp,
+    at_doc_bits(own, A.sum_k + (long long)b * nb, nb, KEYS / kAtDocBlock, tiles.begin, tiles.end, warp,
                 kAfThreads / 32, live, mix, pad);
     __syncthreads();
   }
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp == 4) {
+  if (warp == 8) {
     if (lane == 0) {
       int it = 0;
       bool ok = true;
-      for (int t = tiles.first(); t < tiles.end; t = tiles.next(t + 1), it++) {
+      for (int t = tiles.first(); t < tiles.end; t = tiles.next(t), it++) {
         const int s = it % Cfg::STAGES;
         const uint32_t ph = ((it / Cfg::STAGES) & 1) ^ 1;
         if (it >= Cfg::STAGES && !(ok = mbar_wait(&k_empty[s], ph, A.err))) break;
         mbar_arrive_expect_tx(&k_full[s], Cfg::TILE);
         for (int p = 0; p < Cfg::PANELS; p++)
-          tma_load_4d(smem + (1 + s) * Cfg::TILE + p * kAfPanel, &P.tk, &k_full[s], p * 64, t * kAfKeys, hk, b);
+          tma_load_4d(smem + Cfg::QTILE + s * Cfg::TILE + p * Cfg::KPANEL, &P.tk, &k_full[s], p * 64, t * KEYS, hk, b);
         if (it >= Cfg::STAGES && !(ok = mbar_wait(&v_empty[s], ph, A.err))) {
           mbar_wait(&k_full[s], (it / Cfg::STAGES) & 1, A.err);
           break;
         }
         mbar_arrive_expect_tx(&v_full[s], Cfg::TILE);
         for (int p = 0; p < Cfg::PANELS; p++)
-          tma_load_4d(smem + (1 + Cfg::STAGES + s) * Cfg::TILE + p * kAfPanel, &P.tv, &v_full[s], p * 64, t * kAfKeys,
-                      hk, b);
+          tma_load_4d(smem + Cfg::QTILE + (Cfg::STAGES + s) * Cfg::TILE + p * Cfg::KPANEL, &P.tv, &v_full[s], p * 64,
+                      t * KEYS, hk, b);
       }
       // no copy of this CTA may be in flight when it ends
       for (int i = max(0, it - Cfg::STAGES); i < it; i++) {
@@ -166,189 +172,207 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       }
     }
     __syncwarp();
-  } else if (warp == 5) {
-    if (lane == 0) {
-      const int ks = (A.D + 15) / 16;  // K steps of Q·Kᵀ; N of P·V is 16·ks
-      const uint32_t id_s = at_idesc(BF16, 128, kAfKeys, false), id_o = at_idesc(BF16, 128, 16 * ks, true);
-      auto qk = [&](int it) {
-        const uint32_t kb = sk + (it % Cfg::STAGES) * Cfg::TILE;
-        for (int k = 0; k < ks; k++) {
-          const uint32_t o = (k / 4) * kAfPanel + (k % 4) * 32;
-          umma_f16(tmem + Cfg::COL_S, smem_desc_kmajor(sq + o, 128), smem_desc_kmajor(kb + o, 128), id_s, k > 0);
-        }
-        umma_commit(&k_empty[it % Cfg::STAGES]);
-        umma_commit(&s_full);
-      };
-      int it = 0, t = tiles.first();
-      bool ok = true;
-      if (t < tiles.end && (ok = mbar_wait(&k_full[0], 0, A.err))) {
-        tc_fence_after();
-        qk(0);
-      }
-      while (ok && t < tiles.end) {
-        const int tn = tiles.next(t + 1), s = it % Cfg::STAGES, s1 = (it + 1) % Cfg::STAGES;
-        const uint32_t ph = (it / Cfg::STAGES) & 1, ph1 = ((it + 1) / Cfg::STAGES) & 1;
-        if (Cfg::EARLY && tn < tiles.end) {
-          if (!(ok = mbar_wait(&k_full[s1], ph1, A.err) && mbar_wait(&s_free, it & 1, A.err))) break;
-          tc_fence_after();
-          qk(it + 1);
-        }
-        if (!(ok = mbar_wait(&v_full[s], ph, A.err) && mbar_wait(&p_full, it & 1, A.err))) break;
-        tc_fence_after();
-        const uint32_t vb = sv + s * Cfg::TILE;
+  } else if (warp == 9) {
+    const int ks = (A.D + 15) / 16;  // K steps of Q·Kᵀ; N of P·V is 16·ks
+    const uint32_t id_s = at_idesc(BF16, 128, KEYS, false), id_o = at_idesc(BF16, 128, 16 * ks, true);
+    const uint64_t dq = smem_desc_kmajor(sq, 128), dk = smem_desc_kmajor(sk, 128), dv = at_desc_mn(sv, Cfg::KPANEL);
+    const int count = __shfl_sync(0xffffffffu, tiles.count(), 0);
+    auto qk = [&](int it) {  // offsets in a descriptor: bytes / 16
+      const uint64_t kb = dk + ((it % Cfg::STAGES) * Cfg::TILE >> 4);
 #pragma unroll
-        for (int k = 0; k < kAfKeys / 16; k++)
-          umma_f16_ts(tmem + Cfg::COL_O, tmem + Cfg::COL_P + k * 8, at_desc_mn(vb + k * 16 * 128, kAfPanel), id_o,
-                      (it | k) != 0);
-        umma_commit(&v_empty[s]);
-        umma_commit(&pv_done);
-        if (!Cfg::EARLY && tn < tiles.end) {
-          if (!(ok = mbar_wait(&k_full[s1], ph1, A.err))) break;
-          tc_fence_after();
-          qk(it + 1);
-        }
-        t = tn;
-        it++;
-      }
-      if (!ok) {  // let the issued MMAs finish before TMEM is freed
-        umma_commit(&drain);
-        mbar_wait(&drain, 0, A.err);
-      }
+      for (int k = 0; k < DP / 16; k++)
+        if (k < ks)
+          mma_ss(tmem + Cfg::COL_S, dq + (((k / 4) * Cfg::QPANEL + (k % 4) * 32) >> 4),
+                 kb + (((k / 4) * Cfg::KPANEL + (k % 4) * 32) >> 4), id_s, k > 0);
+      mma_commit(&k_empty[it % Cfg::STAGES]);
+      mma_commit(&s_full);
+    };
+    bool ok = true;
+    if (count > 0 && (ok = at_wait_warp(&k_full[0], 0, A.err))) {
+      tc_fence_after();
+      qk(0);
     }
-    __syncwarp();
+    for (int it = 0; ok && it < count; it++) {
+      const int s = it % Cfg::STAGES, s1 = (it + 1) % Cfg::STAGES;
+      if (it + 1 < count && !(ok = at_wait_warp(&k_full[s1], ((it + 1) / Cfg::STAGES) & 1, A.err))) break;
+      if (!(ok = at_wait_warp(&v_full[s], (it / Cfg::STAGES) & 1, A.err))) break;
+      if (!(ok = at_wait_warp(&p_full, it & 1, A.err))) break;
+      tc_fence_after();
+      if (it + 1 < count) qk(it + 1);  // S is free once P is written
+      const uint64_t vb = dv + (s * Cfg::TILE >> 4);
+#pragma unroll
+      for (int k = 0; k < KEYS / 16; k++)
+        mma_ts(tmem + Cfg::COL_O, tmem + Cfg::COL_P + k * 8, vb + (k * 16 * 128 >> 4), id_o, (it | k) != 0);
+      mma_commit(&v_empty[s]);
+      mma_commit(&pv_done);
+    }
+    if (!ok) {  // let the issued MMAs finish before TMEM is freed
+      mma_commit(&drain);
+      at_wait_warp(&drain, 0, A.err);
+    }
   } else {
-    const uint32_t lane_base = uint32_t(warp * 32) << 16;
-    const bool idle = r0 + warp * 32 >= rows;  // no row of this warp exists: it only keeps step
+    const int wg = warp / 4, row_of = tid % kAfRows, pair_bar = 2 + warp % 4;
+    const int c0 = wg * (KEYS / 2);  // first column of this thread
+    const uint32_t lane_base = uint32_t((warp % 4) * 32) << 16;
+    const bool idle = r0 + (warp % 4) * 32 >= rows;  // no row of this warp exists: it only keeps step
     const int pos = off + qi;
     const int lim = valid ? at_limit(A, n, prefix, pos) : 0;
-    // scores in log2 units are x·cmul: the scale is applied with the exponent's FMA when nothing else needs it
-    const float cmul = CAP || BIAS ? 1.f : A.scale * kAtLog2e;
-    const float cap2 = A.cap * kAtLog2e, cap_in = CAP ? 2.f * A.scale * kAtLog2e / A.cap : 0.f;
-    const float slope = BIAS && valid ? A.slopes[head] * kAtLog2e : 0.f;
-    const float2 cell = BIAS == 2 ? at_cell(A, pos) : make_float2(0.f, 0.f);
-    float m = -INFINITY, l = 0.f;  // reference maximum (log2 units) and sum
+    AtBias bias;
+    bias.mul = CAP ? 2.f * A.scale * kAtLog2e / A.cap : A.scale * kAtLog2e;
+    bias.cap2 = A.cap * kAtLog2e;
+    bias.slope = BIAS && valid ? A.slopes[head] * kAtLog2e : 0.f;
+    bias.y = bias.x = 0.f;
+    if (BIAS == 2) {
+      const float2 cell = at_cell(A, pos);
+      bias.y = cell.x * bias.slope;
+      bias.x = cell.y * bias.slope;
+    }
+    float m = valid ? -INFINITY : 0.f;  // the row's reference maximum, log2 units (−∞: nothing seen yet)
+    float l = 0.f;                      // this thread's part of the row's sum
     int it = 0;
     bool ok = true;
-    for (int t = tiles.first(); t < tiles.end; t = tiles.next(t + 1), it++) {
-      const int j0 = t * kAfKeys;
+    for (int t = tiles.first(); t < tiles.end; t = tiles.next(t), it++) {
+      const int j0 = t * KEYS;
       const bool by_doc = docs && at_bit(mix, t - tiles.begin);
-      const bool dirty = (n < A.Lk && j0 + kAfKeys > n) || (docs && at_bit(pad, t - tiles.begin));
-      int key_doc = 0;
+      const bool masked = by_doc || j0 + KEYS > lim_min;
+      const bool dirty = (n < A.Lk && j0 + KEYS > n) || (docs && at_bit(pad, t - tiles.begin));
       if (by_doc || BIAS == 2) {  // per-key data of the tile, one key a thread
-        if (docs) {
-          key_doc = j0 + tid < n ? A.doc_k[(long long)b * A.Lk + j0 + tid] : -1;
-          col_doc[it & 1][tid] = key_doc < 0 ? -1 : key_doc;
+        if (tid < KEYS) {
+          const int j = j0 + tid;
+          if (docs) {
+            const int id = j < n ? A.doc_k[(long long)b * A.Lk + j] : -1;
+            col_doc[it & 1][tid] = id < 0 ? -1 : id;
+          }
+          if (BIAS == 2) {
+            const float2 cell = at_cell(A, j);
+            col_y[it & 1][tid] = cell.x;
+            col_x[it & 1][tid] = cell.y;
+          }
         }
-        if (BIAS == 2) col_cell[it & 1][tid] = at_cell(A, j0 + tid);
-        named_bar_sync(1, 128);
+        named_bar_sync(1, kAfSoft);
       }
       if (!(ok = at_wait_warp(&s_full, it & 1, A.err))) break;
       tc_fence_after();
-      float x[kAfKeys];
-#pragma unroll
-      for (int c = 0; c < kAfKeys; c += 32) tmem_ld32_nowait(tmem + lane_base + Cfg::COL_S + c, x + c);
-      tmem_wait_ld();
-      if (Cfg::EARLY) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free);
-      }
-      if (!idle) {
-        if (CAP) {
-#pragma unroll
-          for (int c = 0; c < kAfKeys; c++)
-            x[c] = fmaf(-2.f * cap2, at_rcp(1.f + at_ex2(x[c] * cap_in)), cap2);
-        } else if (BIAS) {
-#pragma unroll
-          for (int c = 0; c < kAfKeys; c++) x[c] *= A.scale * kAtLog2e;
+
+      // Scores of chunk k in log2 units plus `add`; returns their maximum.
+      auto scores = [&](int k, float add, float (&x)[32]) {
+        const int c1 = c0 + 32 * k;
+        tmem_ld32_nowait(tmem + lane_base + Cfg::COL_S + c1, x);
+        uint32_t vis = 0xffffffffu;
+        if (masked) {
+          vis = at_low_bits(lim - j0 - c1);
+          if (by_doc) vis &= at_doc_bits32(&col_doc[it & 1][c1], my_doc);
         }
-        if (BIAS == 1) {
-          const float rel = float(pos - j0);
+        if (BIAS == 1) bias.y = float(pos - j0 - c1) * bias.slope;
+        AtLine line;
+        if (BIAS == 1) line.start(bias);
+        tmem_wait_ld();
+        if (CAP && masked) at_mask32(x, vis, 0.f);
+        const float2 add2x[2] = {make_float2(add, add), make_float2(add, add)};
 #pragma unroll
-          for (int c = 0; c < kAfKeys; c++) x[c] = fmaf(-slope, fabsf(rel - float(c)), x[c]);
-        }
-        if (BIAS == 2) {
-          const float4* cells = reinterpret_cast<const float4*>(col_cell[it & 1]);
-#pragma unroll
-          for (int c = 0; c < kAfKeys; c += 2) {
-            const float4 k2 = cells[c / 2];
-            x[c] = fmaf(-slope, fabsf(cell.x - k2.x) + fabsf(cell.y - k2.y), x[c]);
-            x[c + 1] = fmaf(-slope, fabsf(cell.x - k2.z) + fabsf(cell.y - k2.w), x[c + 1]);
+        for (int c = 0; c < 32; c += 4) {
+          float2 s2[2] = {make_float2(x[c], x[c + 1]), make_float2(x[c + 2], x[c + 3])}, sig[2];
+          float4 ky = {}, kx = {};
+          if (BIAS == 2) {
+            ky = *reinterpret_cast<const float4*>(&col_y[it & 1][c1 + c]);
+            kx = *reinterpret_cast<const float4*>(&col_x[it & 1][c1 + c]);
           }
+          at_scores4<CAP, BIAS>(bias, s2, add2x, line, ky, kx, sig);
+          x[c] = s2[0].x;
+          x[c + 1] = s2[0].y;
+          x[c + 2] = s2[1].x;
+          x[c + 3] = s2[1].y;
         }
-        if (j0 + kAfKeys > lim_min) {
-          const int e = lim - j0;
+        if (masked) at_mask32(x, vis, -INFINITY);
+        float top = fmaxf(x[0], x[1]), top1 = fmaxf(x[2], x[3]);
 #pragma unroll
-          for (int c = 0; c < kAfKeys; c++) x[c] = c < e ? x[c] : -INFINITY;
+        for (int c = 4; c < 32; c += 4) {
+          top = fmaxf(fmaxf(top, x[c]), x[c + 1]);
+          top1 = fmaxf(fmaxf(top1, x[c + 2]), x[c + 3]);
         }
-        if (by_doc) {
-          const int4* kd = reinterpret_cast<const int4*>(col_doc[it & 1]);
+        return fmaxf(top, top1);
+      };
+      // Raises the reference m of rows whose scores' maximum `over` (of this thread's columns, relative to `base`) calls
+      // for it; returns the factor by which what was summed against the old one has to be multiplied.
+      auto raise = [&](float over, float base) {
+        pair_top[wg][row_of] = over;
+        named_bar_sync(pair_bar, 64);
+        over = fmaxf(over, pair_top[wg ^ 1][row_of]);
+        if (m == -INFINITY ? !(over > -INFINITY) : !(over > kAfGrow)) return 1.f;
+        const float old = m;
+        m = base + over;
+        const float f = old == -INFINITY ? 0.f : at_ex2(old - m);
+        l *= f;
+        return f;
+      };
+      auto rescale = [&](float f) {
+#pragma unroll 1
+        for (int c = wg * (DP / 2); c < (wg + 1) * (DP / 2); c += 16) {
+          float o[16];
+          tmem_ld16(tmem + lane_base + Cfg::COL_O + c, o);
 #pragma unroll
-          for (int c = 0; c < kAfKeys; c += 4) {
-            const int4 d = kd[c / 4];
-            x[c] = d.x == my_doc ? x[c] : -INFINITY;
-            x[c + 1] = d.y == my_doc ? x[c + 1] : -INFINITY;
-            x[c + 2] = d.z == my_doc ? x[c + 2] : -INFINITY;
-            x[c + 3] = d.w == my_doc ? x[c + 3] : -INFINITY;
+          for (int i = 0; i < 16; i++) o[i] = f == 0.f ? 0.f : o[i] * f;
+          tmem_st16(tmem + lane_base + Cfg::COL_O + c, reinterpret_cast<const uint32_t*>(o));
+        }
+      };
+
+      bool pv_waited = it == 0;  // P and O are free once the previous P·V is done
+      if (__any_sync(0xffffffffu, m == -INFINITY)) {  // the same in both warps of the rows
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int k = 0; k < Cfg::CHUNKS; k++) {
+          float x[32];
+          top = fmaxf(top, scores(k, 0.f, x));
+        }
+        // rows that have a reference already go on with it: the pass below finds out if it is too low
+        const float f = raise(m == -INFINITY ? top : -INFINITY, 0.f);
+        if (it > 0) {
+          if (!(ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err))) break;
+          tc_fence_after();
+          pv_waited = true;
+          rescale(f);
+        }
+      }
+      const float l0 = l;
+      for (int pass = 0;; pass++) {
+        float over = -INFINITY;  // largest score over the reference
+        if (!idle) {
+          const float neg = m == -INFINITY ? 0.f : -m;
+          float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+          for (int k = 0; k < Cfg::CHUNKS; k++) {
+            float x[32];
+            over = fmaxf(over, scores(k, neg, x));
+            uint32_t p[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const float2 e = make_float2(at_ex2(x[2 * i]), at_ex2(x[2 * i + 1]));
+              sum[i & 1] = add2(sum[i & 1], e);
+              p[i] = Half16<T>::pack(e.x, e.y);
+            }
+            if (!pv_waited) {
+              if (!(ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err))) break;
+              tc_fence_after();
+              pv_waited = true;
+            }
+            tmem_st16(tmem + lane_base + Cfg::COL_P + (c0 + 32 * k) / 2, p);
           }
+          const float2 s = add2(sum[0], sum[1]);
+          l = s.x + s.y;
         }
+        if (!at_pair_any(pair_bar, over > kAfGrow && pass == 0) || !ok) break;
+        l = l0;  // rare: take the tile once more against the raised reference
+        const float f = raise(over, m);
+        if (it > 0) rescale(f);
       }
-      float factor = 1.f;
-      if (!idle) {
-        float top4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-        for (int c = 4; c < kAfKeys; c++) top4[c % 4] = fmaxf(top4[c % 4], x[c]);
-        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * cmul;
-        if (top > m + kAfGrow || (m == -INFINITY && top > -INFINITY)) {
-          factor = m == -INFINITY ? 0.f : at_ex2(m - top);
-          m = top;
-          l *= factor;
-        }
-      }
-      // O and P are free once the previous P·V is done
-      if (it > 0) {
-        if (!(ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err))) break;
-        tc_fence_after();
-        if (__any_sync(0xffffffffu, factor != 1.f)) {
-#pragma unroll
-          for (int c = 0; c < DP; c += 16) {
-            float o[16];
-            tmem_ld16(tmem + lane_base + Cfg::COL_O + c, o);
-#pragma unroll
-            for (int i = 0; i < 16; i++) o[i] = factor == 0.f ? 0.f : o[i] * factor;
-            tmem_st16(tmem + lane_base + Cfg::COL_O + c, reinterpret_cast<const uint32_t*>(o));
-          }
-        }
-      }
-      if (!idle) {
-        const float neg = m == -INFINITY ? 0.f : -m;
-        const float2 mul = make_float2(cmul, cmul), add = make_float2(neg, neg);
-        float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-        for (int c = 0; c < kAfKeys; c += 64) {
-          uint32_t p[32];
-#pragma unroll
-          for (int i = 0; i < 32; i++) {
-            float2 e = make_float2(x[c + 2 * i], x[c + 2 * i + 1]);
-            e = CAP || BIAS ? add2(e, add) : fma2(e, mul, add);
-            e.x = at_ex2(e.x);
-            e.y = at_ex2(e.y);
-            sum[i & 1] = add2(sum[i & 1], e);
-            p[i] = Half16<T>::pack(e.x, e.y);
-          }
-          tmem_st32(tmem + lane_base + Cfg::COL_P + c / 2, p);
-        }
-        const float2 s = add2(sum[0], sum[1]);
-        l = s.x + s.y;
-      }
+      if (!ok) break;
       if (dirty) {  // V rows of keys that no query sees hold anything, NaN included: 0·NaN must not enter O
         if (!(ok = at_wait_warp(&v_full[it % Cfg::STAGES], (it / Cfg::STAGES) & 1, A.err))) break;
-        const int j = j0 + tid;
-        if (j >= n || (docs && A.doc_k[(long long)b * A.Lk + j] < 0)) {
-          uint8_t* v = smem + (1 + Cfg::STAGES + it % Cfg::STAGES) * Cfg::TILE + tid * 128;
-          for (int p = 0; p < Cfg::PANELS; p++)
+        const int key = tid % KEYS, j = j0 + key, panel = tid / KEYS;
+        if (panel < Cfg::PANELS && (j >= n || (docs && A.doc_k[(long long)b * A.Lk + j] < 0))) {
+          uint8_t* v = smem + Cfg::QTILE + (Cfg::STAGES + it % Cfg::STAGES) * Cfg::TILE + panel * Cfg::KPANEL + key * 128;
 #pragma unroll
-            for (int c = 0; c < 8; c++) *reinterpret_cast<uint4*>(v + p * kAfPanel + c * 16) = make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < 8; c++) *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
       }
@@ -360,23 +384,23 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     if (ok && it > 0) ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err);
     if (ok) {
       tc_fence_after();
+      pair_sum[wg][row_of] = l;
+      named_bar_sync(pair_bar, 64);
+      l += pair_sum[wg ^ 1][row_of];
       const long long row = ((long long)b * A.Hq + head) * A.Lq + qi;
       const long long part_row = (long long)split * A.B * A.Hq * A.Lq + row;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays one
       T* o_ptr = static_cast<T*>(P.o.p) + b * P.o.sb + qi * P.o.st + head * P.o.sh;
 #pragma unroll
-      for (int c = 0; c < DP; c += 32) {
+      for (int c = wg * (DP / 2); c < (wg + 1) * (DP / 2); c += 16) {
         if (c >= A.D) break;
-        float o[32];
-        if (it > 0) {
-          tmem_ld32_nowait(tmem + lane_base + Cfg::COL_O + c, o);
-          tmem_wait_ld();
-        }
+        float o[16];
+        if (it > 0) tmem_ld16(tmem + lane_base + Cfg::COL_O + c, o);
 #pragma unroll
-        for (int i = 0; i < 32; i++) o[i] = it > 0 && l != 0.f ? o[i] : 0.f;
+        for (int i = 0; i < 16; i++) o[i] = it > 0 && l != 0.f ? o[i] : 0.f;
         if (!valid) continue;
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
+        for (int i = 0; i < 16; i += 8) {
           if (c + i >= A.D) break;
           float v8[8];
 #pragma unroll
@@ -392,7 +416,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
           }
         }
       }
-      if (valid) {
+      if (valid && wg == 0) {
         if (P.splits > 1)
           P.stats[part_row] = make_float2(m, l);
         else if (P.lse)
@@ -402,7 +426,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem, 256);
   }
