@@ -190,7 +190,7 @@ struct AtSplit {
   int splits, tiles;
 };
 AtSplit at_split(const osam_attn_desc& a) {
-  const int keys = attn_fwd_tile_keys(a.dim), tiles = (a.len_k + keys - 1) / keys;
+  const int keys = 64, tiles = (a.len_k + keys - 1) / keys;
   const long long ctas = (((long long)a.len_q * (a.heads_q / a.heads_k) + 127) / 128) * a.batch * a.heads_k;
   AtSplit s{1, std::max(tiles, 1)};
   if (ctas == 0 || a.len_k < 512 || ctas >= 2 * kAtSms) return s;
@@ -293,7 +293,7 @@ int osam_attn_fwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   AttnFwdLaunch L{};
   if ((rc = at_dev(*a, W, w, &L.d, st)) != OSAM_OK) return rc;
   const bool bf16 = a->dtype == OSAM_BF16;
-  const int keys = attn_fwd_tile_keys(a->dim);
+  const int keys = 64;
   // without keys every query is empty: no tile is visited, so the maps only have to be valid
   const osam_view& kk = a->len_k > 0 ? k : q;
   const osam_view& vv = a->len_k > 0 ? v : q;

@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
       int it = 0;
       for (; x.more(tiles, streams); x.step(tiles), it++) {
         const int s = it % Cfg::STAGES;
-        if (it >= Cfg::STAGES && !mbar_wait(&empty[s], ((it / Cfg::STAGES) & 1) ^ 1, A.err)) break;
+        if (it >= Cfg::STAGES && !at_wait(&empty[s], ((it / Cfg::STAGES) & 1) ^ 1, A.err)) break;
         uint8_t* d = strm + s * 2 * Cfg::STRM;
         mbar_arrive_expect_tx(&full[s], 2 * Cfg::STRM + (DKV ? Cfg::ROWS : 0));
         const int h = DKV ? hd * A.G + x.g : hd / A.G;
@@ -175,11 +175,12 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
                     &full[s]);
       }
       // no copy of this CTA may be in flight when it ends
-      if (any) mbar_wait(&stat_full, 0, A.err);
-      for (int i = max(0, it - Cfg::STAGES); i < it; i++) mbar_wait(&full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, A.err);
+      if (any) at_wait(&stat_full, 0, A.err);
+      for (int i = max(0, it - Cfg::STAGES); i < it; i++) at_wait(&full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, A.err);
     }
     __syncwarp();
   } else if (warp == 8 * NB + 1) {
+    const uint32_t leader = elect_leader();
     const int ks = (A.D + 15) / 16;
     const uint32_t id_x = at_idesc(BF16, 128, kAbCols, false), id_g = at_idesc(BF16, 128, 16 * ks, true);
     const uint32_t a1 = smem_u32(smem), sb = smem_u32(strm);
@@ -193,14 +194,14 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
 #pragma unroll
       for (int k = 0; k < DP / 16; k++)
         if (k < ks)
-          mma_ss(d, da1 + (((k / 4) * kAbRows * 128 + (k % 4) * 32) >> 4),
+          mma_ss(leader, d, da1 + (((k / 4) * kAbRows * 128 + (k % 4) * 32) >> 4),
                  b1 + (((k / 4) * kAbCols * 128 + (k % 4) * 32) >> 4), id_x, k > 0);
 #pragma unroll
       for (int k = 0; k < DP / 16; k++)
         if (k < ks)
-          mma_ss(d + 64, da2 + (((k / 4) * kAbRows * 128 + (k % 4) * 32) >> 4),
+          mma_ss(leader, d + 64, da2 + (((k / 4) * kAbRows * 128 + (k % 4) * 32) >> 4),
                  b2 + (((k / 4) * kAbCols * 128 + (k % 4) * 32) >> 4), id_x, k > 0);
-      mma_commit(&xy_full[it % NB]);
+      mma_commit(leader, &xy_full[it % NB]);
     };
     bool ok = count == 0 || at_wait_warp(&stat_full, 0, A.err);
     for (int it = 0; ok && it < NB && it < count; it++) {
@@ -217,19 +218,19 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
       if (DKV) {
 #pragma unroll
         for (int k = 0; k < kAbCols / 16; k++)
-          mma_ts(tmem + Cfg::COL_ACC2, d + k / 2 * 32 + k % 2 * 8, g2 + (k * 16 * 128 >> 4), id_g, (it | k) != 0);
+          mma_ts(leader, tmem + Cfg::COL_ACC2, d + k / 2 * 32 + k % 2 * 8, g2 + (k * 16 * 128 >> 4), id_g, (it | k) != 0);
       }
 #pragma unroll
       for (int k = 0; k < kAbCols / 16; k++)
-        mma_ts(tmem + Cfg::COL_ACC1, d + 64 + k / 2 * 32 + k % 2 * 8, g1 + (k * 16 * 128 >> 4), id_g, (it | k) != 0);
-      mma_commit(&empty[s]);
+        mma_ts(leader, tmem + Cfg::COL_ACC1, d + 64 + k / 2 * 32 + k % 2 * 8, g1 + (k * 16 * 128 >> 4), id_g, (it | k) != 0);
+      mma_commit(leader, &empty[s]);
       if (ia < count) {
         if (!(ok = at_wait_warp(&full[ia % Cfg::STAGES], (ia / Cfg::STAGES) & 1, A.err))) break;
         tc_fence_after();
         scores(ia);
       }
     }
-    mma_commit(&acc_done);
+    mma_commit(leader, &acc_done);
     if (!ok) at_wait_warp(&acc_done, 0, A.err);  // the issued MMAs finish before TMEM is freed
   } else {
     const int buf = warp / 8, half = warp / 4 % 2, r = tid % 128;
@@ -318,9 +319,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
       if (BIAS == 1) bias.y = float(pos - (DKV ? off + c0 : c0) - h0) * bias.slope;
       const uint32_t xcol = tmem + lane_base + buf * 128;
       float sv[32], dp[32];
-      tmem_ld32_nowait(xcol + h0, sv);
-      tmem_ld32_nowait(xcol + 64 + h0, dp);
-      tmem_wait_ld();
+      at_ld32x2(xcol + h0, sv, xcol + 64 + h0, dp);
       uint32_t vis = 0xffffffffu;
       if (by_lim || by_doc) {  // hidden: p = 0 and ds = 0 whatever the operands hold
         vis = DKV ? (from == INT_MAX ? 0u : ~at_low_bits(from - c0 - h0)) : at_low_bits(lim - c0 - h0);
@@ -408,7 +407,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
         const int lo = me % parts * (DP / parts), hi = lo + DP / parts;
         for (int c = lo; c < hi && c < A.D; c += 16) {
           float a[16];
-          if (any) tmem_ld16(acc + c, a);
+          if (any) at_ld16(acc + c, a);
 #pragma unroll
           for (int i = 0; i < 16; i++) a[i] = any ? a[i] * f : 0.f;
           if (!valid) continue;

@@ -3,34 +3,30 @@
 // single token of many heads still fills rows.  Long caches with few rows are split over the keys: each split
 // writes its unnormalised output with its maximum and sum, and k_attn_join (attn.cu) adds them.
 //
-// Per key tile:  S = Q·Kᵀ (tcgen05, fp32 in TMEM) → two threads per row (half of the columns each) read its scores from
-// TMEM 32 at a time, apply cap, bias and masks, take p = 2^(x − m) against the row's reference maximum m and write
-// P in 16 bits back to TMEM → O += P·V with P as the TMEM operand.  A row is a TMEM lane, so its maximum and sum need no
-// shuffles.  m is taken from the first tile and kept while scores stay below m + 8 (P ≤ 2^8 keeps its relative
-// precision in 16 bits, the sum is fp32): scores turn into P in one pass, without waiting for the tile's maximum.
-// When a score does pass m + 8 (one flag barrier of the row's two warps a tile tells), m is raised, O and the sum are
-// rescaled and the tile's pass is taken again from S, which is kept until then.
-// Warps 0–7: softmax (warps w and w + 4 share rows), warp 8: TMA producer, warp 9: TMEM owner and MMA issuer.
-// TMEM, 256 columns a CTA: two CTAs per SM, whose softmax and MMA phases overlap.  Up to 64 head dims 128 keys a tile
-// (S 128 | O 64 | P 64), above 64 keys (S 64 | P 32 | O 128).
+// Per 64-key tile:  S = Q·Kᵀ (tcgen05, fp32 in TMEM) → one thread per row reads its 64 scores into registers, applies cap,
+// bias and masks, takes p = 2^(x − m) against the row's reference maximum m and writes P in 16 bits back to TMEM → O +=
+// P·V with P as the TMEM operand.  A row is a TMEM lane: its maximum and sum need no shuffles.  m follows the
+// maximum only when a tile exceeds it by more than 2^8 (P ≤ 2^8 keeps its relative precision in 16 bits, the sum is
+// fp32): then O, which stays in TMEM, is rescaled.  Tiles are visited from the CTA's own positions outwards, so that
+// with a distance bias the largest scores come first and this stays rare.
+// Warps 0–3: softmax, warp 4: TMA producer, warp 5: TMEM owner and MMA issuer.  TMEM, 256 columns a CTA (two CTAs per
+// SM): S, which the next tile's Q·Kᵀ overwrites as soon as it is in registers, two buffers of P, and O.
 #pragma once
 #include "attn.cuh"
 
 namespace osam {
 
-constexpr int kAfRows = 128;
-constexpr int kAfSoft = 256;    // softmax threads
+constexpr int kAfRows = 128, kAfKeys = 64;
+constexpr int kAfSoft = 128;    // softmax threads
 constexpr int kAfThreads = kAfSoft + 64;
 constexpr float kAfGrow = 8.f;  // log2 growth over a row's reference maximum that forces a rescale
 
 template <int DP>
 struct AfCfg {
   static constexpr int PANELS = DP / 64;
-  static constexpr int KEYS = DP == 64 ? 128 : 64;  // per tile
-  static constexpr int CHUNKS = KEYS / 64;          // of 32 columns, per thread
-  static constexpr int STAGES = 2;
-  static constexpr int COL_S = 0, COL_P = DP == 64 ? 192 : 64, COL_O = 128;
-  static constexpr int QPANEL = kAfRows * 128, KPANEL = KEYS * 128;  // bytes of a 64-dim panel
+  static constexpr int STAGES = DP == 64 ? 4 : 2;
+  static constexpr int COL_S = 0, COL_P = 64, COL_O = 128;  // P buffer i at COL_P + 32·i
+  static constexpr int QPANEL = kAfRows * 128, KPANEL = kAfKeys * 128;  // bytes of a 64-dim panel
   static constexpr int QTILE = PANELS * QPANEL, TILE = PANELS * KPANEL;
   static constexpr int SMEM = 1024 + QTILE + 2 * STAGES * TILE;
 };
@@ -39,16 +35,15 @@ template <typename T, int DP, bool CAP, int BIAS>
 __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constant__ AttnFwdLaunch P) {
   using Cfg = AfCfg<DP>;
   constexpr bool BF16 = Half16<T>::kBf16;
-  constexpr int KEYS = Cfg::KEYS;
+  constexpr int KEYS = kAfKeys;
   extern __shared__ uint8_t af_raw[];
   __shared__ __align__(8) uint64_t k_full[Cfg::STAGES], k_empty[Cfg::STAGES], v_full[Cfg::STAGES], v_empty[Cfg::STAGES];
-  __shared__ __align__(8) uint64_t s_full, p_full, pv_done, drain;
+  __shared__ __align__(8) uint64_t s_full, s_free, p_full[2], pv_done, o_done;
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t live[kAtDocWords], mix[kAtDocWords], pad[kAtDocWords];
   __shared__ AtDocs own_docs[4];
   __shared__ __align__(16) int col_doc[2][KEYS];
   __shared__ __align__(16) float col_y[BIAS == 2 ? 2 : 1][KEYS], col_x[BIAS == 2 ? 2 : 1][KEYS];
-  __shared__ float pair_top[2][kAfRows], pair_sum[2][kAfRows];  // what the two threads of a row tell each other
 
   const AttnDev& A = P.d;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -75,8 +70,8 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   tiles.live = docs ? live : nullptr;
 
   // ---- this thread's row
-  const int r = r0 + tid % kAfRows;
-  const bool valid = warp < 8 && r < rows;
+  const int r = r0 + tid;
+  const bool valid = warp < 4 && r < rows;
   const int qi = valid ? r / A.G : 0, head = hk * A.G + (valid ? r - qi * A.G : 0);
   int my_doc = -2;
   if (valid && docs) {
@@ -92,18 +87,20 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       mbar_init(&v_empty[i], 1);
     }
     mbar_init(&s_full, 1);
-    mbar_init(&p_full, 8);
+    mbar_init(&s_free, 4);
+    mbar_init(&p_full[0], 4);  // two: a warp may be a tile ahead of another
+    mbar_init(&p_full[1], 4);
     mbar_init(&pv_done, 1);
-    mbar_init(&drain, 1);
+    mbar_init(&o_done, 1);
     fence_barrier_init();
     tma_prefetch_desc(&P.tk);
     tma_prefetch_desc(&P.tv);
   }
-  if (warp == 9) {
+  if (warp == 5) {
     tmem_alloc(&tmem_slot, 256);
     tmem_relinquish();
   }
-  if (warp < 8) {
+  if (warp < 4) {
     // Q rows into the K-major swizzled panels; rows past the end and dims past D are zero
     constexpr int CH = DP / 8;
     const T* q = static_cast<const T*>(P.q.p) + b * P.q.sb;
@@ -118,7 +115,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       *reinterpret_cast<uint4*>(smem + (ch / 8) * Cfg::QPANEL + at_sw128(row, ch % 8)) = u;
     }
     fence_proxy_async_smem();
-    if (docs && warp < 4) {
+    if (docs) {
       AtDocs d{my_doc >= 0 ? my_doc : INT_MAX, my_doc, valid && my_doc < 0, 0};
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -145,19 +142,19 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp == 8) {
+  if (warp == 4) {
     if (lane == 0) {
       int it = 0;
       bool ok = true;
       for (int t = tiles.first(); t < tiles.end; t = tiles.next(t), it++) {
         const int s = it % Cfg::STAGES;
         const uint32_t ph = ((it / Cfg::STAGES) & 1) ^ 1;
-        if (it >= Cfg::STAGES && !(ok = mbar_wait(&k_empty[s], ph, A.err))) break;
+        if (it >= Cfg::STAGES && !(ok = at_wait(&k_empty[s], ph, A.err))) break;
         mbar_arrive_expect_tx(&k_full[s], Cfg::TILE);
         for (int p = 0; p < Cfg::PANELS; p++)
           tma_load_4d(smem + Cfg::QTILE + s * Cfg::TILE + p * Cfg::KPANEL, &P.tk, &k_full[s], p * 64, t * KEYS, hk, b);
-        if (it >= Cfg::STAGES && !(ok = mbar_wait(&v_empty[s], ph, A.err))) {
-          mbar_wait(&k_full[s], (it / Cfg::STAGES) & 1, A.err);
+        if (it >= Cfg::STAGES && !(ok = at_wait(&v_empty[s], ph, A.err))) {
+          at_wait(&k_full[s], (it / Cfg::STAGES) & 1, A.err);
           break;
         }
         mbar_arrive_expect_tx(&v_full[s], Cfg::TILE);
@@ -167,12 +164,13 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       }
       // no copy of this CTA may be in flight when it ends
       for (int i = max(0, it - Cfg::STAGES); i < it; i++) {
-        mbar_wait(&k_full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, A.err);
-        mbar_wait(&v_full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, A.err);
+        at_wait(&k_full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, A.err);
+        at_wait(&v_full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, A.err);
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == 5) {
+    const uint32_t leader = elect_leader();
     const int ks = (A.D + 15) / 16;  // K steps of Q·Kᵀ; N of P·V is 16·ks
     const uint32_t id_s = at_idesc(BF16, 128, KEYS, false), id_o = at_idesc(BF16, 128, 16 * ks, true);
     const uint64_t dq = smem_desc_kmajor(sq, 128), dk = smem_desc_kmajor(sk, 128), dv = at_desc_mn(sv, Cfg::KPANEL);
@@ -182,10 +180,10 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
 #pragma unroll
       for (int k = 0; k < DP / 16; k++)
         if (k < ks)
-          mma_ss(tmem + Cfg::COL_S, dq + (((k / 4) * Cfg::QPANEL + (k % 4) * 32) >> 4),
+          mma_ss(leader, tmem + Cfg::COL_S, dq + (((k / 4) * Cfg::QPANEL + (k % 4) * 32) >> 4),
                  kb + (((k / 4) * Cfg::KPANEL + (k % 4) * 32) >> 4), id_s, k > 0);
-      mma_commit(&k_empty[it % Cfg::STAGES]);
-      mma_commit(&s_full);
+      mma_commit(leader, &s_full);
+      mma_commit(leader, &k_empty[it % Cfg::STAGES]);
     };
     bool ok = true;
     if (count > 0 && (ok = at_wait_warp(&k_full[0], 0, A.err))) {
@@ -194,29 +192,31 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     }
     for (int it = 0; ok && it < count; it++) {
       const int s = it % Cfg::STAGES, s1 = (it + 1) % Cfg::STAGES;
-      if (it + 1 < count && !(ok = at_wait_warp(&k_full[s1], ((it + 1) / Cfg::STAGES) & 1, A.err))) break;
+      if (it + 1 < count) {
+        if (!(ok = at_wait_warp(&k_full[s1], ((it + 1) / Cfg::STAGES) & 1, A.err))) break;
+        if (!(ok = at_wait_warp(&s_free, it & 1, A.err))) break;
+        tc_fence_after();
+        qk(it + 1);
+      }
       if (!(ok = at_wait_warp(&v_full[s], (it / Cfg::STAGES) & 1, A.err))) break;
-      if (!(ok = at_wait_warp(&p_full, it & 1, A.err))) break;
+      if (!(ok = at_wait_warp(&p_full[it & 1], (it >> 1) & 1, A.err))) break;
       tc_fence_after();
-      if (it + 1 < count) qk(it + 1);  // S is free once P is written
       const uint64_t vb = dv + (s * Cfg::TILE >> 4);
 #pragma unroll
       for (int k = 0; k < KEYS / 16; k++)
-        mma_ts(tmem + Cfg::COL_O, tmem + Cfg::COL_P + k * 8, vb + (k * 16 * 128 >> 4), id_o, (it | k) != 0);
-      mma_commit(&v_empty[s]);
-      mma_commit(&pv_done);
+        mma_ts(leader, tmem + Cfg::COL_O, tmem + Cfg::COL_P + (it & 1) * 32 + k * 8, vb + (k * 16 * 128 >> 4), id_o, (it | k) != 0);
+      mma_commit(leader, &v_empty[s]);
+      mma_commit(leader, &pv_done);
     }
-    if (!ok) {  // let the issued MMAs finish before TMEM is freed
-      mma_commit(&drain);
-      at_wait_warp(&drain, 0, A.err);
-    }
+    mma_commit(leader, &o_done);
+    if (!ok) at_wait_warp(&o_done, 0, A.err);  // the issued MMAs finish before TMEM is freed
   } else {
-    const int wg = warp / 4, row_of = tid % kAfRows, pair_bar = 2 + warp % 4;
-    const int c0 = wg * (KEYS / 2);  // first column of this thread
-    const uint32_t lane_base = uint32_t((warp % 4) * 32) << 16;
-    const bool idle = r0 + (warp % 4) * 32 >= rows;  // no row of this warp exists: it only keeps step
+    const uint32_t lane_base = uint32_t(warp * 32) << 16;
+    const bool idle = r0 + warp * 32 >= rows;  // no row of this warp exists: it only keeps step
     const int pos = off + qi;
     const int lim = valid ? at_limit(A, n, prefix, pos) : 0;
+    // without cap and bias the scale is applied with the exponent's FMA: x·cmul are scores in log2 units
+    const float cmul = CAP || BIAS ? 1.f : A.scale * kAtLog2e;
     AtBias bias;
     bias.mul = CAP ? 2.f * A.scale * kAtLog2e / A.cap : A.scale * kAtLog2e;
     bias.cap2 = A.cap * kAtLog2e;
@@ -227,15 +227,26 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       bias.y = cell.x * bias.slope;
       bias.x = cell.y * bias.slope;
     }
-    float m = valid ? -INFINITY : 0.f;  // the row's reference maximum, log2 units (−∞: nothing seen yet)
-    float l = 0.f;                      // this thread's part of the row's sum
+    float m = -INFINITY;  // the row's reference maximum, log2 units (−∞: nothing seen yet)
+    float l = 0.f;        // its sum
     int it = 0;
     bool ok = true;
-    for (int t = tiles.first(); t < tiles.end; t = tiles.next(t), it++) {
-      const int j0 = t * KEYS;
-      const bool by_doc = docs && at_bit(mix, t - tiles.begin);
-      const bool masked = by_doc || j0 + KEYS > lim_min;
-      const bool dirty = (n < A.Lk && j0 + KEYS > n) || (docs && at_bit(pad, t - tiles.begin));
+    struct Tile {
+      int t, j0;
+      bool by_doc, masked, dirty;
+    };
+    auto tile_at = [&](int t) {
+      Tile x{t, t * KEYS, false, t * KEYS + KEYS > lim_min, n < A.Lk && t * KEYS + KEYS > n};
+      if (docs && t < tiles.end) {
+        x.by_doc = at_bit(mix, t - tiles.begin);
+        x.masked |= x.by_doc;
+        x.dirty |= at_bit(pad, t - tiles.begin);
+      }
+      return x;
+    };
+    for (Tile cur = tile_at(tiles.first()); cur.t < tiles.end; it++) {
+      const int j0 = cur.j0;
+      const bool by_doc = cur.by_doc, masked = cur.masked, dirty = cur.dirty;
       if (by_doc || BIAS == 2) {  // per-key data of the tile, one key a thread
         if (tid < KEYS) {
           const int j = j0 + tid;
@@ -251,124 +262,109 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         }
         named_bar_sync(1, kAfSoft);
       }
-      if (!(ok = at_wait_warp(&s_full, it & 1, A.err))) break;
+      ok = at_wait(&s_full, it & 1, A.err);
       tc_fence_after();
-
-      // Scores of chunk k in log2 units plus `add`; returns their maximum.
-      auto scores = [&](int k, float add, float (&x)[32]) {
-        const int c1 = c0 + 32 * k;
-        tmem_ld32_nowait(tmem + lane_base + Cfg::COL_S + c1, x);
-        uint32_t vis = 0xffffffffu;
+      float f = 1.f, neg = 0.f;
+      float x[KEYS];
+      at_ld64(tmem + lane_base + Cfg::COL_S, x);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_free);
+      if (!idle) {
+        uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
         if (masked) {
-          vis = at_low_bits(lim - j0 - c1);
-          if (by_doc) vis &= at_doc_bits32(&col_doc[it & 1][c1], my_doc);
-        }
-        if (BIAS == 1) bias.y = float(pos - j0 - c1) * bias.slope;
-        AtLine line;
-        if (BIAS == 1) line.start(bias);
-        tmem_wait_ld();
-        if (CAP && masked) at_mask32(x, vis, 0.f);
-        const float2 add2x[2] = {make_float2(add, add), make_float2(add, add)};
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          float2 s2[2] = {make_float2(x[c], x[c + 1]), make_float2(x[c + 2], x[c + 3])}, sig[2];
-          float4 ky = {}, kx = {};
-          if (BIAS == 2) {
-            ky = *reinterpret_cast<const float4*>(&col_y[it & 1][c1 + c]);
-            kx = *reinterpret_cast<const float4*>(&col_x[it & 1][c1 + c]);
+          for (int k = 0; k < 2; k++) {
+            vis[k] = at_low_bits(lim - j0 - 32 * k);
+            if (by_doc) vis[k] &= at_doc_bits32(&col_doc[it & 1][32 * k], my_doc);
           }
-          at_scores4<CAP, BIAS>(bias, s2, add2x, line, ky, kx, sig);
-          x[c] = s2[0].x;
-          x[c + 1] = s2[0].y;
-          x[c + 2] = s2[1].x;
-          x[c + 3] = s2[1].y;
         }
-        if (masked) at_mask32(x, vis, -INFINITY);
-        float top = fmaxf(x[0], x[1]), top1 = fmaxf(x[2], x[3]);
+        AtLine line;
+        if (BIAS == 1) {
+          bias.y = float(pos - j0) * bias.slope;
+          line.start(bias);
+        }
+        if (CAP && masked) {
+          at_mask32(x, vis[0], 0.f);
+          at_mask32(x + 32, vis[1], 0.f);
+        }
+        if (CAP || BIAS) {
+          const float2 none[2] = {};
 #pragma unroll
-        for (int c = 4; c < 32; c += 4) {
-          top = fmaxf(fmaxf(top, x[c]), x[c + 1]);
-          top1 = fmaxf(fmaxf(top1, x[c + 2]), x[c + 3]);
+          for (int c = 0; c < KEYS; c += 4) {
+            float2 s2[2] = {make_float2(x[c], x[c + 1]), make_float2(x[c + 2], x[c + 3])}, sig[2];
+            float4 ky = {}, kx = {};
+            if (BIAS == 2) {
+              ky = *reinterpret_cast<const float4*>(&col_y[it & 1][c]);
+              kx = *reinterpret_cast<const float4*>(&col_x[it & 1][c]);
+            }
+            at_scores4<CAP, BIAS>(bias, s2, none, line, ky, kx, sig);
+            x[c] = s2[0].x;
+            x[c + 1] = s2[0].y;
+            x[c + 2] = s2[1].x;
+            x[c + 3] = s2[1].y;
+          }
         }
-        return fmaxf(top, top1);
-      };
-      // Raises the reference m of rows whose scores' maximum `over` (of this thread's columns, relative to `base`) calls
-      // for it; returns the factor by which what was summed against the old one has to be multiplied.
-      auto raise = [&](float over, float base) {
-        pair_top[wg][row_of] = over;
-        named_bar_sync(pair_bar, 64);
-        over = fmaxf(over, pair_top[wg ^ 1][row_of]);
-        if (m == -INFINITY ? !(over > -INFINITY) : !(over > kAfGrow)) return 1.f;
-        const float old = m;
-        m = base + over;
-        const float f = old == -INFINITY ? 0.f : at_ex2(old - m);
-        l *= f;
-        return f;
-      };
-      auto rescale = [&](float f) {
+        if (masked) {
+          at_mask32(x, vis[0], -INFINITY);
+          at_mask32(x + 32, vis[1], -INFINITY);
+        }
+        float top4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int c = 4; c < KEYS; c += 8) {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (c + 4 + i < KEYS)
+              top4[i] = fmaxf(fmaxf(top4[i], x[c + i]), x[c + 4 + i]);
+            else
+              top4[i] = fmaxf(top4[i], x[c + i]);
+        }
+        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * cmul;
+        if (top > m + kAfGrow || (m == -INFINITY && top > -INFINITY)) {
+          f = m == -INFINITY ? 0.f : at_ex2(m - top);
+          m = top;
+          l *= f;
+        }
+        neg = m == -INFINITY ? 0.f : -m;
+      }
+      if (__any_sync(0xffffffffu, f != 1.f || !ok)) {  // rescale O, once the previous P·V is in it
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok && it > 0) ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err);
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll 1
-        for (int c = wg * (DP / 2); c < (wg + 1) * (DP / 2); c += 16) {
+        for (int c = 0; it > 0 && c < DP; c += 16) {
           float o[16];
-          tmem_ld16(tmem + lane_base + Cfg::COL_O + c, o);
+          at_ld16(tmem + lane_base + Cfg::COL_O + c, o);
 #pragma unroll
           for (int i = 0; i < 16; i++) o[i] = f == 0.f ? 0.f : o[i] * f;
           tmem_st16(tmem + lane_base + Cfg::COL_O + c, reinterpret_cast<const uint32_t*>(o));
         }
-      };
-
-      bool pv_waited = it == 0;  // P and O are free once the previous P·V is done
-      if (__any_sync(0xffffffffu, m == -INFINITY)) {  // the same in both warps of the rows
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int k = 0; k < Cfg::CHUNKS; k++) {
-          float x[32];
-          top = fmaxf(top, scores(k, 0.f, x));
-        }
-        // rows that have a reference already go on with it: the pass below finds out if it is too low
-        const float f = raise(m == -INFINITY ? top : -INFINITY, 0.f);
-        if (it > 0) {
-          if (!(ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err))) break;
-          tc_fence_after();
-          pv_waited = true;
-          rescale(f);
-        }
       }
-      const float l0 = l;
-      for (int pass = 0;; pass++) {
-        float over = -INFINITY;  // largest score over the reference
-        if (!idle) {
-          const float neg = m == -INFINITY ? 0.f : -m;
-          float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-          for (int k = 0; k < Cfg::CHUNKS; k++) {
-            float x[32];
-            over = fmaxf(over, scores(k, neg, x));
-            uint32_t p[16];
+      cur = tile_at(tiles.next(cur.t));  // here, where the exponentials leave issue slots
+      if (!idle) {
+        const float2 mul = make_float2(cmul, cmul), add = make_float2(neg, neg);
+        float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const float2 e = make_float2(at_ex2(x[2 * i]), at_ex2(x[2 * i + 1]));
-              sum[i & 1] = add2(sum[i & 1], e);
-              p[i] = Half16<T>::pack(e.x, e.y);
-            }
-            if (!pv_waited) {
-              if (!(ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err))) break;
-              tc_fence_after();
-              pv_waited = true;
-            }
-            tmem_st16(tmem + lane_base + Cfg::COL_P + (c0 + 32 * k) / 2, p);
+        for (int c = 0; c < KEYS; c += 32) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            float2 e = make_float2(x[c + 2 * i], x[c + 2 * i + 1]);
+            e = CAP || BIAS ? add2(e, add) : fma2(e, mul, add);
+            e.x = at_ex2(e.x);
+            e.y = at_ex2(e.y);
+            sum[i & 1] = add2(sum[i & 1], e);
+            p[i] = Half16<T>::pack(e.x, e.y);
           }
-          const float2 s = add2(sum[0], sum[1]);
-          l = s.x + s.y;
+          tmem_st16(tmem + lane_base + Cfg::COL_P + (it & 1) * 32 + c / 2, p);  // free: S tells that the P·V before last is done
         }
-        if (!at_pair_any(pair_bar, over > kAfGrow && pass == 0) || !ok) break;
-        l = l0;  // rare: take the tile once more against the raised reference
-        const float f = raise(over, m);
-        if (it > 0) rescale(f);
+        const float2 s = add2(sum[0], sum[1]);
+        l = s.x + s.y;
       }
-      if (!ok) break;
       if (dirty) {  // V rows of keys that no query sees hold anything, NaN included: 0·NaN must not enter O
         if (!(ok = at_wait_warp(&v_full[it % Cfg::STAGES], (it / Cfg::STAGES) & 1, A.err))) break;
-        const int key = tid % KEYS, j = j0 + key, panel = tid / KEYS;
+        const int key = tid % KEYS, j = j0 + key, panel = tid / KEYS;  // a thread per row and panel
         if (panel < Cfg::PANELS && (j >= n || (docs && A.doc_k[(long long)b * A.Lk + j] < 0))) {
           uint8_t* v = smem + Cfg::QTILE + (Cfg::STAGES + it % Cfg::STAGES) * Cfg::TILE + panel * Cfg::KPANEL + key * 128;
 #pragma unroll
@@ -379,23 +375,20 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full);
+      if (lane == 0) mbar_arrive(&p_full[it & 1]);
     }
-    if (ok && it > 0) ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err);
+    ok = ok && at_wait_warp(&o_done, 0, A.err);
     if (ok) {
       tc_fence_after();
-      pair_sum[wg][row_of] = l;
-      named_bar_sync(pair_bar, 64);
-      l += pair_sum[wg ^ 1][row_of];
       const long long row = ((long long)b * A.Hq + head) * A.Lq + qi;
       const long long part_row = (long long)split * A.B * A.Hq * A.Lq + row;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays one
       T* o_ptr = static_cast<T*>(P.o.p) + b * P.o.sb + qi * P.o.st + head * P.o.sh;
 #pragma unroll
-      for (int c = wg * (DP / 2); c < (wg + 1) * (DP / 2); c += 16) {
+      for (int c = 0; c < DP; c += 16) {
         if (c >= A.D) break;
         float o[16];
-        if (it > 0) tmem_ld16(tmem + lane_base + Cfg::COL_O + c, o);
+        if (it > 0) at_ld16(tmem + lane_base + Cfg::COL_O + c, o);
 #pragma unroll
         for (int i = 0; i < 16; i++) o[i] = it > 0 && l != 0.f ? o[i] : 0.f;
         if (!valid) continue;
@@ -416,7 +409,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
           }
         }
       }
-      if (valid && wg == 0) {
+      if (valid) {
         if (P.splits > 1)
           P.stats[part_row] = make_float2(m, l);
         else if (P.lse)
@@ -426,7 +419,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(tmem, 256);
   }
