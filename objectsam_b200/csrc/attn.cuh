@@ -199,6 +199,17 @@ __device__ __forceinline__ void at_scores4(const AtBias& P, float2 (&s)[2], cons
   }
 }
 
+// Barrier of the two warps that share rows, with the OR of a flag.
+__device__ __forceinline__ bool at_pair_any(int id, bool flag) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(r)
+      : "r"(uint32_t(flag)), "r"(id)
+      : "memory");
+  return r != 0;
+}
+
 // The MMA warp runs its loop with all lanes and issues from one, `leader`, by predicate: with warp-uniform control flow
 // the descriptors stay in uniform registers, where the instruction reads them (issued from inside a one-lane branch,
 // every MMA first moved its operands over, about 100 cycles each: more than these small MMAs take).
@@ -263,21 +274,15 @@ __device__ __forceinline__ void at_ld16(uint32_t taddr, float (&v)[16]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void at_ld64(uint32_t taddr, float (&v)[64]) {
+__device__ __forceinline__ void at_ld32(uint32_t taddr, float (&v)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
-      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, "
-      "%42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, "
-      "%62, %63}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), 
         "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), 
         "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), 
-        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]), 
-        "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]), 
-        "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]), 
-        "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]), 
-        "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
       : "r"(taddr)
       : "memory");
 }
@@ -309,14 +314,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Bounded wait (as mbar_wait) without the suspend-time hint: with it the test sleeps in steps of a microsecond and
-// more, too coarse for tiles that take about one (a producer that overslept kept the tensor cores waiting for most
-// of a tile's time).
+// Bounded wait (as mbar_wait) without the suspend-time hint, with which the test sleeps in steps of a microsecond and
+// more: about a tile's time.
 __device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, int* err) {
   if (mbar_try_wait(bar, parity)) return true;
   const unsigned long long t0 = globaltimer();
   while (true) {
-    for (int i = 0; i < 256; i++)
+    for (int i = 0; i < 64; i++)
       if (mbar_try_wait(bar, parity)) return true;
     if (globaltimer() - t0 > kWaitBudgetNs) {
       record_error(err, kDevErrTimeout);

@@ -3,21 +3,24 @@
 // single token of many heads still fills rows.  Long caches with few rows are split over the keys: each split
 // writes its unnormalised output with its maximum and sum, and k_attn_join (attn.cu) adds them.
 //
-// Per 64-key tile:  S = Q·Kᵀ (tcgen05, fp32 in TMEM) → one thread per row reads its 64 scores into registers, applies cap,
-// bias and masks, takes p = 2^(x − m) against the row's reference maximum m and writes P in 16 bits back to TMEM → O +=
-// P·V with P as the TMEM operand.  A row is a TMEM lane: its maximum and sum need no shuffles.  m follows the
-// maximum only when a tile exceeds it by more than 2^8 (P ≤ 2^8 keeps its relative precision in 16 bits, the sum is
-// fp32): then O, which stays in TMEM, is rescaled.  Tiles are visited from the CTA's own positions outwards, so that
-// with a distance bias the largest scores come first and this stays rare.
-// Warps 0–3: softmax, warp 4: TMA producer, warp 5: TMEM owner and MMA issuer.  TMEM, 256 columns a CTA (two CTAs per
-// SM): S, which the next tile's Q·Kᵀ overwrites as soon as it is in registers, two buffers of P, and O.
+// Per 64-key tile:  S = Q·Kᵀ (tcgen05, fp32 in TMEM) → two threads per row read 32 scores each into registers, apply cap,
+// bias and masks, take p = 2^(x − m) against the row's reference maximum m and write P in 16 bits back to TMEM → O +=
+// P·V with P as the TMEM operand.  A row is a TMEM lane: its maximum and sum need no shuffles.  m follows the maximum
+// only when a tile exceeds it by more than 2^8 (P ≤ 2^8 keeps its relative precision in 16 bits, the sum is fp32):
+// then the row's two threads agree on it and O, which stays in TMEM, is rescaled; otherwise one flag barrier of the
+// two warps tells that nothing is to do.  Tiles are visited from the CTA's own positions outwards, so that with a
+// distance bias the largest scores come first and this stays rare.
+// Warps 0–7: softmax (warps w and w + 4 share rows), warp 8: TMA producer, warp 9: TMEM owner and MMA issuer.  The
+// softmax is a chain of latencies (barriers, TMEM loads, the exponentials' unit) that four warps a scheduler hide:
+// two CTAs per SM, 256 TMEM columns each: S, which the next tile's Q·Kᵀ overwrites as soon as it is in registers,
+// two buffers of P, and O.
 #pragma once
 #include "attn.cuh"
 
 namespace osam {
 
 constexpr int kAfRows = 128, kAfKeys = 64;
-constexpr int kAfSoft = 128;    // softmax threads
+constexpr int kAfSoft = 256;    // softmax threads
 constexpr int kAfThreads = kAfSoft + 64;
 constexpr float kAfGrow = 8.f;  // log2 growth over a row's reference maximum that forces a rescale
 
@@ -40,6 +43,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   __shared__ __align__(8) uint64_t k_full[Cfg::STAGES], k_empty[Cfg::STAGES], v_full[Cfg::STAGES], v_empty[Cfg::STAGES];
   __shared__ __align__(8) uint64_t s_full, s_free, p_full[2], pv_done, o_done;
   __shared__ uint32_t tmem_slot;
+  __shared__ float pair_top[2][kAfRows], pair_sum[2][kAfRows];  // what the two threads of a row tell each other
   __shared__ uint32_t live[kAtDocWords], mix[kAtDocWords], pad[kAtDocWords];
   __shared__ AtDocs own_docs[4];
   __shared__ __align__(16) int col_doc[2][KEYS];
@@ -70,8 +74,8 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   tiles.live = docs ? live : nullptr;
 
   // ---- this thread's row
-  const int r = r0 + tid;
-  const bool valid = warp < 4 && r < rows;
+  const int r = r0 + tid % kAfRows;
+  const bool valid = warp < 8 && r < rows;
   const int qi = valid ? r / A.G : 0, head = hk * A.G + (valid ? r - qi * A.G : 0);
   int my_doc = -2;
   if (valid && docs) {
@@ -87,20 +91,20 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       mbar_init(&v_empty[i], 1);
     }
     mbar_init(&s_full, 1);
-    mbar_init(&s_free, 4);
-    mbar_init(&p_full[0], 4);  // two: a warp may be a tile ahead of another
-    mbar_init(&p_full[1], 4);
+    mbar_init(&s_free, 8);
+    mbar_init(&p_full[0], 8);  // two: a warp may be a tile ahead of another
+    mbar_init(&p_full[1], 8);
     mbar_init(&pv_done, 1);
     mbar_init(&o_done, 1);
     fence_barrier_init();
     tma_prefetch_desc(&P.tk);
     tma_prefetch_desc(&P.tv);
   }
-  if (warp == 5) {
+  if (warp == 9) {
     tmem_alloc(&tmem_slot, 256);
     tmem_relinquish();
   }
-  if (warp < 4) {
+  if (warp < 8) {
     // Q rows into the K-major swizzled panels; rows past the end and dims past D are zero
     constexpr int CH = DP / 8;
     const T* q = static_cast<const T*>(P.q.p) + b * P.q.sb;
@@ -115,7 +119,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       *reinterpret_cast<uint4*>(smem + (ch / 8) * Cfg::QPANEL + at_sw128(row, ch % 8)) = u;
     }
     fence_proxy_async_smem();
-    if (docs) {
+    if (docs && warp < 4) {
       AtDocs d{my_doc >= 0 ? my_doc : INT_MAX, my_doc, valid && my_doc < 0, 0};
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -142,7 +146,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp == 4) {
+  if (warp == 8) {
     if (lane == 0) {
       int it = 0;
       bool ok = true;
@@ -169,7 +173,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       }
     }
     __syncwarp();
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     const uint32_t leader = elect_leader();
     const int ks = (A.D + 15) / 16;  // K steps of Q·Kᵀ; N of P·V is 16·ks
     const uint32_t id_s = at_idesc(BF16, 128, KEYS, false), id_o = at_idesc(BF16, 128, 16 * ks, true);
@@ -204,15 +208,17 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       const uint64_t vb = dv + (s * Cfg::TILE >> 4);
 #pragma unroll
       for (int k = 0; k < KEYS / 16; k++)
-        mma_ts(leader, tmem + Cfg::COL_O, tmem + Cfg::COL_P + (it & 1) * 32 + k * 8, vb + (k * 16 * 128 >> 4), id_o, (it | k) != 0);
+        mma_ts(leader, tmem + Cfg::COL_O, tmem + Cfg::COL_P + (it & 1) * 32 + k * 8,
+               vb + (k * 16 * 128 >> 4), id_o, (it | k) != 0);
       mma_commit(leader, &v_empty[s]);
       mma_commit(leader, &pv_done);
     }
     mma_commit(leader, &o_done);
     if (!ok) at_wait_warp(&o_done, 0, A.err);  // the issued MMAs finish before TMEM is freed
   } else {
-    const uint32_t lane_base = uint32_t(warp * 32) << 16;
-    const bool idle = r0 + warp * 32 >= rows;  // no row of this warp exists: it only keeps step
+    const int half = warp / 4, row_of = tid % kAfRows, h0 = half * 32, pair_bar = 2 + warp % 4;
+    const uint32_t lane_base = uint32_t((warp % 4) * 32) << 16;
+    const bool idle = r0 + (warp % 4) * 32 >= rows;  // no row of this warp exists: it only keeps step
     const int pos = off + qi;
     const int lim = valid ? at_limit(A, n, prefix, pos) : 0;
     // without cap and bias the scale is applied with the exponent's FMA: x·cmul are scores in log2 units
@@ -228,7 +234,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       bias.x = cell.y * bias.slope;
     }
     float m = -INFINITY;  // the row's reference maximum, log2 units (−∞: nothing seen yet)
-    float l = 0.f;        // its sum
+    float l = 0.f;        // this thread's part of its sum
     int it = 0;
     bool ok = true;
     struct Tile {
@@ -264,39 +270,33 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       }
       ok = at_wait(&s_full, it & 1, A.err);
       tc_fence_after();
-      float f = 1.f, neg = 0.f;
-      float x[KEYS];
-      at_ld64(tmem + lane_base + Cfg::COL_S, x);
+      float top = -INFINITY;
+      float x[32];
+      at_ld32(tmem + lane_base + Cfg::COL_S + h0, x);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_free);
       if (!idle) {
-        uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
+        uint32_t vis = 0xffffffffu;
         if (masked) {
-#pragma unroll
-          for (int k = 0; k < 2; k++) {
-            vis[k] = at_low_bits(lim - j0 - 32 * k);
-            if (by_doc) vis[k] &= at_doc_bits32(&col_doc[it & 1][32 * k], my_doc);
-          }
-        }
-        AtLine line;
-        if (BIAS == 1) {
-          bias.y = float(pos - j0) * bias.slope;
-          line.start(bias);
-        }
-        if (CAP && masked) {
-          at_mask32(x, vis[0], 0.f);
-          at_mask32(x + 32, vis[1], 0.f);
+          vis = at_low_bits(lim - j0 - h0);
+          if (by_doc) vis &= at_doc_bits32(&col_doc[it & 1][h0], my_doc);
+          if (CAP) at_mask32(x, vis, 0.f);
         }
         if (CAP || BIAS) {
+          AtLine line;
+          if (BIAS == 1) {
+            bias.y = float(pos - j0 - h0) * bias.slope;
+            line.start(bias);
+          }
           const float2 none[2] = {};
 #pragma unroll
-          for (int c = 0; c < KEYS; c += 4) {
+          for (int c = 0; c < 32; c += 4) {
             float2 s2[2] = {make_float2(x[c], x[c + 1]), make_float2(x[c + 2], x[c + 3])}, sig[2];
             float4 ky = {}, kx = {};
             if (BIAS == 2) {
-              ky = *reinterpret_cast<const float4*>(&col_y[it & 1][c]);
-              kx = *reinterpret_cast<const float4*>(&col_x[it & 1][c]);
+              ky = *reinterpret_cast<const float4*>(&col_y[it & 1][h0 + c]);
+              kx = *reinterpret_cast<const float4*>(&col_x[it & 1][h0 + c]);
             }
             at_scores4<CAP, BIAS>(bias, s2, none, line, ky, kx, sig);
             x[c] = s2[0].x;
@@ -305,35 +305,32 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
             x[c + 3] = s2[1].y;
           }
         }
-        if (masked) {
-          at_mask32(x, vis[0], -INFINITY);
-          at_mask32(x + 32, vis[1], -INFINITY);
-        }
-        float top4[4] = {x[0], x[1], x[2], x[3]};
+        if (masked) at_mask32(x, vis, -INFINITY);
+        float top1 = x[1];
+        top = x[0];
 #pragma unroll
-        for (int c = 4; c < KEYS; c += 8) {
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (c + 4 + i < KEYS)
-              top4[i] = fmaxf(fmaxf(top4[i], x[c + i]), x[c + 4 + i]);
-            else
-              top4[i] = fmaxf(top4[i], x[c + i]);
+        for (int c = 2; c + 3 < 32; c += 4) {
+          top = fmaxf(fmaxf(top, x[c]), x[c + 1]);
+          top1 = fmaxf(fmaxf(top1, x[c + 2]), x[c + 3]);
         }
-        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * cmul;
+        top = fmaxf(fmaxf(top, top1), fmaxf(x[30], x[31])) * cmul;
+      }
+      if (at_pair_any(pair_bar, top > m + kAfGrow || (m == -INFINITY && top > -INFINITY) || !ok)) {
+        ok = !at_pair_any(pair_bar, !ok);
+        pair_top[half][row_of] = top;
+        named_bar_sync(pair_bar, 64);
+        top = fmaxf(top, pair_top[half ^ 1][row_of]);
+        float f = 1.f;
         if (top > m + kAfGrow || (m == -INFINITY && top > -INFINITY)) {
           f = m == -INFINITY ? 0.f : at_ex2(m - top);
           m = top;
           l *= f;
         }
-        neg = m == -INFINITY ? 0.f : -m;
-      }
-      if (__any_sync(0xffffffffu, f != 1.f || !ok)) {  // rescale O, once the previous P·V is in it
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok && it > 0) ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err);
+        if (ok && it > 0) ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err);  // the previous P·V is in O
         if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
-        for (int c = 0; it > 0 && c < DP; c += 16) {
+        for (int c = half * (DP / 2); it > 0 && c < (half + 1) * (DP / 2); c += 16) {
           float o[16];
           at_ld16(tmem + lane_base + Cfg::COL_O + c, o);
 #pragma unroll
@@ -343,22 +340,21 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       }
       cur = tile_at(tiles.next(cur.t));  // here, where the exponentials leave issue slots
       if (!idle) {
+        const float neg = m == -INFINITY ? 0.f : -m;
         const float2 mul = make_float2(cmul, cmul), add = make_float2(neg, neg);
         float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
+        uint32_t p[16];
 #pragma unroll
-        for (int c = 0; c < KEYS; c += 32) {
-          uint32_t p[16];
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            float2 e = make_float2(x[c + 2 * i], x[c + 2 * i + 1]);
-            e = CAP || BIAS ? add2(e, add) : fma2(e, mul, add);
-            e.x = at_ex2(e.x);
-            e.y = at_ex2(e.y);
-            sum[i & 1] = add2(sum[i & 1], e);
-            p[i] = Half16<T>::pack(e.x, e.y);
-          }
-          tmem_st16(tmem + lane_base + Cfg::COL_P + (it & 1) * 32 + c / 2, p);  // free: S tells that the P·V before last is done
+        for (int i = 0; i < 16; i++) {
+          float2 e = make_float2(x[2 * i], x[2 * i + 1]);
+          e = CAP || BIAS ? add2(e, add) : fma2(e, mul, add);
+          e.x = at_ex2(e.x);
+          e.y = at_ex2(e.y);
+          sum[i & 1] = add2(sum[i & 1], e);
+          p[i] = Half16<T>::pack(e.x, e.y);
         }
+        // this buffer of P is free: S tells that the P·V before last is done
+        tmem_st16(tmem + lane_base + Cfg::COL_P + (it & 1) * 32 + h0 / 2, p);
         const float2 s = add2(sum[0], sum[1]);
         l = s.x + s.y;
       }
@@ -380,12 +376,15 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     ok = ok && at_wait_warp(&o_done, 0, A.err);
     if (ok) {
       tc_fence_after();
+      pair_sum[half][row_of] = l;
+      named_bar_sync(pair_bar, 64);
+      l += pair_sum[half ^ 1][row_of];
       const long long row = ((long long)b * A.Hq + head) * A.Lq + qi;
       const long long part_row = (long long)split * A.B * A.Hq * A.Lq + row;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays one
       T* o_ptr = static_cast<T*>(P.o.p) + b * P.o.sb + qi * P.o.st + head * P.o.sh;
 #pragma unroll
-      for (int c = 0; c < DP; c += 16) {
+      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 16) {
         if (c >= A.D) break;
         float o[16];
         if (it > 0) at_ld16(tmem + lane_base + Cfg::COL_O + c, o);
@@ -409,7 +408,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
           }
         }
       }
-      if (valid) {
+      if (valid && half == 0) {
         if (P.splits > 1)
           P.stats[part_row] = make_float2(m, l);
         else if (P.lse)
@@ -419,7 +418,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem, 256);
   }
