@@ -315,22 +315,34 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Bounded wait (as mbar_wait) without the suspend-time hint, with which the test sleeps in steps of a microsecond and
-// more: about a tile's time.
-__device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, int* err) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = globaltimer();
-  while (true) {
-    for (int i = 0; i < 64; i++)
-      if (mbar_try_wait(bar, parity)) return true;
-    if (globaltimer() - t0 > kWaitBudgetNs) {
-      record_error(err, kDevErrTimeout);
-      return false;
-    }
+// more (about a tile's time), and bounded by a count, which costs the waiting loop nothing: one test takes tens of
+// cycles at least, so 2^25 take from about half a second to a few.
+constexpr uint32_t kAtWaitTests = 1u << 25;
+__device__ __forceinline__ bool at_wait(uint32_t bar, uint32_t parity, int* err) {
+  for (uint32_t n = 0;; n++) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (n == kAtWaitTests) break;
   }
+  record_error(err, kDevErrTimeout);
+  return false;
+}
+__device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, int* err) {
+  return at_wait(smem_u32(bar), parity, err);
 }
 // A wait that a whole warp takes together: every lane learns whether any lane's budget ran out.
 __device__ __forceinline__ bool at_wait_warp(uint64_t* bar, uint32_t parity, int* err) {
   return __all_sync(0xffffffffu, at_wait(bar, parity, err));
+}
+__device__ __forceinline__ void at_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // Which tiles of the streamed side a CTA visits: of [begin, end) all, or with documents those whose bit is set (built
@@ -371,6 +383,7 @@ struct AtTiles {
     return t >= begin ? t : up(from + 1);
   }
   __device__ __forceinline__ int next(int t) const {
+    if (!live) return t > from ? t + 1 : t == begin ? from + 1 : t - 1;
     if (t > from) return up(t + 1);
     t = down(t - 1);
     return t >= begin ? t : up(from + 1);

@@ -234,25 +234,21 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       bias.x = cell.y * bias.slope;
     }
     float m = -INFINITY;  // the row's reference maximum, log2 units (−∞: nothing seen yet)
+    float neg = 0.f;      // −m, or 0 while there is none
     float l = 0.f;        // this thread's part of its sum
-    int it = 0;
+    const uint32_t bar_s = smem_u32(&s_full), bar_free = smem_u32(&s_free), bar_p = smem_u32(&p_full[0]);
+    const uint32_t s_addr = tmem + lane_base + Cfg::COL_S + h0, p_addr = tmem + lane_base + Cfg::COL_P + h0 / 2;
+    const int tail = n < A.Lk ? n : INT_MAX;  // keys from here on hold anything
     bool ok = true;
-    struct Tile {
-      int t, j0;
-      bool by_doc, masked, dirty;
-    };
-    auto tile_at = [&](int t) {
-      Tile x{t, t * KEYS, false, t * KEYS + KEYS > lim_min, n < A.Lk && t * KEYS + KEYS > n};
-      if (docs && t < tiles.end) {
-        x.by_doc = at_bit(mix, t - tiles.begin);
-        x.masked |= x.by_doc;
-        x.dirty |= at_bit(pad, t - tiles.begin);
+    int it = 0;
+    for (int t = tiles.first(); t < tiles.end; it++) {
+      const int j0 = t * KEYS;
+      bool by_doc = false, dirty = j0 + KEYS > tail;
+      if (docs) {
+        by_doc = at_bit(mix, t - tiles.begin);
+        dirty |= at_bit(pad, t - tiles.begin);
       }
-      return x;
-    };
-    for (Tile cur = tile_at(tiles.first()); cur.t < tiles.end; it++) {
-      const int j0 = cur.j0;
-      const bool by_doc = cur.by_doc, masked = cur.masked, dirty = cur.dirty;
+      const bool masked = by_doc || j0 + KEYS > lim_min;
       if (by_doc || BIAS == 2) {  // per-key data of the tile, one key a thread
         if (tid < KEYS) {
           const int j = j0 + tid;
@@ -268,14 +264,15 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         }
         named_bar_sync(1, kAfSoft);
       }
-      ok = at_wait(&s_full, it & 1, A.err);
+      ok = at_wait(bar_s, it & 1, A.err);
       tc_fence_after();
       float top = -INFINITY;
       float x[32];
-      at_ld32(tmem + lane_base + Cfg::COL_S + h0, x);
+      at_ld32(s_addr, x);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s_free);
+      if (lane == 0) at_arrive(bar_free);
+      t = tiles.next(t);
       if (!idle) {
         uint32_t vis = 0xffffffffu;
         if (masked) {
@@ -315,15 +312,16 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         }
         top = fmaxf(fmaxf(top, top1), fmaxf(x[30], x[31])) * cmul;
       }
-      if (at_pair_any(pair_bar, top > m + kAfGrow || (m == -INFINITY && top > -INFINITY) || !ok)) {
+      if (at_pair_any(pair_bar, top > m + kAfGrow || !ok)) {  // also the first score that a row sees: −∞ + 8 = −∞
         ok = !at_pair_any(pair_bar, !ok);
         pair_top[half][row_of] = top;
         named_bar_sync(pair_bar, 64);
         top = fmaxf(top, pair_top[half ^ 1][row_of]);
         float f = 1.f;
-        if (top > m + kAfGrow || (m == -INFINITY && top > -INFINITY)) {
+        if (top > m + kAfGrow) {
           f = m == -INFINITY ? 0.f : at_ex2(m - top);
           m = top;
+          neg = -m;
           l *= f;
         }
         if (ok && it > 0) ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err);  // the previous P·V is in O
@@ -338,9 +336,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
           tmem_st16(tmem + lane_base + Cfg::COL_O + c, reinterpret_cast<const uint32_t*>(o));
         }
       }
-      cur = tile_at(tiles.next(cur.t));  // here, where the exponentials leave issue slots
       if (!idle) {
-        const float neg = m == -INFINITY ? 0.f : -m;
         const float2 mul = make_float2(cmul, cmul), add = make_float2(neg, neg);
         float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
         uint32_t p[16];
@@ -354,7 +350,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
           p[i] = Half16<T>::pack(e.x, e.y);
         }
         // this buffer of P is free: S tells that the P·V before last is done
-        tmem_st16(tmem + lane_base + Cfg::COL_P + (it & 1) * 32 + h0 / 2, p);
+        tmem_st16(p_addr + (it & 1) * 32, p);
         const float2 s = add2(sum[0], sum[1]);
         l = s.x + s.y;
       }
@@ -371,7 +367,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[it & 1]);
+      if (lane == 0) at_arrive(bar_p + (it & 1) * 8);
     }
     ok = ok && at_wait_warp(&o_done, 0, A.err);
     if (ok) {
