@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const float* part, const floa
 // block, 16 lanes per row (a 16-byte vector each).
 template <typename T>
 __global__ void __launch_bounds__(256) k_attn_rows(const AtView o, const AtView dout, const float* lse, int Hq, int Lq,
-                                                   int D, float2* rows, float* peak) {
+                                                   int D, float* rows, float* peak) {
   __shared__ float top[8];
   constexpr float up = Half16<T>::kBf16 ? 0.f : kAbUp;
   const int nb = (Lq + kAbCols - 1) / kAbCols;
@@ -114,7 +114,11 @@ __global__ void __launch_bounds__(256) k_attn_rows(const AtView o, const AtView 
     }
 #pragma unroll
     for (int s = 8; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
-    if (c == 0) rows[(bh * nb + blk) * kAbCols + r] = make_float2(live ? up - L * kAtLog2e : -INFINITY, live ? -d : 0.f);
+    if (c == 0) {
+      float* out = rows + (bh * nb + blk) * 2 * kAbCols + r;
+      out[0] = live ? up - L * kAtLog2e : -INFINITY;
+      out[kAbCols] = live ? -d : 0.f;
+    }
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
@@ -225,7 +229,7 @@ AtLayout at_layout(const osam_attn_desc& a) {
     fwd += up256(rows * s.splits * sizeof(float2));
   }
   const size_t blocks = (size_t)a.batch * a.heads_q * ((a.len_q + kAbCols - 1) / kAbCols);
-  L.peak = at + up256(blocks * kAbCols * sizeof(float2));
+  L.peak = at + up256(blocks * 2 * kAbCols * sizeof(float));
   L.bytes = std::max(fwd, L.peak + up256(blocks * sizeof(float)));
   return L;
 }
@@ -235,6 +239,7 @@ int at_dev(const osam_attn_desc& a, const AtLayout& W, char* ws, AttnDev* A, cud
   A->G = a.heads_q / a.heads_k; A->D = a.dim;
   A->mask = a.mask; A->scale = a.scale; A->cap = a.cap;
   A->grid_w = a.grid_w;
+  A->f_g.set(A->G);
   A->f_w.set(a.grid_w);
   A->lens = a.lens; A->prefix = a.prefix; A->doc_q = a.doc_q; A->doc_k = a.doc_k; A->slopes = a.slopes;
   A->err = device_error_word();
@@ -345,7 +350,7 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   const bool bf16 = a->dtype == OSAM_BF16;
   AttnBwdLaunch L{};
   if ((rc = at_dev(*a, W, w, &L.d, st)) != OSAM_OK) return rc;
-  float2* rows = reinterpret_cast<float2*>(w + W.rows);
+  float* rows = reinterpret_cast<float*>(w + W.rows);
   float* peak = reinterpret_cast<float*>(w + W.peak);
   const int blocks = a->batch * a->heads_q * ((a->len_q + kAbCols - 1) / kAbCols);
   if (blocks > 0) {

@@ -38,6 +38,7 @@ struct AttnDev {
   int mask;  // OSAM_ATTN_*
   float scale, cap;
   int grid_w;
+  FastDiv f_g;  // ÷ G
   FastDiv f_w;  // ÷ grid_w (positions are not negative there or clamped, see at_cell)
   const int* lens;
   const int* prefix;
@@ -168,34 +169,41 @@ struct AtLine {
   }
 };
 // Four consecutive columns; `line` holds their distances (line), ky / kx their cells (grid).  out: the scores plus
-// `add`; with CAP, sig = 1/(1 + 2^u), from which 1 − tanh² = 4·sig·(1 − sig).
-template <bool CAP, int BIAS>
+// `add` (ADD); with CAP, sig = 1/(1 + 2^u), from which 1 − tanh² = 4·sig·(1 − sig).
+template <bool CAP, int BIAS, bool ADD>
 __device__ __forceinline__ void at_scores4(const AtBias& P, float2 (&s)[2], const float2 (&add)[2], AtLine& line,
                                            const float4& ky, const float4& kx, float2 (&sig)[2]) {
   const float2 mul = make_float2(P.mul, P.mul);
   float2 b[2] = {add[0], add[1]};
   if (BIAS == 1) {
-    b[0] = make_float2(b[0].x - fabsf(line.d[0].x), b[0].y - fabsf(line.d[0].y));
-    b[1] = make_float2(b[1].x - fabsf(line.d[1].x), b[1].y - fabsf(line.d[1].y));
+    const float2 t0 = make_float2(-fabsf(line.d[0].x), -fabsf(line.d[0].y)),
+                 t1 = make_float2(-fabsf(line.d[1].x), -fabsf(line.d[1].y));
+    b[0] = ADD ? make_float2(b[0].x + t0.x, b[0].y + t0.y) : t0;
+    b[1] = ADD ? make_float2(b[1].x + t1.x, b[1].y + t1.y) : t1;
     line.next();
   }
   if (BIAS == 2) {
     const float2 ns = make_float2(-P.slope, -P.slope), y = make_float2(P.y, P.y), x = make_float2(P.x, P.x);
     const float2 y0 = fma2(ns, make_float2(ky.x, ky.y), y), y1 = fma2(ns, make_float2(ky.z, ky.w), y);
     const float2 x0 = fma2(ns, make_float2(kx.x, kx.y), x), x1 = fma2(ns, make_float2(kx.z, kx.w), x);
-    b[0] = add2(b[0], make_float2(-fabsf(y0.x) - fabsf(x0.x), -fabsf(y0.y) - fabsf(x0.y)));
-    b[1] = add2(b[1], make_float2(-fabsf(y1.x) - fabsf(x1.x), -fabsf(y1.y) - fabsf(x1.y)));
+    const float2 t0 = make_float2(-fabsf(y0.x) - fabsf(x0.x), -fabsf(y0.y) - fabsf(x0.y)),
+                 t1 = make_float2(-fabsf(y1.x) - fabsf(x1.x), -fabsf(y1.y) - fabsf(x1.y));
+    b[0] = ADD ? add2(b[0], t0) : t0;
+    b[1] = ADD ? add2(b[1], t1) : t1;
   }
   if (CAP) {
     sig[0] = mul2(s[0], mul);
     sig[1] = mul2(s[1], mul);
     at_sigmoid4(sig);
     const float2 m2 = make_float2(-2.f * P.cap2, -2.f * P.cap2), c2 = make_float2(P.cap2, P.cap2);
-    s[0] = fma2(m2, sig[0], add2(c2, b[0]));
-    s[1] = fma2(m2, sig[1], add2(c2, b[1]));
-  } else {
+    s[0] = fma2(m2, sig[0], ADD || BIAS ? add2(c2, b[0]) : c2);
+    s[1] = fma2(m2, sig[1], ADD || BIAS ? add2(c2, b[1]) : c2);
+  } else if (ADD || BIAS) {
     s[0] = fma2(s[0], mul, b[0]);
     s[1] = fma2(s[1], mul, b[1]);
+  } else {
+    s[0] = mul2(s[0], mul);
+    s[1] = mul2(s[1], mul);
   }
 }
 
@@ -444,7 +452,7 @@ struct AttnBwdLaunch {
   AttnDev d;
   CUtensorMap stat1, stat2, strm1, strm2;
   AtView out1, out2;      // dK, dV (DKV); dQ (DQ)
-  const float2* rows;     // [B][Hq][⌈Lq/64⌉·64] (log2 of P's factor − lse·log2 e, −∞ where the query is empty; −δ)
+  const float* rows;      // [B][Hq][⌈Lq/64⌉][2][64]: log2 of P's factor − lse·log2 e (−∞ where the query is empty), −δ
   const float* peak;      // [B][Hq][⌈Lq/64⌉] max |dO| of the block
 };
 template <typename T, bool DKV>

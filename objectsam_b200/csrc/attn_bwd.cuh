@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
           tma_load_4d(d + Cfg::STRM + p * kAbCols * 128, &P.strm2, &full[s], p * 64, x.t * kAbCols, h, b);
         }
         if (DKV)
-          bulk_load(srows + s * Cfg::ROWS, P.rows + (((long long)b * A.Hq + h) * nq64 + x.t) * kAbCols, Cfg::ROWS,
+          bulk_load(srows + s * Cfg::ROWS, P.rows + (((long long)b * A.Hq + h) * nq64 + x.t) * 2 * kAbCols, Cfg::ROWS,
                     &full[s]);
       }
       // no copy of this CTA may be in flight when it ends
@@ -263,9 +263,9 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     }
     float row_lse = 0.f, row_delta = 0.f;
     if (!DKV) {
-      const float2 v = valid ? P.rows[((long long)b * A.Hq + hd) * nq64 * kAbCols + row] : make_float2(-INFINITY, 0.f);
-      row_lse = v.x;
-      row_delta = v.y;
+      const float* v = P.rows + (((long long)b * A.Hq + hd) * nq64 + row / kAbCols) * 2 * kAbCols + row % kAbCols;
+      row_lse = valid ? v[0] : -INFINITY;
+      row_delta = valid ? v[kAbCols] * F : 0.f;
     }
     AtBias bias;
     bias.mul = CAP ? 2.f * A.scale * kAtLog2e / A.cap : A.scale * kAtLog2e;
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
       if (!(ok = at_wait_warp(&xy_full[buf], (it / NB) & 1, A.err))) break;
       tc_fence_after();
       const int s = it % Cfg::STAGES;
-      const float4* rows2 = reinterpret_cast<const float4*>(srows + s * Cfg::ROWS + h0 * 8);
+      const float* rows = reinterpret_cast<const float*>(srows + s * Cfg::ROWS) + h0;
       if (DKV) {  // written by the bulk copy that this barrier counts
         if (!(ok = at_wait_warp(&full[s], (it / Cfg::STAGES) & 1, A.err))) break;
       }
@@ -335,11 +335,11 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
         float2 v[2] = {make_float2(sv[c], sv[c + 1]), make_float2(sv[c + 2], sv[c + 3])}, sig[2];
         float2 add[2], del[2];  // −lse (with P's factor) and −δ
         if (DKV) {
-          const float4 q0 = rows2[c / 2], q1 = rows2[c / 2 + 1];
-          add[0] = make_float2(q0.x, q0.z);
-          add[1] = make_float2(q1.x, q1.z);
-          del[0] = make_float2(q0.y, q0.w);
-          del[1] = make_float2(q1.y, q1.w);
+          const float4 ql = *reinterpret_cast<const float4*>(rows + c), qd = *reinterpret_cast<const float4*>(rows + kAbCols + c);
+          add[0] = make_float2(ql.x, ql.y);
+          add[1] = make_float2(ql.z, ql.w);
+          del[0] = make_float2(qd.x, qd.y);
+          del[1] = make_float2(qd.z, qd.w);
         } else {
           add[0] = add[1] = make_float2(row_lse, row_lse);
           del[0] = del[1] = make_float2(row_delta, row_delta);
@@ -353,22 +353,20 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
           ky = *reinterpret_cast<const float4*>(&col_y[buf][slot][h0 + c]);
           kx = *reinterpret_cast<const float4*>(&col_x[buf][slot][h0 + c]);
         }
-        at_scores4<CAP, BIAS>(bias, v, add, line, ky, kx, sig);
+        at_scores4<CAP, BIAS, true>(bias, v, add, line, ky, kx, sig);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           float2 p = make_float2(at_ex2(v[i].x), at_ex2(v[i].y));
-          float2 d = add2(make_float2(dp[c + 2 * i], dp[c + 2 * i + 1]), del[i]);
+          // (dP − δ)·F: for DQ in one step, δ being the row's; for DKV with P's factor below
+          float2 d = make_float2(dp[c + 2 * i], dp[c + 2 * i + 1]);
+          d = BF16 || DKV ? add2(d, del[i]) : fma2(d, make_float2(F, F), del[i]);
           if (CAP) {  // 1 − t² = 4·sig·(1 − sig)
             const float2 g = fma2(sig[i], make_float2(-4.f, -4.f), make_float2(4.f, 4.f));
             d = mul2(d, mul2(g, sig[i]));
           }
-          d = mul2(d, BF16 ? p : mul2(p, make_float2(F, F)));
+          d = mul2(d, BF16 || !DKV ? p : mul2(p, make_float2(F, F)));
           if (DKV) pp[c / 2 + i] = Half16<T>::pack(p.x, p.y);
-          if (!BF16) {
-            d.x = fminf(fmaxf(d.x, -65504.f), 65504.f);
-            d.y = fminf(fmaxf(d.y, -65504.f), 65504.f);
-          }
-          dd[c / 2 + i] = Half16<T>::pack(d.x, d.y);
+          dd[c / 2 + i] = Half16<T>::pack_sat(d.x, d.y);
         }
       }
       if (DKV) tmem_st16(xcol + h0, pp);  // over the scores that this thread has read
@@ -388,7 +386,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ds_full[buf]);
+      if (lane == 0) at_arrive(smem_u32(&ds_full[buf]));
       tile++;
     }
     const bool any = it > 0;

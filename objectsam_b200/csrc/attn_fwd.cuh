@@ -65,25 +65,36 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   const int r0 = qt * kAfRows, r_last = min(r0 + kAfRows, rows) - 1;
   const int n = at_keys(A, b), off = n - A.Lq;
   const int prefix = A.mask == OSAM_ATTN_PREFIX ? A.prefix[b] : 0;
-  const int lim_max = at_limit(A, n, prefix, off + r_last / A.G), lim_min = at_limit(A, n, prefix, off + r0 / A.G);
+  const int lim_max = at_limit(A, n, prefix, off + A.f_g.quo(r_last)), lim_min = at_limit(A, n, prefix, off + A.f_g.quo(r0));
   AtTiles tiles;
   tiles.begin = split * P.tiles_per_split;
   tiles.end = max(tiles.begin, min((lim_max + KEYS - 1) / KEYS, tiles.begin + P.tiles_per_split));
-  tiles.from = min(max((off + r_last / A.G) / KEYS, tiles.begin), tiles.end - 1);
+  tiles.from = min(max((off + A.f_g.quo(r_last)) / KEYS, tiles.begin), tiles.end - 1);
   const bool docs = A.doc_q != nullptr;
   tiles.live = docs ? live : nullptr;
 
   // ---- this thread's row
   const int r = r0 + tid % kAfRows;
   const bool valid = warp < 8 && r < rows;
-  const int qi = valid ? r / A.G : 0, head = hk * A.G + (valid ? r - qi * A.G : 0);
+  const int qi = valid ? A.f_g.quo(r) : 0, head = hk * A.G + (valid ? r - qi * A.G : 0);
   int my_doc = -2;
   if (valid && docs) {
     my_doc = A.doc_q[(long long)b * A.Lq + qi];
     if (my_doc < 0) my_doc = -2;
   }
 
-  if (tid == 0) {
+  // the producer warp sets the barriers up and, where no document summaries have to be looked through first, starts
+  // loading at once, under the rest of the prologue
+  int made = 0, next_tile = tiles.end;
+  auto load = [&](int it, int t, bool v) {
+    const int s = it % Cfg::STAGES;
+    uint64_t* bar = v ? &v_full[s] : &k_full[s];
+    mbar_arrive_expect_tx(bar, Cfg::TILE);
+    for (int p = 0; p < Cfg::PANELS; p++)
+      tma_load_4d(smem + Cfg::QTILE + ((v ? Cfg::STAGES : 0) + s) * Cfg::TILE + p * Cfg::KPANEL, v ? &P.tv : &P.tk, bar,
+                  p * 64, t * KEYS, hk, b);
+  };
+  if (warp == 8 && lane == 0) {
     for (int i = 0; i < Cfg::STAGES; i++) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -97,8 +108,11 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     mbar_init(&pv_done, 1);
     mbar_init(&o_done, 1);
     fence_barrier_init();
-    tma_prefetch_desc(&P.tk);
-    tma_prefetch_desc(&P.tv);
+    if (!docs)
+      for (next_tile = tiles.first(); made < Cfg::STAGES && next_tile < tiles.end; next_tile = tiles.next(next_tile), made++) {
+        load(made, next_tile, false);
+        load(made, next_tile, true);
+      }
   }
   if (warp == 9) {
     tmem_alloc(&tmem_slot, 256);
@@ -113,7 +127,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       const int row = c / CH, ch = c % CH, rr = r0 + row;
       uint4 u = make_uint4(0, 0, 0, 0);
       if (rr < rows && ch * 8 < A.D) {
-        const int i = rr / A.G, h = hk * A.G + rr - i * A.G;
+        const int i = A.f_g.quo(rr), h = hk * A.G + rr - i * A.G;
         u = *reinterpret_cast<const uint4*>(q + i * P.q.st + h * P.q.sh + ch * 8);
       }
       *reinterpret_cast<uint4*>(smem + (ch / 8) * Cfg::QPANEL + at_sw128(row, ch % 8)) = u;
@@ -148,23 +162,18 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
 
   if (warp == 8) {
     if (lane == 0) {
-      int it = 0;
-      bool ok = true;
-      for (int t = tiles.first(); t < tiles.end; t = tiles.next(t), it++) {
+      if (docs) next_tile = tiles.first();
+      int it = made;
+      for (int t = next_tile; t < tiles.end; t = tiles.next(t), it++) {
         const int s = it % Cfg::STAGES;
         const uint32_t ph = ((it / Cfg::STAGES) & 1) ^ 1;
-        if (it >= Cfg::STAGES && !(ok = at_wait(&k_empty[s], ph, A.err))) break;
-        mbar_arrive_expect_tx(&k_full[s], Cfg::TILE);
-        for (int p = 0; p < Cfg::PANELS; p++)
-          tma_load_4d(smem + Cfg::QTILE + s * Cfg::TILE + p * Cfg::KPANEL, &P.tk, &k_full[s], p * 64, t * KEYS, hk, b);
-        if (it >= Cfg::STAGES && !(ok = at_wait(&v_empty[s], ph, A.err))) {
+        if (it >= Cfg::STAGES && !at_wait(&k_empty[s], ph, A.err)) break;
+        load(it, t, false);
+        if (it >= Cfg::STAGES && !at_wait(&v_empty[s], ph, A.err)) {
           at_wait(&k_full[s], (it / Cfg::STAGES) & 1, A.err);
           break;
         }
-        mbar_arrive_expect_tx(&v_full[s], Cfg::TILE);
-        for (int p = 0; p < Cfg::PANELS; p++)
-          tma_load_4d(smem + Cfg::QTILE + (Cfg::STAGES + s) * Cfg::TILE + p * Cfg::KPANEL, &P.tv, &v_full[s], p * 64,
-                      t * KEYS, hk, b);
+        load(it, t, true);
       }
       // no copy of this CTA may be in flight when it ends
       for (int i = max(0, it - Cfg::STAGES); i < it; i++) {
@@ -295,7 +304,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
               ky = *reinterpret_cast<const float4*>(&col_y[it & 1][h0 + c]);
               kx = *reinterpret_cast<const float4*>(&col_x[it & 1][h0 + c]);
             }
-            at_scores4<CAP, BIAS>(bias, s2, none, line, ky, kx, sig);
+            at_scores4<CAP, BIAS, false>(bias, s2, none, line, ky, kx, sig);
             x[c] = s2[0].x;
             x[c + 1] = s2[0].y;
             x[c + 2] = s2[1].x;
