@@ -116,7 +116,30 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
   const bool docs = A.doc_q != nullptr;
   tiles.live = docs ? live : nullptr;
 
-  if (tid == 0) {
+  // the producer warp sets the barriers up and, where no document summaries have to be looked through first, starts
+  // loading at once, under the rest of the prologue
+  AbIter made;
+  made.start(tiles);
+  int n_made = 0;
+  auto load_stat = [&]() {
+    mbar_arrive_expect_tx(&stat_full, 2 * Cfg::STAT);
+    for (int p = 0; p < Cfg::PANELS; p++) {
+      tma_load_4d(smem + p * kAbRows * 128, &P.stat1, &stat_full, p * 64, row0, hd, b);
+      tma_load_4d(smem + Cfg::STAT + p * kAbRows * 128, &P.stat2, &stat_full, p * 64, row0, hd, b);
+    }
+  };
+  auto load_strm = [&](int it, const AbIter& x) {
+    const int s = it % Cfg::STAGES, h = DKV ? hd * A.G + x.g : hd / A.G;
+    uint8_t* d = strm + s * 2 * Cfg::STRM;
+    mbar_arrive_expect_tx(&full[s], 2 * Cfg::STRM + (DKV ? Cfg::ROWS : 0));
+    for (int p = 0; p < Cfg::PANELS; p++) {
+      tma_load_4d(d + p * kAbCols * 128, &P.strm1, &full[s], p * 64, x.t * kAbCols, h, b);
+      tma_load_4d(d + Cfg::STRM + p * kAbCols * 128, &P.strm2, &full[s], p * 64, x.t * kAbCols, h, b);
+    }
+    if (DKV)
+      bulk_load(srows + s * Cfg::ROWS, P.rows + (((long long)b * A.Hq + h) * nq64 + x.t) * 2 * kAbCols, Cfg::ROWS, &full[s]);
+  };
+  if (warp == 8 * NB && lane == 0) {
     mbar_init(&stat_full, 1);
     for (int i = 0; i < Cfg::STAGES; i++) {
       mbar_init(&full[i], 1);
@@ -128,10 +151,10 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     }
     mbar_init(&acc_done, 1);
     fence_barrier_init();
-    tma_prefetch_desc(&P.stat1);
-    tma_prefetch_desc(&P.stat2);
-    tma_prefetch_desc(&P.strm1);
-    tma_prefetch_desc(&P.strm2);
+    if (!docs && made.more(tiles, streams)) {
+      load_stat();
+      for (; n_made < Cfg::STAGES && made.more(tiles, streams); made.step(tiles), n_made++) load_strm(n_made, made);
+    }
   }
   if (warp == 8 * NB + 1) {
     tmem_alloc(&tmem_slot, Cfg::TMEM);
@@ -149,33 +172,17 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
 
   if (warp == 8 * NB) {
     if (lane == 0) {
-      AbIter x;
-      x.start(tiles);
-      const bool any = x.more(tiles, streams);
-      if (any) {
-        mbar_arrive_expect_tx(&stat_full, 2 * Cfg::STAT);
-        for (int p = 0; p < Cfg::PANELS; p++) {
-          tma_load_4d(smem + p * kAbRows * 128, &P.stat1, &stat_full, p * 64, row0, hd, b);
-          tma_load_4d(smem + Cfg::STAT + p * kAbRows * 128, &P.stat2, &stat_full, p * 64, row0, hd, b);
-        }
+      if (docs) {
+        made.start(tiles);
+        if (made.more(tiles, streams)) load_stat();
       }
-      int it = 0;
-      for (; x.more(tiles, streams); x.step(tiles), it++) {
-        const int s = it % Cfg::STAGES;
-        if (it >= Cfg::STAGES && !at_wait(&empty[s], ((it / Cfg::STAGES) & 1) ^ 1, A.err)) break;
-        uint8_t* d = strm + s * 2 * Cfg::STRM;
-        mbar_arrive_expect_tx(&full[s], 2 * Cfg::STRM + (DKV ? Cfg::ROWS : 0));
-        const int h = DKV ? hd * A.G + x.g : hd / A.G;
-        for (int p = 0; p < Cfg::PANELS; p++) {
-          tma_load_4d(d + p * kAbCols * 128, &P.strm1, &full[s], p * 64, x.t * kAbCols, h, b);
-          tma_load_4d(d + Cfg::STRM + p * kAbCols * 128, &P.strm2, &full[s], p * 64, x.t * kAbCols, h, b);
-        }
-        if (DKV)
-          bulk_load(srows + s * Cfg::ROWS, P.rows + (((long long)b * A.Hq + h) * nq64 + x.t) * 2 * kAbCols, Cfg::ROWS,
-                    &full[s]);
+      int it = n_made;
+      for (; made.more(tiles, streams); made.step(tiles), it++) {
+        if (it >= Cfg::STAGES && !at_wait(&empty[it % Cfg::STAGES], ((it / Cfg::STAGES) & 1) ^ 1, A.err)) break;
+        load_strm(it, made);
       }
       // no copy of this CTA may be in flight when it ends
-      if (any) at_wait(&stat_full, 0, A.err);
+      if (it > 0) at_wait(&stat_full, 0, A.err);
       for (int i = max(0, it - Cfg::STAGES); i < it; i++) at_wait(&full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, A.err);
     }
     __syncwarp();
