@@ -222,10 +222,20 @@ def check(rc: int) -> None:
         raise OsamError(rc, lib().osam_last_error().decode(errors="replace"))
 
 
+_raw_stream = None
+
+
 def stream_ptr(stream=None) -> int:
-    import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    """The CUDA stream handle of `stream`, or of the current device's current stream."""
+    if stream is not None:
+        return stream.cuda_stream
+    global _raw_stream
+    if _raw_stream is None:  # the handle without a Stream object around it, where this torch has that
+        import torch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _raw_stream = (lambda: raw(torch.cuda.current_device())) if raw is not None else \
+            (lambda: torch.cuda.current_stream().cuda_stream)
+    return _raw_stream()
 
 
 def device_error() -> int:

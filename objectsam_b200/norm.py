@@ -22,11 +22,13 @@ _DTYPE = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _ws_cache: dict = {}
 
 
-def _rows(t, like, dtype, name: str):
+def _rows(t, shape, dtype, name: str):
     """(pointer, elements from row to row) of a tensor whose leading dimensions are equally spaced rows."""
-    if t.dtype != dtype or t.shape != like.shape or not t.is_cuda:
-        raise ValueError(f"{name}: CUDA {dtype} of shape {tuple(like.shape)} expected")
-    shape, stride = t.shape, t.stride()
+    if t.dtype is not dtype or t.shape != shape or not t.is_cuda:
+        raise ValueError(f"{name}: CUDA {dtype} of shape {tuple(shape)} expected")
+    if t.is_contiguous():
+        return t.data_ptr(), shape[-1]
+    stride = t.stride()
     if stride[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name}: channels are contiguous")
     ld = n = 0
@@ -45,33 +47,36 @@ def _rows(t, like, dtype, name: str):
 def _f32(t, n: int, name: str):
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or not t.is_cuda:
+    if t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous() or not t.is_cuda:
         raise ValueError(f"{name}: contiguous CUDA float32 of {n} elements expected")
     return t.data_ptr()
 
 
 def _in(x):
-    if x.dtype not in _DTYPE:
+    """(type code, type, shape, channels, rows)"""
+    dtype, shape = x.dtype, x.shape
+    code = _DTYPE.get(dtype)
+    if code is None:
         raise ValueError("rms norm takes float16 or bfloat16")
-    C = x.shape[-1]
-    return _DTYPE[x.dtype], C, x.numel() // max(C, 1)
+    C = shape[-1]
+    return code, dtype, shape, C, x.numel() // max(C, 1)
 
 
 def rms_norm_fwd(x, w, eps: float, y, res=None, total=None, rstd=None, stream=None) -> None:
-    dtype, C, rows = _in(x)
-    r = (None, 0) if res is None else _rows(res, x, x.dtype, "res")
-    t = (None, 0) if total is None else _rows(total, x, x.dtype, "total")
-    check(lib().osam_rms_fwd(dtype, *_rows(x, x, x.dtype, "x"), *r, _f32(w, C, "w"), rows, C, eps, *t,
-                             *_rows(y, x, x.dtype, "y"), _f32(rstd, rows, "rstd"), stream_ptr(stream)))
+    code, dtype, shape, C, rows = _in(x)
+    r = (None, 0) if res is None else _rows(res, shape, dtype, "res")
+    t = (None, 0) if total is None else _rows(total, shape, dtype, "total")
+    check(lib().osam_rms_fwd(code, *_rows(x, shape, dtype, "x"), *r, _f32(w, C, "w"), rows, C, eps, *t,
+                             *_rows(y, shape, dtype, "y"), _f32(rstd, rows, "rstd"), stream_ptr(stream)))
 
 
 def rms_norm_fwd_q8(x, w, eps: float, q, qscale, res=None, total=None, rstd=None, stream=None) -> None:
     """q: float8_e4m3fn like x; qscale: float32 (rows, ⌈C/128⌉)."""
-    dtype, C, rows = _in(x)
-    r = (None, 0) if res is None else _rows(res, x, x.dtype, "res")
-    t = (None, 0) if total is None else _rows(total, x, x.dtype, "total")
-    check(lib().osam_rms_fwd_q8(dtype, *_rows(x, x, x.dtype, "x"), *r, _f32(w, C, "w"), rows, C, eps, *t,
-                                *_rows(q, x, torch.float8_e4m3fn, "q"), _f32(qscale, rows * -(-C // GROUP), "qscale"),
+    code, dtype, shape, C, rows = _in(x)
+    r = (None, 0) if res is None else _rows(res, shape, dtype, "res")
+    t = (None, 0) if total is None else _rows(total, shape, dtype, "total")
+    check(lib().osam_rms_fwd_q8(code, *_rows(x, shape, dtype, "x"), *r, _f32(w, C, "w"), rows, C, eps, *t,
+                                *_rows(q, shape, torch.float8_e4m3fn, "q"), _f32(qscale, rows * -(-C // GROUP), "qscale"),
                                 _f32(rstd, rows, "rstd"), stream_ptr(stream)))
 
 
@@ -91,9 +96,9 @@ def workspace(C: int, device, stream=None) -> torch.Tensor:
 def rms_norm_bwd(dy, h, w, rstd, dx, dw, dtotal=None, ws=None, stream=None) -> None:
     """h: the forward's total (its x where there was no residual); dtotal: the gradient that reaches h by the
     residual path."""
-    dtype, C, rows = _in(dy)
-    d = (None, 0) if dtotal is None else _rows(dtotal, dy, dy.dtype, "dtotal")
+    code, dtype, shape, C, rows = _in(dy)
+    d = (None, 0) if dtotal is None else _rows(dtotal, shape, dtype, "dtotal")
     ws = ws if ws is not None else workspace(C, dy.device, stream)
-    check(lib().osam_rms_bwd(dtype, *_rows(dy, dy, dy.dtype, "dy"), *_rows(h, dy, dy.dtype, "h"), _f32(w, C, "w"),
-                             _f32(rstd, rows, "rstd"), *d, rows, C, *_rows(dx, dy, dy.dtype, "dx"), _f32(dw, C, "dw"),
+    check(lib().osam_rms_bwd(code, *_rows(dy, shape, dtype, "dy"), *_rows(h, shape, dtype, "h"), _f32(w, C, "w"),
+                             _f32(rstd, rows, "rstd"), *d, rows, C, *_rows(dx, shape, dtype, "dx"), _f32(dw, C, "dw"),
                              ws.data_ptr(), ws.numel() * ws.element_size(), stream_ptr(stream)))
