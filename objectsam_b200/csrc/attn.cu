@@ -82,6 +82,26 @@ __global__ void __launch_bounds__(256) k_attn_join(const float* part, const floa
   if (lane == 0 && lse) lse[row] = l == 0.f ? -INFINITY : (M + at_lg2(l)) * kAtLn2;
 }
 
+// Adds the parts of one gradient in part order and rounds: a thread per 8 dims of a (batch, head, token) row.
+template <typename T>
+__global__ void __launch_bounds__(256) k_attn_sum(const float* part, int parts, long long stride, int heads, int L, int D,
+                                                  long long n8, AtView out) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  grid_dep_wait();
+  if (i >= n8) return;
+  float v[8] = {};
+  for (int p = 0; p < parts; p++) {
+    const float4* s = reinterpret_cast<const float4*>(part + p * stride + i * 8);
+    const float4 a = s[0], b = s[1];
+    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+  }
+  const int c8 = D / 8;
+  const long long row = i / c8, bh = row / L;
+  const int c = int(i - row * c8) * 8, t = int(row - bh * L), h = int(bh % heads);
+  *reinterpret_cast<uint4*>(static_cast<T*>(out.p) + bh / heads * out.sb + t * out.st + h * out.sh + c) = pack8<T>(v);
+}
+
 // Row terms of the backward pass, per 64-query block (padded to whole blocks): (u − lse·log2 e, −δ), δ = do·o, u = log2
 // of the factor that the backward holds P times — (−∞, 0) for that see nothing and for the padding, whose P is then 0 — and the block's largest |dO|.  One CTA per
 // block, 16 lanes per row (a 16-byte vector each).
@@ -204,11 +224,33 @@ AtSplit at_split(const osam_attn_desc& a) {
   return s;
 }
 
+// Into how many parts the backward splits the streamed side of a tile: by a model of its time in units of a streamed
+// tile (0.7 us measured): rounds of CTAs over the GPU × (tiles of a part + 5 for a CTA's start and end), and for the
+// parts' sum 8 and its traffic.  One part where the tiles fill the GPU (16 heads of 4096 tokens); with 2 key heads of
+// 8192 tokens (128 tiles for 296 places) two parts took dK and dV from 634 to 350 us.
+int at_parts(const osam_attn_desc& a, bool dkv) {
+  const int slots = kAtSms * (a.dim <= 64 ? 2 : 1), own = dkv ? a.len_k : a.len_q, other = dkv ? a.len_q : a.len_k;
+  const int heads = dkv ? a.heads_k : a.heads_q;
+  const double ctas = (double)((own + 127) / 128) * a.batch * heads;
+  const double tiles = (double)((other + 63) / 64) * (dkv ? a.heads_q / a.heads_k : 1) * (a.mask == OSAM_ATTN_NONE ? 1 : 0.5);
+  const double out_us = (double)own * a.batch * heads * a.dim * (dkv ? 2 : 1) * 8 / 4e6;
+  int best = 1;
+  double least = 1e30;
+  for (int p = 1; p <= 8 && (p == 1 || (other + 63) / 64 >= 4 * p); p++) {
+    const double t = std::ceil(ctas * p / slots) * (tiles / p + 5) + (p > 1 ? 8 + p * out_us / 0.7 : 0);
+    if (t < least) {
+      least = t;
+      best = p;
+    }
+  }
+  return best;
+}
+
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Workspace: document summaries | split outputs and statistics (forward) or row terms (backward).
 struct AtLayout {
-  size_t sum_q = 0, sum_k = 0, part = 0, stats = 0, rows = 0, peak = 0, bytes = 0;
+  size_t sum_q = 0, sum_k = 0, part = 0, stats = 0, rows = 0, peak = 0, grad = 0, bytes = 0;
 };
 AtLayout at_layout(const osam_attn_desc& a) {
   AtLayout L;
@@ -230,7 +272,11 @@ AtLayout at_layout(const osam_attn_desc& a) {
   }
   const size_t blocks = (size_t)a.batch * a.heads_q * ((a.len_q + kAbCols - 1) / kAbCols);
   L.peak = at + up256(blocks * 2 * kAbCols * sizeof(float));
-  L.bytes = std::max(fwd, L.peak + up256(blocks * sizeof(float)));
+  L.grad = L.peak + up256(blocks * sizeof(float));
+  const int pk = at_parts(a, true), pq = at_parts(a, false);
+  const size_t nk = (size_t)a.batch * a.heads_k * a.len_k * a.dim, nq = rows * a.dim;
+  const size_t grad = std::max(pk > 1 ? pk * 2 * nk : 0, pq > 1 ? pq * nq : 0) * sizeof(float);
+  L.bytes = std::max(fwd, L.grad + up256(grad));
   return L;
 }
 
@@ -369,7 +415,18 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   auto map = [&](CUtensorMap* m, const osam_view& t, bool query, int box) {
     return at_map(m, t, a->batch, query ? lq : lk, query ? hq : a->heads_k, a->dim, box, bf16);
   };
+  L.part = reinterpret_cast<float*>(w + W.grad);
+  auto sum = [&](const osam_view& out, int which, int outs, int heads, int len) {
+    const float* part = L.part + (size_t)which * a->batch * heads * len * a->dim;
+    long long n8 = (long long)a->batch * heads * len * (a->dim / 8), stride = n8 * 8 * outs;
+    int D = a->dim;
+    AtView v = at_view(out);
+    void* args[] = {&part, &L.parts, &stride, &heads, &len, &D, &n8, &v};
+    const void* k = bf16 ? (const void*)k_attn_sum<__nv_bfloat16> : (const void*)k_attn_sum<__half>;
+    return at_cuda(launch_dependent(k, (unsigned)((n8 + 255) / 256), 256, args, st), "sum launch");
+  };
   if (!ek) {
+    L.parts = at_parts(*a, true);
     if ((rc = map(&L.stat1, vk, false, kAbRows)) != OSAM_OK || (rc = map(&L.stat2, vv, false, kAbRows)) != OSAM_OK ||
         (rc = map(&L.strm1, vq, true, kAbCols)) != OSAM_OK || (rc = map(&L.strm2, vdo, true, kAbCols)) != OSAM_OK)
       return rc;
@@ -377,14 +434,18 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
     L.out2 = at_view(dv);
     const cudaError_t e = bf16 ? launch_attn_bwd<__nv_bfloat16, true>(L, st) : launch_attn_bwd<__half, true>(L, st);
     if (e != cudaSuccess) return at_cuda(e, "backward launch (dK, dV)");
+    if (L.parts > 1 && ((rc = sum(dk, 0, 2, a->heads_k, a->len_k)) != OSAM_OK || (rc = sum(dv, 1, 2, a->heads_k, a->len_k)) != OSAM_OK))
+      return rc;
   }
   if (!eq) {
+    L.parts = at_parts(*a, false);
     if ((rc = map(&L.stat1, vq, true, kAbRows)) != OSAM_OK || (rc = map(&L.stat2, vdo, true, kAbRows)) != OSAM_OK ||
         (rc = map(&L.strm1, vk, false, kAbCols)) != OSAM_OK || (rc = map(&L.strm2, vv, false, kAbCols)) != OSAM_OK)
       return rc;
     L.out1 = at_view(dq);
     const cudaError_t e = bf16 ? launch_attn_bwd<__nv_bfloat16, false>(L, st) : launch_attn_bwd<__half, false>(L, st);
     if (e != cudaSuccess) return at_cuda(e, "backward launch (dQ)");
+    if (L.parts > 1) return sum(dq, 0, 1, a->heads_q, a->len_q);
   }
   return OSAM_OK;
 }

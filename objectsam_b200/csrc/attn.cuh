@@ -431,6 +431,8 @@ struct AttnBwdLaunch {
   AtView out1, out2;      // dK, dV (DKV); dQ (DQ)
   const float* rows;      // [B][Hq][⌈Lq/64⌉][2][64]: log2 of P's factor − lse·log2 e (−∞ where the query is empty), −δ
   const float* peak;      // [B][Hq][⌈Lq/64⌉] max |dO| of the block
+  int parts;              // CTAs that share a tile's streamed side (few tiles: to fill the GPU); above 1 they write
+  float* part;            // [parts][outputs][B][heads][L][D] fp32, which k_attn_sum adds in order
 };
 template <typename T, bool DKV>
 cudaError_t launch_attn_bwd(const AttnBwdLaunch& L, cudaStream_t st);

@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
 
   // ---- which tile (with a causal bound the longest first)
   const int heads = DKV ? A.Hk : A.Hq, nt = ((DKV ? A.Lk : A.Lq) + kAbRows - 1) / kAbRows;
-  const int per = A.B * heads;
+  const int per = A.B * heads * P.parts;
   int rt, rest;
   if (A.mask == OSAM_ATTN_NONE) {
     rt = int(blockIdx.x) % nt;
@@ -93,6 +93,8 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     rest = int(blockIdx.x) % per;
     if (!DKV) rt = nt - 1 - rt;
   }
+  const int part = rest % P.parts;
+  rest /= P.parts;
   const int hd = rest % heads, b = rest / heads;
   const int row0 = rt * kAbRows;
   const int n = at_keys(A, b), off = n - A.Lq;
@@ -111,6 +113,12 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     tiles.begin = 0;
     tiles.end = (at_limit(A, n, prefix, off + last) + kAbCols - 1) / kAbCols;
     lim_min = at_limit(A, n, prefix, off + row0);
+  }
+  if (P.parts > 1) {
+    const int first = tiles.begin;
+    const long long len = max(0, tiles.end - first);
+    tiles.begin = first + int(len * part / P.parts);
+    tiles.end = first + int(len * (part + 1) / P.parts);
   }
   tiles.from = tiles.begin - 1;  // the order does not matter here: upwards
   const bool docs = A.doc_q != nullptr;
@@ -416,6 +424,14 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
 #pragma unroll
           for (int i = 0; i < 16; i++) a[i] = any ? a[i] * f : 0.f;
           if (!valid) continue;
+          if (P.parts > 1) {
+            float* f32 = P.part + ((((long long)part * outs + which) * A.B + b) * heads + hd) * ((long long)(DKV ? A.Lk : A.Lq) * A.D) +
+                         (long long)row * A.D + c;
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              if (c + i < A.D) *reinterpret_cast<float4*>(f32 + i) = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+            continue;
+          }
           const float lo8[8] = {a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7]};
           const float hi8[8] = {a[8], a[9], a[10], a[11], a[12], a[13], a[14], a[15]};
           *reinterpret_cast<uint4*>(o + c) = pack8<T>(lo8);
@@ -463,7 +479,7 @@ cudaError_t attn_bwd_dp(const AttnBwdLaunch& L, int grid, cudaStream_t st) {
 template <typename T, bool DKV>
 cudaError_t launch_attn_bwd(const AttnBwdLaunch& L, cudaStream_t st) {
   const int nt = ((DKV ? L.d.Lk : L.d.Lq) + kAbRows - 1) / kAbRows;
-  const int grid = nt * L.d.B * (DKV ? L.d.Hk : L.d.Hq);
+  const int grid = nt * L.d.B * (DKV ? L.d.Hk : L.d.Hq) * L.parts;
   if (grid == 0) return cudaSuccess;
   return L.d.D <= 64 ? attn_bwd_dp<T, 64, DKV>(L, grid, st) : attn_bwd_dp<T, 128, DKV>(L, grid, st);
 }
