@@ -15,6 +15,8 @@ __global__ void __launch_bounds__(256) k_attn_docs(const int* doc_q, const int* 
                                                    AtDocs* sk) {
   const int nq = (Lq + kAtDocBlock - 1) / kAtDocBlock, nk = (Lk + kAtDocBlock - 1) / kAtDocBlock;
   const int w = (blockIdx.x * 256 + threadIdx.x) / 32, lane = threadIdx.x % 32;
+  grid_dep_wait();
+  grid_dep_launch();
   const bool is_q = w < B * nq;
   const int i = is_q ? w : w - B * nq, nb = is_q ? nq : nk, L = is_q ? Lq : Lk;
   if (i >= B * nb) return;
@@ -50,6 +52,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const float* part, const floa
   const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / 32;
   const int lane = threadIdx.x % 32;
   grid_dep_wait();
+  grid_dep_launch();
   if (row >= nrows) return;
   float M = -INFINITY;
   for (int s = lane; s < splits; s += 32) M = fmaxf(M, stats[s * nrows + row].x);
@@ -88,6 +91,7 @@ __global__ void __launch_bounds__(256) k_attn_sum(const float* part, int parts, 
                                                   long long n8, AtView out) {
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   grid_dep_wait();
+  grid_dep_launch();
   if (i >= n8) return;
   float v[8] = {};
   for (int p = 0; p < parts; p++) {
@@ -114,6 +118,8 @@ __global__ void __launch_bounds__(256) k_attn_rows(const AtView o, const AtView 
   const int blk = blockIdx.x % nb, h = (blockIdx.x / nb) % Hq, b = blockIdx.x / nb / Hq;
   const int c = threadIdx.x % 16;
   const long long bh = (long long)b * Hq + h;
+  grid_dep_wait();
+  grid_dep_launch();
   float big = 0.f;
 #pragma unroll
   for (int k = 0; k < kAbCols; k += 16) {
@@ -296,23 +302,11 @@ int at_dev(const osam_attn_desc& a, const AtLayout& W, char* ws, AttnDev* A, cud
     A->sum_q = sq;
     A->sum_k = sk;
     const long long warps = (long long)a.batch * ((a.len_q + 63) / 64 + (a.len_k + 63) / 64);
-    k_attn_docs<<<(unsigned)((warps + 7) / 8), 256, 0, st>>>(a.doc_q, a.doc_k, a.batch, a.len_q, a.len_k, sq, sk);
-    return at_cuda(cudaGetLastError(), "document summaries");
+    return at_cuda(launch_dependent(k_attn_docs, (unsigned)((warps + 7) / 8), 256, 0, st, a.doc_q, a.doc_k, a.batch, a.len_q,
+                                    a.len_k, sq, sk),
+                   "document summaries");
   }
   return OSAM_OK;
-}
-
-cudaError_t launch_dependent(const void* k, unsigned grid, unsigned threads, void** args, cudaStream_t st) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelExC(&cfg, k, args);
 }
 
 }  // namespace
@@ -360,13 +354,11 @@ int osam_attn_fwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   L.stats = reinterpret_cast<float2*>(w + W.stats);
   cudaError_t e = bf16 ? launch_attn_fwd<__nv_bfloat16>(L, st) : launch_attn_fwd<__half>(L, st);
   if (e != cudaSuccess || s.splits == 1) return at_cuda(e, "forward launch");
-  long long nrows = (long long)a->batch * a->heads_q * a->len_q;
-  const float* part = L.part;
-  const float2* stats = L.stats;
-  int splits = s.splits, Hq = a->heads_q, Lq = a->len_q, D = a->dim;
-  void* args[] = {&part, &stats, &splits, &nrows, &Hq, &Lq, &D, &L.o, &lse};
-  const void* join = bf16 ? (const void*)k_attn_join<__nv_bfloat16> : (const void*)k_attn_join<__half>;
-  return at_cuda(launch_dependent(join, (unsigned)((nrows + 7) / 8), 256, args, st), "join launch");
+  const long long nrows = (long long)a->batch * a->heads_q * a->len_q;
+  const unsigned grid = (unsigned)((nrows + 7) / 8);
+  e = launch_dependent(bf16 ? k_attn_join<__nv_bfloat16> : k_attn_join<__half>, grid, 256, 0, st, (const float*)L.part,
+                       (const float2*)L.stats, s.splits, nrows, a->heads_q, a->len_q, a->dim, L.o, lse);
+  return at_cuda(e, "join launch");
 }
 
 int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v, osam_view o, const float* lse,
@@ -400,11 +392,10 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   float* peak = reinterpret_cast<float*>(w + W.peak);
   const int blocks = a->batch * a->heads_q * ((a->len_q + kAbCols - 1) / kAbCols);
   if (blocks > 0) {
-    if (bf16)
-      k_attn_rows<__nv_bfloat16><<<blocks, 256, 0, st>>>(at_view(o), at_view(dout), lse, a->heads_q, a->len_q, a->dim, rows, peak);
-    else
-      k_attn_rows<__half><<<blocks, 256, 0, st>>>(at_view(o), at_view(dout), lse, a->heads_q, a->len_q, a->dim, rows, peak);
-    if ((rc = at_cuda(cudaGetLastError(), "row terms")) != OSAM_OK) return rc;
+    if ((rc = at_cuda(launch_dependent(bf16 ? k_attn_rows<__nv_bfloat16> : k_attn_rows<__half>, blocks, 256, 0, st, at_view(o),
+                                       at_view(dout), lse, a->heads_q, a->len_q, a->dim, rows, peak),
+                      "row terms")) != OSAM_OK)
+      return rc;
   }
   L.rows = rows;
   L.peak = peak;
@@ -417,13 +408,11 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   };
   L.part = reinterpret_cast<float*>(w + W.grad);
   auto sum = [&](const osam_view& out, int which, int outs, int heads, int len) {
-    const float* part = L.part + (size_t)which * a->batch * heads * len * a->dim;
-    long long n8 = (long long)a->batch * heads * len * (a->dim / 8), stride = n8 * 8 * outs;
-    int D = a->dim;
-    AtView v = at_view(out);
-    void* args[] = {&part, &L.parts, &stride, &heads, &len, &D, &n8, &v};
-    const void* k = bf16 ? (const void*)k_attn_sum<__nv_bfloat16> : (const void*)k_attn_sum<__half>;
-    return at_cuda(launch_dependent(k, (unsigned)((n8 + 255) / 256), 256, args, st), "sum launch");
+    const long long n8 = (long long)a->batch * heads * len * (a->dim / 8);
+    return at_cuda(launch_dependent(bf16 ? k_attn_sum<__nv_bfloat16> : k_attn_sum<__half>, (unsigned)((n8 + 255) / 256), 256, 0,
+                                    st, (const float*)(L.part + which * n8 * 8), L.parts, n8 * 8 * outs, heads, len, a->dim, n8,
+                                    at_view(out)),
+                   "sum launch");
   };
   if (!ek) {
     L.parts = at_parts(*a, true);
@@ -439,6 +428,7 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   }
   if (!eq) {
     L.parts = at_parts(*a, false);
+    L.late = !ek && L.parts == 1;  // its own parts would go over those that a sum in front still reads
     if ((rc = map(&L.stat1, vq, true, kAbRows)) != OSAM_OK || (rc = map(&L.stat2, vdo, true, kAbRows)) != OSAM_OK ||
         (rc = map(&L.strm1, vk, false, kAbCols)) != OSAM_OK || (rc = map(&L.strm2, vv, false, kAbCols)) != OSAM_OK)
       return rc;

@@ -11,6 +11,8 @@
 #pragma once
 #include <limits.h>
 
+#include <utility>
+
 #include "conv_internal.h"
 #include "half16.cuh"
 #include "pair_math.cuh"
@@ -409,6 +411,24 @@ __device__ __forceinline__ void at_doc_bits(const AtDocs& own, const AtDocs* s, 
   }
 }
 
+// Every kernel here is launched with the programmatic-serialization attribute: it may be scheduled while the kernel
+// in front of it drains, sets itself up and then waits for that kernel's end (grid_dep_wait) before its first
+// global access.
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*k)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k, std::forward<A>(args)...);
+}
+
 // ---- host side (attn.cu): one call's launches
 struct AttnFwdLaunch {
   AttnDev d;
@@ -431,6 +451,7 @@ struct AttnBwdLaunch {
   AtView out1, out2;      // dK, dV (DKV); dQ (DQ)
   const float* rows;      // [B][Hq][⌈Lq/64⌉][2][64]: log2 of P's factor − lse·log2 e (−∞ where the query is empty), −δ
   const float* peak;      // [B][Hq][⌈Lq/64⌉] max |dO| of the block
+  int late;               // DQ behind DKV, which it does not depend on: waits for that kernel's end only at its own end
   int parts;              // CTAs that share a tile's streamed side (few tiles: to fill the GPU); above 1 they write
   float* part;            // [parts][outputs][B][heads][L][D] fp32, which k_attn_sum adds in order
 };

@@ -75,6 +75,8 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
   __shared__ __align__(16) int col_doc[NB][2][kAbCols];
   __shared__ __align__(16) float col_y[NB][BIAS == 2 ? 2 : 1][kAbCols], col_x[NB][BIAS == 2 ? 2 : 1][kAbCols];
 
+  if (!P.late) grid_dep_wait();
+  grid_dep_launch();
   const AttnDev& A = P.d;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   uint8_t* smem = ab_raw + ((1024 - (smem_u32(ab_raw) & 1023)) & 1023);
@@ -440,6 +442,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
       }
     }
   }
+  if (P.late) grid_dep_wait();  // what waits for this kernel's end then waits for the one in front too
   tc_fence_before();
   __syncthreads();
   if (warp == 8 * NB + 1) {
@@ -460,8 +463,7 @@ cudaError_t attn_bwd_one(const AttnBwdLaunch& L, int grid, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     if (dev < 64) set[dev] = true;
   }
-  k<<<grid, AbCfg<DP>::THREADS, AbCfg<DP>::SMEM, st>>>(L);
-  return cudaGetLastError();
+  return launch_dependent(k, grid, AbCfg<DP>::THREADS, AbCfg<DP>::SMEM, st, L);
 }
 
 template <typename T, int DP, bool DKV>

@@ -49,6 +49,8 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   __shared__ __align__(16) int col_doc[2][KEYS];
   __shared__ __align__(16) float col_y[BIAS == 2 ? 2 : 1][KEYS], col_x[BIAS == 2 ? 2 : 1][KEYS];
 
+  grid_dep_wait();
+  grid_dep_launch();
   const AttnDev& A = P.d;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   uint8_t* smem = af_raw + ((1024 - (smem_u32(af_raw) & 1023)) & 1023);
@@ -441,8 +443,7 @@ cudaError_t attn_fwd_one(const AttnFwdLaunch& L, int grid, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     if (dev < 64) set[dev] = true;
   }
-  k<<<grid, kAfThreads, AfCfg<DP>::SMEM, st>>>(L);
-  return cudaGetLastError();
+  return launch_dependent(k, grid, kAfThreads, AfCfg<DP>::SMEM, st, L);
 }
 
 template <typename T, int DP>

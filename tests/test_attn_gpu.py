@@ -332,3 +332,14 @@ def test_refusals_with_tensors(cuda_lib):
     with pytest.raises(_lib.OsamError):  # strides of 12 elements
         flat = torch.zeros(2 * 16 * 2 * 76, dtype=q.dtype, device=DEV)
         op.fwd(torch.as_strided(flat, (2, 16, 2, 64), (16 * 2 * 76, 2 * 76, 76, 1)), k, v, o, ws=ws)
+
+
+@pytest.mark.parametrize("mask", ["none", "causal", "prefix"])
+@pytest.mark.parametrize("D", [40, 128])
+def test_long_rows_of_few_heads(cuda_lib, mask, D):
+    """Few tiles and long rows: a key tile's queries (and a query tile's keys) are shared among CTAs and summed."""
+    L = 1150
+    q, k, v, do = make(1, L, L, 4, 1, D, seed=17)
+    doc = torch.arange(L, dtype=torch.int32, device=DEV).div(500, rounding_mode="floor").int()[None].contiguous()
+    check(q, k, v, do, mask=mask, doc_q=doc, doc_k=doc,
+          prefix=torch.tensor([600], dtype=torch.int32, device=DEV) if mask == "prefix" else None)
