@@ -68,8 +68,9 @@ class AttnOp:
             check(lib().osam_attn_fwd(ctypes.byref(d), View(), View(), View(), View(), None, None, 0, None))
         self._keep = (slopes, lens, prefix, doc_q, doc_k)
         self._g, self._d, self._ref, self._ws = g, d, ctypes.byref(d), {}
-        self._q = (g.batch, g.len_q, g.heads_q, g.dim)
-        self._k = (g.batch, g.len_k, g.heads_k, g.dim)
+        self._dtype = g.dtype
+        self._q = torch.Size((g.batch, g.len_q, g.heads_q, g.dim))
+        self._k = torch.Size((g.batch, g.len_k, g.heads_k, g.dim))
         return self
 
     def geom(self) -> AttnGeom:
@@ -81,8 +82,8 @@ class AttnOp:
     tune = workspace_size  # as ConvOp.tune: nothing is timed
 
     def _view(self, t, shape, name: str) -> View:
-        if t.dtype != self._g.dtype or tuple(t.shape) != shape or not t.is_cuda:
-            raise ValueError(f"{name}: CUDA {self._g.dtype} of shape {shape} expected")
+        if t.dtype is not self._dtype or t.shape != shape or not t.is_cuda:
+            raise ValueError(f"{name}: CUDA {self._dtype} of shape {tuple(shape)} expected")
         sb, st, sh, sd = t.stride()
         if sd != 1 and shape[3] > 1:
             raise ValueError(f"{name}: the head dimension is contiguous")

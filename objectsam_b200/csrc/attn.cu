@@ -44,35 +44,62 @@ __global__ void __launch_bounds__(256) k_attn_docs(const int* doc_q, const int* 
   if (lane == 0) (is_q ? sq : sk)[i] = s;
 }
 
-// Joins the key splits: one warp per output row.  o = Σ 2^(m_s − M) o_s / Σ 2^(m_s − M) l_s over the splits, in
-// split order.
+// Joins the key splits: o = Σ 2^(m_s − M) o_s / Σ 2^(m_s − M) l_s over the splits.  `W` warps share a row and take
+// every W-th split each, four loads in flight; their sums are added in warp order.  (One warp a row took as long for
+// 64 splits as the attention in front of it.)
 template <typename T>
-__global__ void __launch_bounds__(256) k_attn_join(const float* part, const float2* stats, int splits, long long nrows,
+__global__ void __launch_bounds__(256) k_attn_join(const float* part, const float2* stats, int splits, int W, long long nrows,
                                                    int Hq, int Lq, int D, AtView o, float* lse) {
-  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / 32;
-  const int lane = threadIdx.x % 32;
+  __shared__ float4 acc_of[8][32];
+  __shared__ float l_of[8];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, w = warp % W;
+  const long long row = (long long)blockIdx.x * (8 / W) + warp / W;
+  const bool live = row < nrows;
   grid_dep_wait();
   grid_dep_launch();
-  if (row >= nrows) return;
-  float M = -INFINITY;
-  for (int s = lane; s < splits; s += 32) M = fmaxf(M, stats[s * nrows + row].x);
-#pragma unroll
-  for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int s = 0; s < splits; s++) {
-    const float2 st = stats[s * nrows + row];
-    if (st.y == 0.f) continue;  // no key in this split
-    const float w = at_ex2(st.x - M);
-    l = fmaf(w, st.y, l);
-    if (lane * 4 < D) {
-      const float4 v = *reinterpret_cast<const float4*>(part + (s * nrows + row) * D + lane * 4);
-      acc.x = fmaf(w, v.x, acc.x);
-      acc.y = fmaf(w, v.y, acc.y);
-      acc.z = fmaf(w, v.z, acc.z);
-      acc.w = fmaf(w, v.w, acc.w);
+  float l = 0.f, M = -INFINITY;
+  if (live) {
+    for (int s = lane; s < splits; s += 32) M = fmaxf(M, stats[s * nrows + row].x);
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+    for (int s0 = w; s0 < splits; s0 += 4 * W) {
+      float2 st[4];
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int s = s0 + k * W;
+        st[k] = s < splits ? stats[s * nrows + row] : make_float2(0.f, 0.f);
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s < splits && lane * 4 < D) v[k] = *reinterpret_cast<const float4*>(part + (s * nrows + row) * D + lane * 4);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        if (st[k].y == 0.f) continue;  // no key in this split
+        const float f = at_ex2(st[k].x - M);
+        l = fmaf(f, st[k].y, l);
+        acc.x = fmaf(f, v[k].x, acc.x);
+        acc.y = fmaf(f, v[k].y, acc.y);
+        acc.z = fmaf(f, v[k].z, acc.z);
+        acc.w = fmaf(f, v[k].w, acc.w);
+      }
     }
   }
+  if (W > 1) {
+    acc_of[warp][lane] = acc;
+    if (lane == 0) l_of[warp] = l;
+    __syncthreads();
+    if (w != 0) return;
+    for (int i = 1; i < W; i++) {
+      const float4 a = acc_of[warp + i][lane];
+      acc.x += a.x;
+      acc.y += a.y;
+      acc.z += a.z;
+      acc.w += a.w;
+      l += l_of[warp + i];
+    }
+  }
+  if (!live) return;
   const long long bh = row / Lq;
   const int i = int(row - bh * Lq), h = int(bh % Hq);
   const long long b = bh / Hq;
@@ -215,16 +242,19 @@ int at_map(CUtensorMap* tm, const osam_view& v, int batch, int len, int heads, i
   return make_map(tm, v.p, 4, dims, st, box, 128, bf16);
 }
 
-// How the keys are split: nothing to gain once the query tiles fill the GPU.
+// How the keys are split.  Nothing is gained once the query tiles fill the GPU; below, up to four CTAs an SM (uneven
+// caches balance; 16 sequences over caches of 8192–32768 keys: 282 us, with two an SM 289, with eight 291) of at
+// least 256 keys, 512 over long caches (one sequence, 4 heads, 32768 keys: 19 us, with 256 keys 26).  The join costs a
+// launch: a cache of 517 keys takes 11 us whole and 15 in two, one of 860 keys 21 and 15.
 struct AtSplit {
   int splits, tiles;
 };
 AtSplit at_split(const osam_attn_desc& a) {
-  const int keys = 64, tiles = (a.len_k + keys - 1) / keys;
+  const int tiles = (a.len_k + kAfKeys - 1) / kAfKeys;
   const long long ctas = (((long long)a.len_q * (a.heads_q / a.heads_k) + 127) / 128) * a.batch * a.heads_k;
   AtSplit s{1, std::max(tiles, 1)};
-  if (ctas == 0 || a.len_k < 512 || ctas >= 2 * kAtSms) return s;
-  const int want = (int)std::min<long long>((4LL * kAtSms + ctas - 1) / ctas, a.len_k / 256);
+  if (ctas == 0 || a.len_k < 768 || ctas >= 2 * kAtSms) return s;
+  const int want = (int)std::min<long long>((4LL * kAtSms + ctas - 1) / ctas, a.len_k / (a.len_k <= 2048 ? 256 : 512));
   s.tiles = (tiles + want - 1) / want;
   s.splits = (tiles + s.tiles - 1) / s.tiles;
   return s;
@@ -338,12 +368,11 @@ int osam_attn_fwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   AttnFwdLaunch L{};
   if ((rc = at_dev(*a, W, w, &L.d, st)) != OSAM_OK) return rc;
   const bool bf16 = a->dtype == OSAM_BF16;
-  const int keys = 64;
   // without keys every query is empty: no tile is visited, so the maps only have to be valid
   const osam_view& kk = a->len_k > 0 ? k : q;
   const osam_view& vv = a->len_k > 0 ? v : q;
-  if ((rc = at_map(&L.tk, kk, a->batch, std::max(a->len_k, 1), a->heads_k, a->dim, keys, bf16)) != OSAM_OK ||
-      (rc = at_map(&L.tv, vv, a->batch, std::max(a->len_k, 1), a->heads_k, a->dim, keys, bf16)) != OSAM_OK)
+  if ((rc = at_map(&L.tk, kk, a->batch, std::max(a->len_k, 1), a->heads_k, a->dim, kAfKeys, bf16)) != OSAM_OK ||
+      (rc = at_map(&L.tv, vv, a->batch, std::max(a->len_k, 1), a->heads_k, a->dim, kAfKeys, bf16)) != OSAM_OK)
     return rc;
   L.q = at_view(q);
   L.o = at_view(o);
@@ -355,9 +384,10 @@ int osam_attn_fwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   cudaError_t e = bf16 ? launch_attn_fwd<__nv_bfloat16>(L, st) : launch_attn_fwd<__half>(L, st);
   if (e != cudaSuccess || s.splits == 1) return at_cuda(e, "forward launch");
   const long long nrows = (long long)a->batch * a->heads_q * a->len_q;
-  const unsigned grid = (unsigned)((nrows + 7) / 8);
+  const int warps = s.splits <= 4 ? 1 : s.splits <= 16 ? 4 : 8;
+  const unsigned grid = (unsigned)((nrows + 8 / warps - 1) / (8 / warps));
   e = launch_dependent(bf16 ? k_attn_join<__nv_bfloat16> : k_attn_join<__half>, grid, 256, 0, st, (const float*)L.part,
-                       (const float2*)L.stats, s.splits, nrows, a->heads_q, a->len_q, a->dim, L.o, lse);
+                       (const float2*)L.stats, s.splits, warps, nrows, a->heads_q, a->len_q, a->dim, L.o, lse);
   return at_cuda(e, "join launch");
 }
 

@@ -430,6 +430,7 @@ cudaError_t launch_dependent(void (*k)(P...), unsigned grid, unsigned threads, s
 }
 
 // ---- host side (attn.cu): one call's launches
+constexpr int kAfRows = 128, kAfKeys = 64;  // a forward CTA's query rows, and the keys of a tile
 struct AttnFwdLaunch {
   AttnDev d;
   CUtensorMap tk, tv;

@@ -19,7 +19,6 @@
 
 namespace osam {
 
-constexpr int kAfRows = 128, kAfKeys = 64;
 constexpr int kAfSoft = 256;    // softmax threads
 constexpr int kAfThreads = kAfSoft + 64;
 constexpr float kAfGrow = 8.f;  // log2 growth over a row's reference maximum that forces a rescale
