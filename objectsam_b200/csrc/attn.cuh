@@ -302,11 +302,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Bounded wait (as mbar_wait) without the suspend-time hint, with which the test sleeps in steps of a microsecond and
-// more (about a tile's time), and bounded by a count, which costs the waiting loop nothing: one test takes tens of
-// cycles at least, so 2^25 take from about half a second to a few.
-constexpr uint32_t kAtWaitTests = 1u << 25;
+// more (about a tile's time); the clock is read every 1024 tests, which keeps the loop to a few instructions.
 __device__ __forceinline__ bool at_wait(uint32_t bar, uint32_t parity, int* err) {
-  for (uint32_t n = 0;; n++) {
+  unsigned long long t0 = 0;
+  for (uint32_t n = 1;; n++) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -316,7 +315,11 @@ __device__ __forceinline__ bool at_wait(uint32_t bar, uint32_t parity, int* err)
         : "r"(bar), "r"(parity)
         : "memory");
     if (done) return true;
-    if (n == kAtWaitTests) break;
+    if (n % 1024 == 0) {
+      const unsigned long long t = globaltimer();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > kWaitBudgetNs) break;
+    }
   }
   record_error(err, kDevErrTimeout);
   return false;

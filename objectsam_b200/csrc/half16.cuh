@@ -26,8 +26,6 @@ struct Half16<__half> {
     asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
   }
-  static __device__ __forceinline__ float to_float(__half h) { return __half2float(h); }
-  static __device__ __forceinline__ __half from_float(float f) { return __float2half_rn(f); }
 };
 
 template <>
@@ -41,8 +39,6 @@ struct Half16<__nv_bfloat16> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ uint32_t pack_sat(float a, float b) { return pack(a, b); }
-  static __device__ __forceinline__ float to_float(__nv_bfloat16 h) { return __bfloat162float(h); }
-  static __device__ __forceinline__ __nv_bfloat16 from_float(float f) { return __float2bfloat16_rn(f); }
 };
 
 template <typename T>
