@@ -30,6 +30,7 @@
 
 #include "conv_internal.h"
 #include "half16.cuh"
+#include "launch.cuh"
 #include "pair_math.cuh"
 #include "sm100.cuh"
 
@@ -140,6 +141,8 @@ __global__ void __launch_bounds__(kAdThreads, 8) k_adamw_norm(const AdChunk* chu
                                                            float max_norm, float* norm) {
   __shared__ double red[kAdThreads / 32];
   __shared__ bool last;
+  grid_dep_wait();
+  grid_dep_launch();
   float s = 0.f;
   AdChunk next;
   if ((int)blockIdx.x < nchunks) next = ad_chunk(chunks + blockIdx.x);
@@ -382,8 +385,9 @@ __device__ __forceinline__ void ad_update(const AdChunk& T, const AdState& S, co
 template <bool Q8>
 __global__ void __launch_bounds__(kAdThreads, 4) k_adamw(const AdChunk* chunks, const AdState S, const AdHyper H,
                                                          const AdNorm* norm, float scale) {
-  const AdChunk T = ad_chunk(chunks + blockIdx.x);
+  const AdChunk T = ad_chunk(chunks + blockIdx.x);  // of the table, which no kernel writes
   grid_dep_wait();
+  grid_dep_launch();
   AdData<Q8> d;
   ad_load<Q8>(T, S, d);
   float mul = scale;
@@ -538,23 +542,14 @@ int osam_adamw_step(const osam_adamw* a, void* m, void* v, float* m_scale, float
   H.eps = (float)eps;
   H.keep = (float)(1.0 - lr * weight_decay);
   const float gs = (float)grad_scale;
+  cudaError_t e = cudaSuccess;
   if (clip) {
-    const int grid = (int)std::min<long long>(a->chunks, kAdNormCtas);
-    k_adamw_norm<<<grid, kAdThreads, 0, st>>>(chunks, (int)a->chunks, ns, gs, (float)max_norm, norm);
+    const unsigned grid = (unsigned)std::min<long long>(a->chunks, kAdNormCtas);
+    e = launch_dependent(k_adamw_norm, grid, kAdThreads, 0, st, chunks, (int)a->chunks, ns, gs, (float)max_norm, norm);
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)a->chunks);
-  cfg.blockDim = dim3(kAdThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = clip ? 1 : 0;
-  cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess)
-    e = a->bits == 8 ? cudaLaunchKernelEx(&cfg, k_adamw<true>, chunks, S, H, (const AdNorm*)(clip ? ns : nullptr), gs)
-                     : cudaLaunchKernelEx(&cfg, k_adamw<false>, chunks, S, H, (const AdNorm*)(clip ? ns : nullptr), gs);
+    e = launch_dependent(a->bits == 8 ? k_adamw<true> : k_adamw<false>, (unsigned)a->chunks, kAdThreads, 0, st, chunks, S, H,
+                         (const AdNorm*)(clip ? ns : nullptr), gs);
   if (e != cudaSuccess) {
     set_last_error("osam_adamw_step launch: %s", cudaGetErrorString(e));
     return OSAM_ERR_CUDA;

@@ -11,10 +11,9 @@
 #pragma once
 #include <limits.h>
 
-#include <utility>
-
 #include "conv_internal.h"
 #include "half16.cuh"
+#include "launch.cuh"
 #include "pair_math.cuh"
 #include "sm100.cuh"
 
@@ -412,24 +411,6 @@ __device__ __forceinline__ void at_doc_bits(const AtDocs& own, const AtDocs* s, 
       pad[word] = p;
     }
   }
-}
-
-// Every kernel here is launched with the programmatic-serialization attribute: it may be scheduled while the kernel
-// in front of it drains, sets itself up and then waits for that kernel's end (grid_dep_wait) before its first
-// global access.
-template <typename... P, typename... A>
-cudaError_t launch_dependent(void (*k)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st, A&&... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k, std::forward<A>(args)...);
 }
 
 // ---- host side (attn.cu): one call's launches

@@ -20,6 +20,7 @@
 
 #include "conv_internal.h"
 #include "half16.cuh"
+#include "launch.cuh"
 #include "sm100.cuh"
 
 namespace osam {
@@ -30,7 +31,7 @@ constexpr int kRmsMaxC = 8192;
 constexpr int kRmsGroup = 128;       // channels per e4m3 scale
 constexpr float kE4m3Max = 448.f;
 constexpr int kRmsSms = 148;
-constexpr int kRmsBwdCtas = 4 * kRmsSms;  // at most this many partial dw rows
+constexpr int kRmsBwdCtas = 4 * kRmsSms;  // at most this many partial dw rows (rows above 1024 channels)
 
 struct RmsFwd {
   const void* x;
@@ -80,6 +81,8 @@ template <typename T, int TPR, int NV, bool Q8>
 __global__ void __launch_bounds__(kRmsThreads) k_rms_fwd(const RmsFwd P) {
   __shared__ float red[kRmsThreads / 32];
   constexpr int RPC = kRmsThreads / TPR;  // rows per CTA
+  grid_dep_wait();
+  grid_dep_launch();
   const int t = threadIdx.x % TPR, C8 = P.C / 8;
   float w[NV][8];
 #pragma unroll
@@ -159,11 +162,20 @@ __global__ void __launch_bounds__(kRmsThreads) k_rms_fwd(const RmsFwd P) {
   }
 }
 
+// Rows within a warp: one CTA of 32 warps per SM (16 where a thread holds 32 channels), so that few partial dw rows
+// are left to add; wider rows: as the forward.
+template <int TPR, int NV>
+constexpr int rms_bwd_threads() {
+  return TPR > 32 ? kRmsThreads : NV == 4 ? 512 : 1024;
+}
 template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(kRmsThreads) k_rms_bwd(const RmsBwd P) {
-  __shared__ float red[kRmsThreads / 32];
-  __shared__ float part[TPR <= 32 ? kRmsThreads * 8 : 1];
-  constexpr int RPC = kRmsThreads / TPR;
+__global__ void __launch_bounds__(rms_bwd_threads<TPR, NV>()) k_rms_bwd(const RmsBwd P) {
+  constexpr int THREADS = rms_bwd_threads<TPR, NV>();
+  __shared__ float red[THREADS / 32];
+  __shared__ float part[TPR <= 32 ? THREADS * 8 : 1];
+  constexpr int RPC = THREADS / TPR;
+  grid_dep_wait();
+  grid_dep_launch();
   const int t = threadIdx.x % TPR, C8 = P.C / 8;
   float w[NV][8], dw[NV][8];
 #pragma unroll
@@ -232,7 +244,7 @@ __global__ void __launch_bounds__(kRmsThreads) k_rms_bwd(const RmsBwd P) {
 #pragma unroll
       for (int i = 0; i < 8; i++) part[(threadIdx.x / TPR) * TPR * 8 + t * 8 + i] = dw[k][i];
       __syncthreads();
-      for (int c = threadIdx.x; c < TPR * 8; c += kRmsThreads) {
+      for (int c = threadIdx.x; c < TPR * 8; c += THREADS) {
         float s = 0.f;
 #pragma unroll 8
         for (int g = 0; g < RPC; g++) s += part[g * TPR * 8 + c];
@@ -247,6 +259,7 @@ __global__ void __launch_bounds__(kRmsThreads) k_rms_bwd(const RmsBwd P) {
 __global__ void __launch_bounds__(1024) k_rms_dw(const float* part, int n, int C, float* dw) {
   __shared__ float s[32][33];
   grid_dep_wait();
+  grid_dep_launch();
   const int c = blockIdx.x * 32 + threadIdx.x % 32, l = threadIdx.x / 32;
   float a[4] = {};
   if (c < C)
@@ -297,13 +310,15 @@ void rms_shape(int C, F f) {
 }
 
 template <typename T, bool Q8>
-void launch_rms_fwd(const RmsFwd& P, cudaStream_t st) {
+cudaError_t launch_rms_fwd(const RmsFwd& P, cudaStream_t st) {
+  cudaError_t e = cudaSuccess;
   rms_shape(P.C, [&](auto tpr, auto nv) {
     constexpr int RPC = kRmsThreads / tpr.value;
     const long long need = (P.rows + RPC - 1) / RPC;
     const int grid = (int)std::min<long long>(need, kRmsSms * 8);
-    k_rms_fwd<T, tpr.value, nv.value, Q8><<<grid, kRmsThreads, 0, st>>>(P);
+    e = launch_dependent(k_rms_fwd<T, tpr.value, nv.value, Q8>, grid, kRmsThreads, 0, st, P);
   });
+  return e;
 }
 
 int rms_fwd(int dtype, RmsFwd P, bool q8, cudaStream_t st, const char* name) {
@@ -316,33 +331,25 @@ int rms_fwd(int dtype, RmsFwd P, bool q8, cudaStream_t st, const char* name) {
     return rms_fail(OSAM_ERR_INVALID, "rms: null, misaligned (16 bytes; 8 for e4m3) or overlapping rows");
   P.inv_c = 1.f / P.C;
   P.groups = (P.C + kRmsGroup - 1) / kRmsGroup;
-  if (dtype == OSAM_F16)
-    q8 ? launch_rms_fwd<__half, true>(P, st) : launch_rms_fwd<__half, false>(P, st);
-  else
-    q8 ? launch_rms_fwd<__nv_bfloat16, true>(P, st) : launch_rms_fwd<__nv_bfloat16, false>(P, st);
-  return rms_cuda(cudaGetLastError(), name);
+  const cudaError_t e =
+      dtype == OSAM_F16 ? (q8 ? launch_rms_fwd<__half, true>(P, st) : launch_rms_fwd<__half, false>(P, st))
+                        : (q8 ? launch_rms_fwd<__nv_bfloat16, true>(P, st) : launch_rms_fwd<__nv_bfloat16, false>(P, st));
+  return rms_cuda(e, name);
 }
 
 template <typename T>
 int launch_rms_bwd(const RmsBwd& P, float* dw, cudaStream_t st) {
   int grid = 0;
+  cudaError_t e = cudaSuccess;
   rms_shape(P.C, [&](auto tpr, auto nv) {
-    constexpr int RPC = kRmsThreads / tpr.value;
-    grid = (int)std::min<long long>((P.rows + RPC - 1) / RPC, kRmsBwdCtas);
-    k_rms_bwd<T, tpr.value, nv.value><<<grid, kRmsThreads, 0, st>>>(P);
+    constexpr int threads = rms_bwd_threads<tpr.value, nv.value>(), RPC = threads / tpr.value;
+    const int most = tpr.value > 32 ? kRmsBwdCtas : threads == 512 ? 2 * kRmsSms : kRmsSms;
+    grid = (int)std::min<long long>((P.rows + RPC - 1) / RPC, most);
+    e = launch_dependent(k_rms_bwd<T, tpr.value, nv.value>, grid, threads, 0, st, P);
   });
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return rms_cuda(e, "osam_rms_bwd launch");
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((P.C + 31) / 32);
-  cfg.blockDim = dim3(1024);
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return rms_cuda(cudaLaunchKernelEx(&cfg, k_rms_dw, (const float*)P.part, grid, P.C, dw), "osam_rms_bwd launch");
+  if (e == cudaSuccess)
+    e = launch_dependent(k_rms_dw, (P.C + 31) / 32, 1024, 0, st, (const float*)P.part, grid, P.C, dw);
+  return rms_cuda(e, "osam_rms_bwd launch");
 }
 
 }  // namespace
