@@ -92,16 +92,18 @@ __device__ __forceinline__ float at_min_nan(float a, float b) {
 
 // The first n of 32 bits (n may lie outside 0 … 32).
 __device__ __forceinline__ uint32_t at_low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
-// x where bit i of `vis` is set, `other` elsewhere, over 32 columns.
-__device__ __forceinline__ void at_mask32(float* x, uint32_t vis, float other) {
+// x where bit i of `vis` is set, `other` elsewhere, over N columns.
+template <int N>
+__device__ __forceinline__ void at_mask(float (&x)[N], uint32_t vis, float other) {
 #pragma unroll
-  for (int c = 0; c < 32; c++) x[c] = (vis >> c) & 1 ? x[c] : other;
+  for (int c = 0; c < N; c++) x[c] = (vis >> c) & 1 ? x[c] : other;
 }
-// Which of 32 columns have document `doc`.
-__device__ __forceinline__ uint32_t at_doc_bits32(const int* cols, int doc) {
+// Which of N columns have document `doc`.
+template <int N>
+__device__ __forceinline__ uint32_t at_same_doc(const int* cols, int doc) {
   uint32_t v = 0;
 #pragma unroll
-  for (int c = 0; c < 32; c += 4) {
+  for (int c = 0; c < N; c += 4) {
     const int4 d = *reinterpret_cast<const int4*>(cols + c);
     v |= (uint32_t(d.x == doc) << c) | (uint32_t(d.y == doc) << (c + 1)) | (uint32_t(d.z == doc) << (c + 2)) |
          (uint32_t(d.w == doc) << (c + 3));
@@ -260,6 +262,14 @@ __device__ __forceinline__ void at_ld16(uint32_t taddr, float (&v)[16]) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void at_ld8(uint32_t taddr, float (&v)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void at_ld32(uint32_t taddr, float (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
@@ -297,6 +307,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 

@@ -340,9 +340,9 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
       uint32_t vis = 0xffffffffu;
       if (by_lim || by_doc) {  // hidden: p = 0 and ds = 0 whatever the operands hold
         vis = DKV ? (from == INT_MAX ? 0u : ~at_low_bits(from - c0 - h0)) : at_low_bits(lim - c0 - h0);
-        if (by_doc) vis &= at_doc_bits32(&col_doc[buf][slot][h0], my_doc);
-        at_mask32(sv, vis, CAP ? 0.f : -INFINITY);
-        at_mask32(dp, vis, 0.f);
+        if (by_doc) vis &= at_same_doc<32>(&col_doc[buf][slot][h0], my_doc);
+        at_mask(sv, vis, CAP ? 0.f : -INFINITY);
+        at_mask(dp, vis, 0.f);
       }
       AtLine line;
       if (BIAS == 1) line.start(bias);

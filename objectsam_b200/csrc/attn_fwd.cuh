@@ -10,6 +10,11 @@
 // then the row's two threads agree on it and O, which stays in TMEM, is rescaled; otherwise one flag barrier of the
 // two warps tells that nothing is to do.  Tiles are visited from the CTA's own positions outwards, so that with a
 // distance bias the largest scores come first and this stays rare.
+// Up to 32 rows (single tokens): a warp's instructions cost the same for one row as for 32, and all rows would lie in the
+// lanes of two warps, on one of the SM's four schedulers.  So the rows are repeated in the four 32-lane groups, and
+// group g takes columns 8g … 8g+7 of each half alone, with a maximum and a sum of its own; P of the other columns stays
+// zero, and the groups' outputs are joined in shared memory at the end (16 sequences over caches of 8192–32768 keys: 282
+// us without this, 250 with it).
 // Warps 0–7: softmax (warps w and w + 4 share rows), warp 8: TMA producer, warp 9: TMEM owner and MMA issuer.  The
 // softmax is a chain of latencies (barriers, TMEM loads, the exponentials' unit) that four warps a scheduler hide:
 // two CTAs per SM, 256 TMEM columns each: S, which the next tile's Q·Kᵀ overwrites as soon as it is in registers,
@@ -33,11 +38,11 @@ struct AfCfg {
   static constexpr int SMEM = 1024 + QTILE + 2 * STAGES * TILE;
 };
 
-template <typename T, int DP, bool CAP, int BIAS>
+template <typename T, int DP, bool CAP, int BIAS, bool SPREAD>
 __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constant__ AttnFwdLaunch P) {
   using Cfg = AfCfg<DP>;
   constexpr bool BF16 = Half16<T>::kBf16;
-  constexpr int KEYS = kAfKeys;
+  constexpr int KEYS = kAfKeys, N = SPREAD ? 8 : 32;  // N: columns of a thread
   extern __shared__ uint8_t af_raw[];
   __shared__ __align__(8) uint64_t k_full[Cfg::STAGES], k_empty[Cfg::STAGES], v_full[Cfg::STAGES], v_empty[Cfg::STAGES];
   __shared__ __align__(8) uint64_t s_full, s_free, p_full[2], pv_done, o_done;
@@ -75,7 +80,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   tiles.live = docs ? live : nullptr;
 
   // ---- this thread's row
-  const int r = r0 + tid % kAfRows;
+  const int r = r0 + (SPREAD ? lane : tid % kAfRows);
   const bool valid = warp < 8 && r < rows;
   const int qi = valid ? A.f_g.quo(r) : 0, head = hk * A.G + (valid ? r - qi * A.G : 0);
   int my_doc = -2;
@@ -125,7 +130,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     const T* q = static_cast<const T*>(P.q.p) + b * P.q.sb;
 #pragma unroll 8
     for (int c = tid; c < kAfRows * CH; c += kAfSoft) {
-      const int row = c / CH, ch = c % CH, rr = r0 + row;
+      const int row = c / CH, ch = c % CH, rr = r0 + (SPREAD ? row % 32 : row);
       uint4 u = make_uint4(0, 0, 0, 0);
       if (rr < rows && ch * 8 < A.D) {
         const int i = A.f_g.quo(rr), h = hk * A.G + rr - i * A.G;
@@ -228,7 +233,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   } else {
     const int half = warp / 4, row_of = tid % kAfRows, h0 = half * 32, pair_bar = 2 + warp % 4;
     const uint32_t lane_base = uint32_t((warp % 4) * 32) << 16;
-    const bool idle = r0 + (warp % 4) * 32 >= rows;  // no row of this warp exists: it only keeps step
+    const bool idle = !SPREAD && r0 + (warp % 4) * 32 >= rows;  // no row of this warp exists: it only keeps step
     const int pos = off + qi;
     const int lim = valid ? at_limit(A, n, prefix, pos) : 0;
     // without cap and bias the scale is applied with the exponent's FMA: x·cmul are scores in log2 units
@@ -247,7 +252,13 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     float neg = 0.f;      // −m, or 0 while there is none
     float l = 0.f;        // this thread's part of its sum
     const uint32_t bar_s = smem_u32(&s_full), bar_free = smem_u32(&s_free), bar_p = smem_u32(&p_full[0]);
-    const uint32_t s_addr = tmem + lane_base + Cfg::COL_S + h0, p_addr = tmem + lane_base + Cfg::COL_P + h0 / 2;
+    const int c1 = h0 + (SPREAD ? 8 * (warp % 4) : 0);  // first column of this thread
+    const uint32_t s_addr = tmem + lane_base + Cfg::COL_S + c1, p_addr = tmem + lane_base + Cfg::COL_P + c1 / 2;
+    if (SPREAD) {  // what a group never writes of P
+      const uint32_t zero[16] = {};
+      tmem_st16(tmem + lane_base + Cfg::COL_P + h0 / 2, zero);
+      tmem_st16(tmem + lane_base + Cfg::COL_P + 32 + h0 / 2, zero);
+    }
     const int tail = n < A.Lk ? n : INT_MAX;  // keys from here on hold anything
     bool ok = true;
     int it = 0;
@@ -277,8 +288,11 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       ok = at_wait(bar_s, it & 1, A.err);
       tc_fence_after();
       float top = -INFINITY;
-      float x[32];
-      at_ld32(s_addr, x);
+      float x[N];
+      if constexpr (!SPREAD)
+        at_ld32(s_addr, x);
+      else
+        at_ld8(s_addr, x);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) at_arrive(bar_free);
@@ -286,24 +300,24 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       if (!idle) {
         uint32_t vis = 0xffffffffu;
         if (masked) {
-          vis = at_low_bits(lim - j0 - h0);
-          if (by_doc) vis &= at_doc_bits32(&col_doc[it & 1][h0], my_doc);
-          if (CAP) at_mask32(x, vis, 0.f);
+          vis = at_low_bits(lim - j0 - c1);
+          if (by_doc) vis &= at_same_doc<N>(&col_doc[it & 1][c1], my_doc);
+          if (CAP) at_mask(x, vis, 0.f);
         }
         if (CAP || BIAS) {
           AtLine line;
           if (BIAS == 1) {
-            bias.y = float(pos - j0 - h0) * bias.slope;
+            bias.y = float(pos - j0 - c1) * bias.slope;
             line.start(bias);
           }
           const float2 none[2] = {};
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
+          for (int c = 0; c < N; c += 4) {
             float2 s2[2] = {make_float2(x[c], x[c + 1]), make_float2(x[c + 2], x[c + 3])}, sig[2];
             float4 ky = {}, kx = {};
             if (BIAS == 2) {
-              ky = *reinterpret_cast<const float4*>(&col_y[it & 1][h0 + c]);
-              kx = *reinterpret_cast<const float4*>(&col_x[it & 1][h0 + c]);
+              ky = *reinterpret_cast<const float4*>(&col_y[it & 1][c1 + c]);
+              kx = *reinterpret_cast<const float4*>(&col_x[it & 1][c1 + c]);
             }
             at_scores4<CAP, BIAS, false>(bias, s2, none, line, ky, kx, sig);
             x[c] = s2[0].x;
@@ -312,15 +326,15 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
             x[c + 3] = s2[1].y;
           }
         }
-        if (masked) at_mask32(x, vis, -INFINITY);
-        float top1 = x[1];
-        top = x[0];
+        if (masked) at_mask(x, vis, -INFINITY);
+        float top1 = fmaxf(x[2], x[3]);
+        top = fmaxf(x[0], x[1]);
 #pragma unroll
-        for (int c = 2; c + 3 < 32; c += 4) {
+        for (int c = 4; c < N; c += 4) {
           top = fmaxf(fmaxf(top, x[c]), x[c + 1]);
           top1 = fmaxf(fmaxf(top1, x[c + 2]), x[c + 3]);
         }
-        top = fmaxf(fmaxf(top, top1), fmaxf(x[30], x[31])) * cmul;
+        top = fmaxf(top, top1) * cmul;
       }
       if (at_pair_any(pair_bar, top > m + kAfGrow || !ok)) {  // also the first score that a row sees: −∞ + 8 = −∞
         ok = !at_pair_any(pair_bar, !ok);
@@ -349,9 +363,9 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       if (!idle) {
         const float2 mul = make_float2(cmul, cmul), add = make_float2(neg, neg);
         float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
-        uint32_t p[16];
+        uint32_t p[N / 2];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
+        for (int i = 0; i < N / 2; i++) {
           float2 e = make_float2(x[2 * i], x[2 * i + 1]);
           e = CAP || BIAS ? add2(e, add) : fma2(e, mul, add);
           e.x = at_ex2(e.x);
@@ -360,7 +374,10 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
           p[i] = Half16<T>::pack(e.x, e.y);
         }
         // this buffer of P is free: S tells that the P·V before last is done
-        tmem_st16(p_addr + (it & 1) * 32, p);
+        if constexpr (!SPREAD)
+          tmem_st16(p_addr + (it & 1) * 32, p);
+        else
+          tmem_st4(p_addr + (it & 1) * 32, p);
         const float2 s = add2(sum[0], sum[1]);
         l = s.x + s.y;
       }
@@ -387,8 +404,42 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       l += pair_sum[half ^ 1][row_of];
       const long long row = ((long long)b * A.Hq + head) * A.Lq + qi;
       const long long part_row = (long long)split * A.B * A.Hq * A.Lq + row;
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays one
       T* o_ptr = static_cast<T*>(P.o.p) + b * P.o.sb + qi * P.o.st + head * P.o.sh;
+      // eight dims of the row against m, l: to o, or for a split as they are
+      auto put = [&](int c, const float (&v)[8], float inv) {
+        if (P.splits == 1) {
+          float w[8];
+#pragma unroll
+          for (int k = 0; k < 8; k++) w[k] = v[k] * inv;
+          *reinterpret_cast<uint4*>(o_ptr + c) = pack8<T>(w);
+        } else {
+          float4* d = reinterpret_cast<float4*>(P.part + part_row * A.D + c);
+          d[0] = make_float4(v[0], v[1], v[2], v[3]);
+          d[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
+      };
+      float w4[4] = {1.f, 0.f, 0.f, 0.f};  // the groups' weights
+      float* joined = reinterpret_cast<float*>(smem);  // [group][row][DP + 4]: the operands' room is free by now
+      const int g = warp % 4;
+      if (SPREAD) {
+        if (half == 0) {
+          pair_top[0][row_of] = m;
+          pair_top[1][row_of] = l;
+        }
+        named_bar_sync(1, kAfSoft);
+        float M = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 4; k++) M = fmaxf(M, pair_top[0][k * 32 + lane]);
+        l = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const float mk = pair_top[0][k * 32 + lane];
+          w4[k] = mk == -INFINITY ? 0.f : at_ex2(mk - M);
+          l = fmaf(w4[k], pair_top[1][k * 32 + lane], l);
+        }
+        m = M;
+      }
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays one
 #pragma unroll
       for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 16) {
         if (c >= A.D) break;
@@ -397,24 +448,41 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
 #pragma unroll
         for (int i = 0; i < 16; i++) o[i] = it > 0 && l != 0.f ? o[i] : 0.f;
         if (!valid) continue;
+        const float lo[8] = {o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7]};
+        const float hi[8] = {o[8], o[9], o[10], o[11], o[12], o[13], o[14], o[15]};
+        if (SPREAD) {
+          float4* d = reinterpret_cast<float4*>(joined + (g * 32 + lane) * (DP + 4) + c);
+          d[0] = make_float4(lo[0], lo[1], lo[2], lo[3]);
+          d[1] = make_float4(lo[4], lo[5], lo[6], lo[7]);
+          d[2] = make_float4(hi[0], hi[1], hi[2], hi[3]);
+          d[3] = make_float4(hi[4], hi[5], hi[6], hi[7]);
+          continue;
+        }
+        put(c, lo, inv);
+        if (c + 8 < A.D) put(c + 8, hi, inv);
+      }
+      if (SPREAD) {  // group g joins every fourth of the row's 8-dim pieces of its half
+        named_bar_sync(1, kAfSoft);
+        for (int c = half * (DP / 2) + g * 8; valid && c < (half + 1) * (DP / 2) && c < A.D; c += 32) {
+          float v[8] = {};
 #pragma unroll
-        for (int i = 0; i < 16; i += 8) {
-          if (c + i >= A.D) break;
-          float v8[8];
-#pragma unroll
-          for (int k = 0; k < 8; k++) v8[k] = o[i + k];
-          if (P.splits == 1) {
-#pragma unroll
-            for (int k = 0; k < 8; k++) v8[k] *= inv;
-            *reinterpret_cast<uint4*>(o_ptr + c + i) = pack8<T>(v8);
-          } else {
-            float4* d = reinterpret_cast<float4*>(P.part + part_row * A.D + c + i);
-            d[0] = make_float4(v8[0], v8[1], v8[2], v8[3]);
-            d[1] = make_float4(v8[4], v8[5], v8[6], v8[7]);
+          for (int k = 0; k < 4; k++) {
+            const float4* d = reinterpret_cast<const float4*>(joined + (k * 32 + lane) * (DP + 4) + c);
+            const float4 a = d[0], e = d[1];
+            if (w4[k] == 0.f) continue;  // a group that saw nothing
+            v[0] = fmaf(w4[k], a.x, v[0]);
+            v[1] = fmaf(w4[k], a.y, v[1]);
+            v[2] = fmaf(w4[k], a.z, v[2]);
+            v[3] = fmaf(w4[k], a.w, v[3]);
+            v[4] = fmaf(w4[k], e.x, v[4]);
+            v[5] = fmaf(w4[k], e.y, v[5]);
+            v[6] = fmaf(w4[k], e.z, v[6]);
+            v[7] = fmaf(w4[k], e.w, v[7]);
           }
+          put(c, v, inv);
         }
       }
-      if (valid && half == 0) {
+      if (valid && half == 0 && (!SPREAD || g == 0)) {
         if (P.splits > 1)
           P.stats[part_row] = make_float2(m, l);
         else if (P.lse)
@@ -430,13 +498,13 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   }
 }
 
-template <typename T, int DP, bool CAP, int BIAS>
+template <typename T, int DP, bool CAP, int BIAS, bool SPREAD>
 cudaError_t attn_fwd_one(const AttnFwdLaunch& L, int grid, cudaStream_t st) {
   static bool set[64] = {};  // per device; a race only repeats the call
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  auto* k = k_attn_fwd<T, DP, CAP, BIAS>;
+  auto* k = k_attn_fwd<T, DP, CAP, BIAS, SPREAD>;
   if (dev >= 64 || !set[dev]) {
     e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, AfCfg<DP>::SMEM);
     if (e != cudaSuccess) return e;
@@ -445,23 +513,25 @@ cudaError_t attn_fwd_one(const AttnFwdLaunch& L, int grid, cudaStream_t st) {
   return launch_dependent(k, grid, kAfThreads, AfCfg<DP>::SMEM, st, L);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool SPREAD>
 cudaError_t attn_fwd_dp(const AttnFwdLaunch& L, int grid, cudaStream_t st) {
   const int bias = !L.d.slopes ? 0 : L.d.grid_w > 0 ? 2 : 1;
   if (L.d.cap > 0.f)
-    return bias == 0   ? attn_fwd_one<T, DP, true, 0>(L, grid, st)
-           : bias == 1 ? attn_fwd_one<T, DP, true, 1>(L, grid, st)
-                       : attn_fwd_one<T, DP, true, 2>(L, grid, st);
-  return bias == 0   ? attn_fwd_one<T, DP, false, 0>(L, grid, st)
-         : bias == 1 ? attn_fwd_one<T, DP, false, 1>(L, grid, st)
-                     : attn_fwd_one<T, DP, false, 2>(L, grid, st);
+    return bias == 0   ? attn_fwd_one<T, DP, true, 0, SPREAD>(L, grid, st)
+           : bias == 1 ? attn_fwd_one<T, DP, true, 1, SPREAD>(L, grid, st)
+                       : attn_fwd_one<T, DP, true, 2, SPREAD>(L, grid, st);
+  return bias == 0   ? attn_fwd_one<T, DP, false, 0, SPREAD>(L, grid, st)
+         : bias == 1 ? attn_fwd_one<T, DP, false, 1, SPREAD>(L, grid, st)
+                     : attn_fwd_one<T, DP, false, 2, SPREAD>(L, grid, st);
 }
 
 template <typename T>
 cudaError_t launch_attn_fwd(const AttnFwdLaunch& L, cudaStream_t st) {
   const int nq = (L.d.Lq * L.d.G + kAfRows - 1) / kAfRows;
   const int grid = nq * L.d.B * L.d.Hk * L.splits;
-  return L.d.D <= 64 ? attn_fwd_dp<T, 64>(L, grid, st) : attn_fwd_dp<T, 128>(L, grid, st);
+  if (L.d.Lq * L.d.G <= 32)  // one row a lane of a 32-lane group
+    return L.d.D <= 64 ? attn_fwd_dp<T, 64, true>(L, grid, st) : attn_fwd_dp<T, 128, true>(L, grid, st);
+  return L.d.D <= 64 ? attn_fwd_dp<T, 64, false>(L, grid, st) : attn_fwd_dp<T, 128, false>(L, grid, st);
 }
 
 }  // namespace osam
