@@ -48,15 +48,18 @@ __global__ void __launch_bounds__(256) k_attn_docs(const int* doc_q, const int* 
 // every W-th split each, four loads in flight; their sums are added in warp order.  (One warp a row took as long for
 // 64 splits as the attention in front of it.)
 template <typename T>
-__global__ void __launch_bounds__(256) k_attn_join(const float* part, const float2* stats, int splits, int W, long long nrows,
-                                                   int Hq, int Lq, int D, AtView o, float* lse) {
+__global__ void __launch_bounds__(256) k_attn_join(const float* part, const float2* stats, const __grid_constant__ AttnDev A,
+                                                   const int* chunk, int W, long long nrows, AtView o, float* lse) {
   __shared__ float4 acc_of[8][32];
   __shared__ float l_of[8];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, w = warp % W;
   const long long row = (long long)blockIdx.x * (8 / W) + warp / W;
   const bool live = row < nrows;
+  const int D = A.D;
+  const long long bh = row / A.Lq, b = bh / A.Hq;
   grid_dep_wait();
   grid_dep_launch();
+  const int splits = live ? at_seq_splits(A, int(b), *chunk) : 0;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f, M = -INFINITY;
   if (live) {
@@ -100,9 +103,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const float* part, const floa
     }
   }
   if (!live) return;
-  const long long bh = row / Lq;
-  const int i = int(row - bh * Lq), h = int(bh % Hq);
-  const long long b = bh / Hq;
+  const int i = int(row - bh * A.Lq), h = int(bh % A.Hq);
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   if (lane * 4 < D) {
     T* p = static_cast<T*>(o.p) + b * o.sb + i * o.st + h * o.sh + lane * 4;
@@ -242,28 +243,34 @@ int at_map(CUtensorMap* tm, const osam_view& v, int batch, int len, int heads, i
   return make_map(tm, v.p, 4, dims, st, box, 128, bf16);
 }
 
-// How the keys are split.  Nothing is gained once the query tiles fill the GPU; below, up to four CTAs an SM (uneven
-// caches balance; 16 sequences over caches of 8192–32768 keys: 282 us, with two an SM 289, with eight 291) of at
-// least 256 keys, 512 over long caches (one sequence, 4 heads, 32768 keys: 19 us, with 256 keys 26).  The join costs a
-// launch: a cache of 517 keys takes 11 us whole and 15 in two, one of 860 keys 21 and 15.
+// How the keys are split.  Nothing is gained once the query tiles fill the GPU's places; below, the kernel takes the
+// splits' size from the sequences' lengths (at_best_chunk) and only their bounds are set here: 256 keys at least, 512 over
+// long caches (one sequence, 4 heads, 32768 keys: 16 us, with 256 keys 21), and the CTAs that fill kAfRounds rounds.
+// The join costs a launch: a cache of 517 keys takes 11 us whole and 15 in two, one of 860 keys 21 and 15.
 struct AtSplit {
-  int splits, tiles;
+  int splits, min_tiles, grid, usual;  // at most, …, CTAs, splits of a sequence with all CTAs in use
+  int chunk;  // where every sequence has len_k keys
 };
 AtSplit at_split(const osam_attn_desc& a) {
   const int tiles = (a.len_k + kAfKeys - 1) / kAfKeys;
-  const long long ctas = (((long long)a.len_q * (a.heads_q / a.heads_k) + 127) / 128) * a.batch * a.heads_k;
-  AtSplit s{1, std::max(tiles, 1)};
-  if (ctas == 0 || a.len_k < 768 || ctas >= 2 * kAtSms) return s;
-  const int want = (int)std::min<long long>((4LL * kAtSms + ctas - 1) / ctas, a.len_k / (a.len_k <= 2048 ? 256 : 512));
-  s.tiles = (tiles + want - 1) / want;
-  s.splits = (tiles + s.tiles - 1) / s.tiles;
+  const long long per = ((long long)a.len_q * (a.heads_q / a.heads_k) + kAfRows - 1) / kAfRows * a.heads_k;
+  const long long ctas = per * a.batch;
+  AtSplit s{1, std::max(tiles, 1), (int)ctas, 1, tiles};
+  if (ctas == 0 || a.len_k < 768 || ctas >= kAfPlaces) return s;
+  s.min_tiles = a.len_k <= 2048 ? 4 : 8;
+  const int most = (tiles + s.min_tiles - 1) / s.min_tiles;
+  s.splits = std::min(most, (int)(kAfRounds * kAfPlaces / per) - (a.batch - 1));
+  s.grid = (int)std::min<long long>(kAfRounds * kAfPlaces / per * per, ctas * most);
+  s.usual = s.grid / (int)ctas;
+  s.chunk = at_best_chunk(a.batch, (int)per, s.min_tiles, tiles, a.batch * tiles,
+                          [&](int chunk) { return a.batch * ((tiles + chunk - 1) / chunk); });
   return s;
 }
 
 // Into how many parts the backward splits the streamed side of a tile: by a model of its time in units of a streamed
 // tile (0.7 us measured): rounds of CTAs over the GPU × (tiles of a part + 5 for a CTA's start and end), and for the
 // parts' sum 8 and its traffic.  One part where the tiles fill the GPU (16 heads of 4096 tokens); with 2 key heads of
-// 8192 tokens (128 tiles for 296 places) two parts took dK and dV from 634 to 350 us.
+// 8192 tokens (128 tiles for 296 places) two parts took the whole backward from 907 to 675 us.
 int at_parts(const osam_attn_desc& a, bool dkv) {
   const int slots = kAtSms * (a.dim <= 64 ? 2 : 1), own = dkv ? a.len_k : a.len_q, other = dkv ? a.len_q : a.len_k;
   const int heads = dkv ? a.heads_k : a.heads_q;
@@ -286,7 +293,7 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Workspace: document summaries | split outputs and statistics (forward) or row terms (backward).
 struct AtLayout {
-  size_t sum_q = 0, sum_k = 0, part = 0, stats = 0, rows = 0, peak = 0, grad = 0, bytes = 0;
+  size_t sum_q = 0, sum_k = 0, part = 0, stats = 0, chunk = 0, rows = 0, peak = 0, grad = 0, bytes = 0;
 };
 AtLayout at_layout(const osam_attn_desc& a) {
   AtLayout L;
@@ -305,6 +312,8 @@ AtLayout at_layout(const osam_attn_desc& a) {
     fwd += up256(rows * s.splits * a.dim * sizeof(float));
     L.stats = fwd;
     fwd += up256(rows * s.splits * sizeof(float2));
+    L.chunk = fwd;
+    fwd += 256;
   }
   const size_t blocks = (size_t)a.batch * a.heads_q * ((a.len_q + kAbCols - 1) / kAbCols);
   L.peak = at + up256(blocks * 2 * kAbCols * sizeof(float));
@@ -378,16 +387,19 @@ int osam_attn_fwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   L.o = at_view(o);
   L.lse = lse;
   L.splits = s.splits;
-  L.tiles_per_split = s.tiles;
+  L.min_tiles = s.min_tiles;
+  L.grid = s.grid;
+  L.chunk_all = s.chunk;
+  L.chunk = reinterpret_cast<int*>(w + W.chunk);
   L.part = reinterpret_cast<float*>(w + W.part);
   L.stats = reinterpret_cast<float2*>(w + W.stats);
   cudaError_t e = bf16 ? launch_attn_fwd<__nv_bfloat16>(L, st) : launch_attn_fwd<__half>(L, st);
   if (e != cudaSuccess || s.splits == 1) return at_cuda(e, "forward launch");
   const long long nrows = (long long)a->batch * a->heads_q * a->len_q;
-  const int warps = s.splits <= 4 ? 1 : s.splits <= 16 ? 4 : 8;
+  const int warps = s.usual <= 4 ? 1 : s.usual <= 16 ? 4 : 8;
   const unsigned grid = (unsigned)((nrows + 8 / warps - 1) / (8 / warps));
   e = launch_dependent(bf16 ? k_attn_join<__nv_bfloat16> : k_attn_join<__half>, grid, 256, 0, st, (const float*)L.part,
-                       (const float2*)L.stats, s.splits, warps, nrows, a->heads_q, a->len_q, a->dim, L.o, lse);
+                       (const float2*)L.stats, L.d, (const int*)L.chunk, warps, nrows, L.o, lse);
   return at_cuda(e, "join launch");
 }
 

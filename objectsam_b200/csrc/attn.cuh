@@ -23,6 +23,8 @@ constexpr float kAtLog2e = 1.4426950408889634f, kAtLn2 = 0.6931471805599453f;
 constexpr int kAtDocBlock = 64;      // tokens per document summary
 constexpr int kAtDocWords = 512;     // 32-bit words of a CTA's key-tile bitmaps: 16384 tiles of 64 keys
 constexpr int kAtSms = 148;
+constexpr int kAfRows = 128, kAfKeys = 64;  // a forward CTA's query rows, and the keys of a tile
+constexpr int kAfPlaces = 2 * kAtSms, kAfRounds = 2;  // forward CTAs at a time, and rounds of them that splits may fill
 
 // A [batch][token][head][dim] tensor: element strides, dim contiguous.
 struct AtView {
@@ -55,6 +57,38 @@ struct AttnDev {
 // Keys in use of sequence b.
 __device__ __forceinline__ int at_keys(const AttnDev& A, int b) {
   return A.lens ? max(0, min(A.lens[b], A.Lk)) : A.Lk;
+}
+// Key tiles of a sequence, and its splits of up to `chunk` tiles (one at least: it writes the output's zeros).
+__device__ __forceinline__ int at_seq_tiles(const AttnDev& A, int b) { return (at_keys(A, b) + kAfKeys - 1) / kAfKeys; }
+__device__ __forceinline__ int at_seq_splits(const AttnDev& A, int b, int chunk) {
+  return max(1, (at_seq_tiles(A, b) + chunk - 1) / chunk);
+}
+// Tiles of a split at most, `count(chunk)` being the splits of all B sequences: the smallest chunk with which they fit
+// one or two rounds of the GPU's places, `per` CTAs each, whichever takes less (a CTA's start and end cost about five
+// tiles).  So sequences of any lengths take their share of the CTAs (16 caches of 8192–32768 keys: 233 us, with one
+// number of splits for all 255; 16 caches of 8192 keys: 88 and 108).
+template <typename Count>
+__host__ __device__ __forceinline__ int at_best_chunk(int B, int per, int min_tiles, int max_tiles, int total, Count count) {
+  int best = 0, least = INT_MAX;
+  for (int k = 1; k <= kAfRounds; k++) {
+    const int room = k * kAfPlaces / per;  // at least B
+    int lo = (total + room - 1) / room;    // nothing smaller can fit; rounding up adds less than a split a sequence
+    lo = lo > min_tiles ? lo : min_tiles;
+    int hi = room > B ? (total + room - B - 1) / (room - B) : max_tiles;
+    if (hi < lo || count(lo) <= room) hi = lo;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (count(mid) <= room)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    if (k * (lo + 5) < least) {
+      least = k * (lo + 5);
+      best = lo;
+    }
+  }
+  return best;
 }
 // lim_i of the query at position pos.
 __device__ __forceinline__ int at_limit(const AttnDev& A, int n, int prefix, int pos) {
@@ -429,13 +463,16 @@ __device__ __forceinline__ void at_doc_bits(const AtDocs& own, const AtDocs* s, 
 }
 
 // ---- host side (attn.cu): one call's launches
-constexpr int kAfRows = 128, kAfKeys = 64;  // a forward CTA's query rows, and the keys of a tile
 struct AttnFwdLaunch {
   AttnDev d;
   CUtensorMap tk, tv;
   AtView q, o;
   float* lse;
-  int splits, tiles_per_split;
+  int grid;
+  int splits;     // of a sequence's keys at most; 1: not split
+  int min_tiles;  // of a split at least
+  int chunk_all;  // tiles of a split where all sequences have len_k keys, and for the join what the kernel took
+  int* chunk;
   float* part;    // [split][B][Hq][Lq][D] unnormalised outputs
   float2* stats;  // [split][B][Hq][Lq] (reference maximum in log2 units, sum)
 };

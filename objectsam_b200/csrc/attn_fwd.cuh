@@ -38,6 +38,54 @@ struct AfCfg {
   static constexpr int SMEM = 1024 + QTILE + 2 * STAGES * TILE;
 };
 
+// The chunk (at_best_chunk) for the lengths that `lens` has.
+__device__ __forceinline__ int at_chunk(const AttnDev& A, int per, int min_tiles, int lane) {
+  int total = 0;
+  for (int b = lane; b < A.B; b += 32) total += at_seq_tiles(A, b);
+  total = __reduce_add_sync(0xffffffffu, total);
+  return at_best_chunk(A.B, per, min_tiles, (A.Lk + kAfKeys - 1) / kAfKeys, total, [&](int chunk) {
+    int n = 0;
+    const float inv = 1.f / float(chunk);
+    for (int b = lane; b < A.B; b += 32) {
+      const int t = at_seq_tiles(A, b) + chunk - 1;
+      int s = int(float(t) * inv);  // within one of t / chunk
+      s += (s + 1) * chunk <= t;
+      s -= s * chunk > t;
+      n += max(1, s);
+    }
+    return __reduce_add_sync(0xffffffffu, n);
+  });
+}
+// What CTA `cta` of a split call works on: sequence, number of its splits (0: more CTAs than these lengths need), index
+// among the sequence's CTAs.
+struct AtSplitCta {
+  int seq, splits, i, chunk;
+};
+static __device__ __noinline__ AtSplitCta at_split_cta(const AttnFwdLaunch& P, int per, int lane, int cta) {
+  const AttnDev& A = P.d;
+  AtSplitCta r{0, 0, 0, A.lens ? at_chunk(A, per, P.min_tiles, lane) : P.chunk_all};
+  int base = 0;
+  for (int b0 = 0; b0 < A.B; b0 += 32) {
+    const int s = b0 + lane < A.B ? at_seq_splits(A, b0 + lane, r.chunk) : 0;
+    int end = s * per;
+#pragma unroll
+    for (int k = 1; k < 32; k *= 2) {
+      const int left = __shfl_up_sync(0xffffffffu, end, k);
+      if (lane >= k) end += left;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, cta < base + end);
+    if (past) {
+      const int f = __ffs(past) - 1;
+      r.seq = b0 + f;
+      r.splits = __shfl_sync(0xffffffffu, s, f);
+      r.i = cta - base - __shfl_sync(0xffffffffu, end, f) + r.splits * per;
+      break;
+    }
+    base += __shfl_sync(0xffffffffu, end, 31);
+  }
+  return r;
+}
+
 template <typename T, int DP, bool CAP, int BIAS, bool SPREAD>
 __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constant__ AttnFwdLaunch P) {
   using Cfg = AfCfg<DP>;
@@ -60,21 +108,32 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   uint8_t* smem = af_raw + ((1024 - (smem_u32(af_raw) & 1023)) & 1023);
   const uint32_t sq = smem_u32(smem), sk = sq + Cfg::QTILE, sv = sk + Cfg::STAGES * Cfg::TILE;
 
-  // ---- which tile: with a causal bound the longest rows first
+  // ---- which tile: with a causal bound the longest rows first; or which split
   const int rows = A.Lq * A.G, nq = (rows + kAfRows - 1) / kAfRows;
-  const int per_q = A.B * A.Hk * P.splits;
-  const int qt = A.mask == OSAM_ATTN_NONE ? int(blockIdx.x) % nq : nq - 1 - int(blockIdx.x) / per_q;
-  int rest = A.mask == OSAM_ATTN_NONE ? int(blockIdx.x) / nq : int(blockIdx.x) % per_q;
-  const int split = rest % P.splits;
-  rest /= P.splits;
+  int qt, rest, split = 0, splits = 1, first_tile = 0, own_tiles = 1 << 26;
+  if (P.splits == 1) {
+    const int per_q = A.B * A.Hk;
+    qt = A.mask == OSAM_ATTN_NONE ? int(blockIdx.x) % nq : nq - 1 - int(blockIdx.x) / per_q;
+    rest = A.mask == OSAM_ATTN_NONE ? int(blockIdx.x) / nq : int(blockIdx.x) % per_q;
+  } else {
+    const AtSplitCta c = at_split_cta(P, nq * A.Hk, lane, blockIdx.x);
+    if (blockIdx.x == 0 && tid == 0) *P.chunk = c.chunk;  // for the join
+    if (c.splits == 0) return;
+    split = c.i % c.splits;
+    qt = c.i / c.splits / A.Hk;
+    rest = c.seq * A.Hk + c.i / c.splits % A.Hk;
+    splits = c.splits;
+    own_tiles = (at_seq_tiles(A, c.seq) + splits - 1) / splits;
+    first_tile = split * own_tiles;
+  }
   const int hk = rest % A.Hk, b = rest / A.Hk;
   const int r0 = qt * kAfRows, r_last = min(r0 + kAfRows, rows) - 1;
   const int n = at_keys(A, b), off = n - A.Lq;
   const int prefix = A.mask == OSAM_ATTN_PREFIX ? A.prefix[b] : 0;
   const int lim_max = at_limit(A, n, prefix, off + A.f_g.quo(r_last)), lim_min = at_limit(A, n, prefix, off + A.f_g.quo(r0));
   AtTiles tiles;
-  tiles.begin = split * P.tiles_per_split;
-  tiles.end = max(tiles.begin, min((lim_max + KEYS - 1) / KEYS, tiles.begin + P.tiles_per_split));
+  tiles.begin = first_tile;
+  tiles.end = max(tiles.begin, min((lim_max + KEYS - 1) / KEYS, tiles.begin + own_tiles));
   tiles.from = min(max((off + A.f_g.quo(r_last)) / KEYS, tiles.begin), tiles.end - 1);
   const bool docs = A.doc_q != nullptr;
   tiles.live = docs ? live : nullptr;
@@ -499,7 +558,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
 }
 
 template <typename T, int DP, bool CAP, int BIAS, bool SPREAD>
-cudaError_t attn_fwd_one(const AttnFwdLaunch& L, int grid, cudaStream_t st) {
+cudaError_t attn_fwd_one(const AttnFwdLaunch& L, cudaStream_t st) {
   static bool set[64] = {};  // per device; a race only repeats the call
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -510,28 +569,26 @@ cudaError_t attn_fwd_one(const AttnFwdLaunch& L, int grid, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     if (dev < 64) set[dev] = true;
   }
-  return launch_dependent(k, grid, kAfThreads, AfCfg<DP>::SMEM, st, L);
+  return launch_dependent(k, L.grid, kAfThreads, AfCfg<DP>::SMEM, st, L);
 }
 
 template <typename T, int DP, bool SPREAD>
-cudaError_t attn_fwd_dp(const AttnFwdLaunch& L, int grid, cudaStream_t st) {
+cudaError_t attn_fwd_dp(const AttnFwdLaunch& L, cudaStream_t st) {
   const int bias = !L.d.slopes ? 0 : L.d.grid_w > 0 ? 2 : 1;
   if (L.d.cap > 0.f)
-    return bias == 0   ? attn_fwd_one<T, DP, true, 0, SPREAD>(L, grid, st)
-           : bias == 1 ? attn_fwd_one<T, DP, true, 1, SPREAD>(L, grid, st)
-                       : attn_fwd_one<T, DP, true, 2, SPREAD>(L, grid, st);
-  return bias == 0   ? attn_fwd_one<T, DP, false, 0, SPREAD>(L, grid, st)
-         : bias == 1 ? attn_fwd_one<T, DP, false, 1, SPREAD>(L, grid, st)
-                     : attn_fwd_one<T, DP, false, 2, SPREAD>(L, grid, st);
+    return bias == 0   ? attn_fwd_one<T, DP, true, 0, SPREAD>(L, st)
+           : bias == 1 ? attn_fwd_one<T, DP, true, 1, SPREAD>(L, st)
+                       : attn_fwd_one<T, DP, true, 2, SPREAD>(L, st);
+  return bias == 0   ? attn_fwd_one<T, DP, false, 0, SPREAD>(L, st)
+         : bias == 1 ? attn_fwd_one<T, DP, false, 1, SPREAD>(L, st)
+                     : attn_fwd_one<T, DP, false, 2, SPREAD>(L, st);
 }
 
 template <typename T>
 cudaError_t launch_attn_fwd(const AttnFwdLaunch& L, cudaStream_t st) {
-  const int nq = (L.d.Lq * L.d.G + kAfRows - 1) / kAfRows;
-  const int grid = nq * L.d.B * L.d.Hk * L.splits;
   if (L.d.Lq * L.d.G <= 32)  // one row a lane of a 32-lane group
-    return L.d.D <= 64 ? attn_fwd_dp<T, 64, true>(L, grid, st) : attn_fwd_dp<T, 128, true>(L, grid, st);
-  return L.d.D <= 64 ? attn_fwd_dp<T, 64, false>(L, grid, st) : attn_fwd_dp<T, 128, false>(L, grid, st);
+    return L.d.D <= 64 ? attn_fwd_dp<T, 64, true>(L, st) : attn_fwd_dp<T, 128, true>(L, st);
+  return L.d.D <= 64 ? attn_fwd_dp<T, 64, false>(L, st) : attn_fwd_dp<T, 128, false>(L, st);
 }
 
 }  // namespace osam

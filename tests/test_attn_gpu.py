@@ -171,6 +171,20 @@ def test_tokens_over_a_cache(cuda_lib, Lq, Lk, Hq, Hk, D, cap):
     check(q, k, v, do, mask="causal", lens=lens, cap=cap, slopes=slopes_of(Hq), train=Lk < 5000)
 
 
+@pytest.mark.parametrize("lens,Lk,Hq,Hk", [([5000, 3, 0, 1, 64, 65], 5000, 4, 2), ([0, 0, -1], 900, 2, 2),
+                                           ([1100] * 36, 1100, 2, 1), ([7 * i for i in range(140)], 960, 2, 2),
+                                           ([9000, 1024, 5555, 9001, 700], 9001, 6, 3)])
+@pytest.mark.parametrize("Lq", [1, 70])
+def test_caches_of_any_lengths(cuda_lib, lens, Lk, Hq, Hk, Lq):
+    """The splits follow the sequences' own lengths: more sequences than a warp, one long beside short ones, none."""
+    q, k, v, do = make(len(lens), Lq, Lk, Hq, Hk, 64, seed=Lk + Lq)
+    lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    for b, n in enumerate(lens.clamp(0, Lk).tolist()):
+        k[b, n:] = float("nan")
+        v[b, n:] = float("nan")
+    check(q, k, v, do, mask="causal", lens=lens, train=False)
+
+
 def test_split_documents(cuda_lib):
     q, k, v, do = make(1, 2, 5000, 2, 1, 64, seed=2)
     dk = torch.arange(5000, dtype=torch.int32, device=DEV).div(600, rounding_mode="floor").int()[None].contiguous()
