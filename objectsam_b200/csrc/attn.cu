@@ -261,7 +261,7 @@ AtSplit at_split(const osam_attn_desc& a) {
   const int most = (tiles + s.min_tiles - 1) / s.min_tiles;
   s.splits = std::min(most, (int)(kAfRounds * kAfPlaces / per) - (a.batch - 1));
   s.grid = (int)std::min<long long>(kAfRounds * kAfPlaces / per * per, ctas * most);
-  s.usual = s.grid / (int)ctas;
+  s.usual = (s.grid + (int)ctas - 1) / (int)ctas;
   s.chunk = at_best_chunk(a.batch, (int)per, s.min_tiles, tiles, a.batch * tiles,
                           [&](int chunk) { return a.batch * ((tiles + chunk - 1) / chunk); });
   return s;

@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   __shared__ __align__(8) uint64_t s_full, s_free, p_full[2], pv_done, o_done;
   __shared__ uint32_t tmem_slot;
   __shared__ float pair_top[2][kAfRows], pair_sum[2][kAfRows];  // what the two threads of a row tell each other
+  __shared__ float pair_low[2][SPREAD ? kAfRows : 1];
   __shared__ uint32_t live[kAtDocWords], mix[kAtDocWords], pad[kAtDocWords];
   __shared__ AtDocs own_docs[4];
   __shared__ __align__(16) int col_doc[2][KEYS];
@@ -310,6 +311,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     float m = -INFINITY;  // the row's reference maximum, log2 units (−∞: nothing seen yet)
     float neg = 0.f;      // −m, or 0 while there is none
     float l = 0.f;        // this thread's part of its sum
+    float l16 = 0.f;      // SPREAD: the same of P as the tensor cores read it, rounded to 16 bits
     const uint32_t bar_s = smem_u32(&s_full), bar_free = smem_u32(&s_free), bar_p = smem_u32(&p_full[0]);
     const int c1 = h0 + (SPREAD ? 8 * (warp % 4) : 0);  // first column of this thread
     const uint32_t s_addr = tmem + lane_base + Cfg::COL_S + c1, p_addr = tmem + lane_base + Cfg::COL_P + c1 / 2;
@@ -406,6 +408,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
           m = top;
           neg = -m;
           l *= f;
+          l16 *= f;
         }
         if (ok && it > 0) ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err);  // the previous P·V is in O
         if (!ok) break;
@@ -421,7 +424,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       }
       if (!idle) {
         const float2 mul = make_float2(cmul, cmul), add = make_float2(neg, neg);
-        float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
+        float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)}, low = make_float2(l16, 0.f);
         uint32_t p[N / 2];
 #pragma unroll
         for (int i = 0; i < N / 2; i++) {
@@ -431,7 +434,9 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
           e.y = at_ex2(e.y);
           sum[i & 1] = add2(sum[i & 1], e);
           p[i] = Half16<T>::pack(e.x, e.y);
+          if (SPREAD) low = add2(low, Half16<T>::unpack(p[i]));
         }
+        if (SPREAD) l16 = low.x + low.y;
         // this buffer of P is free: S tells that the P·V before last is done
         if constexpr (!SPREAD)
           tmem_st16(p_addr + (it & 1) * 32, p);
@@ -461,6 +466,15 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       pair_sum[half][row_of] = l;
       named_bar_sync(pair_bar, 64);
       l += pair_sum[half ^ 1][row_of];
+      // few or nearly equal weights share their rounding to 16 bits; against the sum of the rounded weights it cancels (two
+      // tokens over 10860 keys, bf16: error 1.7e-3 instead of 1.9e-3, o's own rounding being 1.6e-3); lse keeps the exact sum
+      float fix = 1.f;
+      if (SPREAD) {
+        pair_low[half][row_of] = l16;
+        named_bar_sync(pair_bar, 64);
+        l16 += pair_low[half ^ 1][row_of];
+        if (l16 > 0.f) fix = l / l16;
+      }
       const long long row = ((long long)b * A.Hq + head) * A.Lq + qi;
       const long long part_row = (long long)split * A.B * A.Hq * A.Lq + row;
       T* o_ptr = static_cast<T*>(P.o.p) + b * P.o.sb + qi * P.o.st + head * P.o.sh;
@@ -505,7 +519,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         float o[16];
         if (it > 0) at_ld16(tmem + lane_base + Cfg::COL_O + c, o);
 #pragma unroll
-        for (int i = 0; i < 16; i++) o[i] = it > 0 && l != 0.f ? o[i] : 0.f;
+        for (int i = 0; i < 16; i++) o[i] = it > 0 && l != 0.f ? (SPREAD ? o[i] * fix : o[i]) : 0.f;
         if (!valid) continue;
         const float lo[8] = {o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7]};
         const float hi[8] = {o[8], o[9], o[10], o[11], o[12], o[13], o[14], o[15]};
