@@ -267,6 +267,16 @@ AtSplit at_split(const osam_attn_desc& a) {
   return s;
 }
 
+// Units of a group (at_order), `bytes` being what one streams: without a bound one; with it all while that stays near
+// L2's size (the last group's longest tiles start late: 64 heads of 4096 × 64 in two groups 308 us instead of 277);
+// beyond, half of L2 (512 heads of 4096 × 64: 2016 us, with a quarter 2097), but three rounds of the GPU's places at
+// least.  512 heads of 4096 × 128: forward 3189 us in one group, 2418 in groups, backward 9121 and 7684.
+int at_group(const osam_attn_desc& a, long long tiles, long long units, double bytes) {
+  if (a.mask == OSAM_ATTN_NONE) return 1;
+  if (bytes * units <= 192e6) return (int)std::max(units, 1LL);
+  return (int)std::min(units, std::max((long long)(64e6 / bytes), 3 * kAfPlaces / std::max(tiles, 1LL) + 1));
+}
+
 // Into how many parts the backward splits the streamed side of a tile: by a model of its time in units of a streamed
 // tile (0.7 us measured): rounds of CTAs over the GPU × (tiles of a part + 5 for a CTA's start and end), and for the
 // parts' sum 8 and its traffic.  One part where the tiles fill the GPU (16 heads of 4096 tokens); with 2 key heads of
@@ -389,6 +399,8 @@ int osam_attn_fwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   L.splits = s.splits;
   L.min_tiles = s.min_tiles;
   L.grid = s.grid;
+  const int g = a->heads_q / a->heads_k;
+  L.group = at_group(*a, ((long long)a->len_q * g + kAfRows - 1) / kAfRows, (long long)a->batch * a->heads_k, 4.0 * a->len_k * a->dim);
   L.chunk_all = s.chunk;
   L.chunk = reinterpret_cast<int*>(w + W.chunk);
   L.part = reinterpret_cast<float*>(w + W.part);
@@ -456,8 +468,11 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
                                     at_view(out)),
                    "sum launch");
   };
+  const int g = a->heads_q / a->heads_k;
   if (!ek) {
     L.parts = at_parts(*a, true);
+    L.group = at_group(*a, (a->len_k + kAbRows - 1) / kAbRows, (long long)a->batch * a->heads_k * L.parts,
+                       4.0 * a->len_q * a->dim * g / L.parts);
     if ((rc = map(&L.stat1, vk, false, kAbRows)) != OSAM_OK || (rc = map(&L.stat2, vv, false, kAbRows)) != OSAM_OK ||
         (rc = map(&L.strm1, vq, true, kAbCols)) != OSAM_OK || (rc = map(&L.strm2, vdo, true, kAbCols)) != OSAM_OK)
       return rc;
@@ -470,6 +485,8 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   }
   if (!eq) {
     L.parts = at_parts(*a, false);
+    L.group = at_group(*a, (a->len_q + kAbRows - 1) / kAbRows, (long long)a->batch * a->heads_q * L.parts,
+                       4.0 * a->len_k * a->dim / g / L.parts);
     L.late = !ek && L.parts == 1;  // its own parts would go over those that a sum in front still reads
     if ((rc = map(&L.stat1, vq, true, kAbRows)) != OSAM_OK || (rc = map(&L.stat2, vdo, true, kAbRows)) != OSAM_OK ||
         (rc = map(&L.strm1, vk, false, kAbCols)) != OSAM_OK || (rc = map(&L.strm2, vv, false, kAbCols)) != OSAM_OK)

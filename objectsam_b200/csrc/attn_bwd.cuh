@@ -85,16 +85,9 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
 
   // ---- which tile (with a causal bound the longest first)
   const int heads = DKV ? A.Hk : A.Hq, nt = ((DKV ? A.Lk : A.Lq) + kAbRows - 1) / kAbRows;
-  const int per = A.B * heads * P.parts;
   int rt, rest;
-  if (A.mask == OSAM_ATTN_NONE) {
-    rt = int(blockIdx.x) % nt;
-    rest = int(blockIdx.x) / nt;
-  } else {
-    rt = int(blockIdx.x) / per;
-    rest = int(blockIdx.x) % per;
-    if (!DKV) rt = nt - 1 - rt;
-  }
+  at_order(blockIdx.x, nt, A.B * heads * P.parts, P.group, rt, rest);
+  if (!DKV && A.mask != OSAM_ATTN_NONE) rt = nt - 1 - rt;
   const int part = rest % P.parts;
   rest /= P.parts;
   const int hd = rest % heads, b = rest / heads;

@@ -113,9 +113,8 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   const int rows = A.Lq * A.G, nq = (rows + kAfRows - 1) / kAfRows;
   int qt, rest, split = 0, splits = 1, first_tile = 0, own_tiles = 1 << 26;
   if (P.splits == 1) {
-    const int per_q = A.B * A.Hk;
-    qt = A.mask == OSAM_ATTN_NONE ? int(blockIdx.x) % nq : nq - 1 - int(blockIdx.x) / per_q;
-    rest = A.mask == OSAM_ATTN_NONE ? int(blockIdx.x) / nq : int(blockIdx.x) % per_q;
+    at_order(blockIdx.x, nq, A.B * A.Hk, P.group, qt, rest);
+    if (A.mask != OSAM_ATTN_NONE) qt = nq - 1 - qt;
   } else {
     const AtSplitCta c = at_split_cta(P, nq * A.Hk, lane, blockIdx.x);
     if (blockIdx.x == 0 && tid == 0) *P.chunk = c.chunk;  // for the join

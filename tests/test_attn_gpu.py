@@ -191,6 +191,16 @@ def test_split_documents(cuda_lib):
     check(q, k, v, do, doc_q=torch.tensor([[3, -1]], dtype=torch.int32, device=DEV), doc_k=dk)
 
 
+def test_many_heads(cuda_lib):
+    """Causal calls whose keys and values pass L2 go over the heads in groups: the same results as in two halves."""
+    t = make(64, 400, 400, 16, 16, 128, seed=4)
+    whole = run(*t, mask="causal")
+    for part in (slice(0, 32), slice(32, 64)):
+        half = run(*(x[part] for x in t), mask="causal")
+        for name, x in half.items():
+            assert torch.equal(whole[name][part], x), name
+
+
 # ---------------------------------------------------------------- ranges
 def test_growing_scores(cuda_lib):
     """Row maxima that grow by far more than the lazy rescale's bound from tile to tile, and shrink again."""
