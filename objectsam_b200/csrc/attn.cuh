@@ -92,7 +92,7 @@ __host__ __device__ __forceinline__ int at_best_chunk(int B, int per, int min_ti
 }
 // Order of the CTAs: `tile` of `unit` (a head, a part of one) for CTA i.  Units go in groups; in a group all units' first
 // tiles come first.  With a causal bound the tiles are ordered longest first, so groups keep a tail of short ones, but all
-// that a group streams should stay in L2 over its tiles (32 × 16 heads of 4096 × 128 in one group: forward 3153 us).
+// that a group streams stays in L2 over its tiles (at_group has what that measured).
 __device__ __forceinline__ void at_order(int i, int tiles, int units, int group, int& tile, int& unit) {
   const int first = i / (group * tiles) * group, here = min(group, units - first);
   i -= first * tiles;
