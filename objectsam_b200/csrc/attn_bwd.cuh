@@ -76,7 +76,6 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
   __shared__ __align__(16) float col_y[NB][BIAS == 2 ? 2 : 1][kAbCols], col_x[NB][BIAS == 2 ? 2 : 1][kAbCols];
 
   if (!P.late) grid_dep_wait();
-  grid_dep_launch();
   const AttnDev& A = P.d;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   uint8_t* smem = ab_raw + ((1024 - (smem_u32(ab_raw) & 1023)) & 1023);
@@ -170,6 +169,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     at_doc_bits(own, DKV ? sq : sk, DKV ? nq64 : nk64, 1, tiles.begin, tiles.end, warp, Cfg::THREADS / 32, live, mix, pad);
   }
   __syncthreads();
+  grid_dep_launch();  // not before TMEM is this CTA's: the next kernel's CTAs may take columns and then wait for this one
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 

@@ -103,7 +103,6 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   __shared__ __align__(16) float col_y[BIAS == 2 ? 2 : 1][KEYS], col_x[BIAS == 2 ? 2 : 1][KEYS];
 
   grid_dep_wait();
-  grid_dep_launch();
   const AttnDev& A = P.d;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   uint8_t* smem = af_raw + ((1024 - (smem_u32(af_raw) & 1023)) & 1023);
@@ -210,6 +209,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     }
   }
   __syncthreads();
+  grid_dep_launch();  // not before TMEM is this CTA's: the next kernel's CTAs may take columns and then wait for this one
   if (docs) {
     AtDocs own = own_docs[0];
     for (int w = 1; w < 4; w++) {
