@@ -230,16 +230,19 @@ __device__ __forceinline__ void at_scores4(const AtBias& P, float2 (&s)[2], cons
   }
 }
 
-// Barrier of the two warps that share rows, with the OR of a flag.
-__device__ __forceinline__ bool at_pair_any(int id, bool flag) {
+// Barrier of `threads` threads with the OR of a flag.  A named barrier has no bound of its own: a warp whose bounded wait
+// ran out stays in step with the others through all of them, without arriving anywhere else and without writing results.
+__device__ __forceinline__ bool at_any(int id, bool flag, int threads) {
   uint32_t r;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
       : "=r"(r)
-      : "r"(uint32_t(flag)), "r"(id)
+      : "r"(uint32_t(flag)), "r"(id), "r"(threads)
       : "memory");
   return r != 0;
 }
+// Of the two warps that share rows.
+__device__ __forceinline__ bool at_pair_any(int id, bool flag) { return at_any(id, flag, 64); }
 
 // The MMA warp runs its loop with all lanes and issues from one, `leader`, by predicate: with warp-uniform control flow
 // the descriptors stay in uniform registers, where the instruction reads them (issued from inside a one-lane branch,

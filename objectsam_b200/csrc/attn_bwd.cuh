@@ -319,13 +319,11 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
         }
         named_bar_sync(1 + buf, 256);
       }
-      if (!(ok = at_wait_warp(&xy_full[buf], (it / NB) & 1, A.err))) break;
+      ok = ok && at_wait_warp(&xy_full[buf], (it / NB) & 1, A.err);
       tc_fence_after();
       const int s = it % Cfg::STAGES;
       const float* rows = reinterpret_cast<const float*>(srows + s * Cfg::ROWS) + h0;
-      if (DKV) {  // written by the bulk copy that this barrier counts
-        if (!(ok = at_wait_warp(&full[s], (it / Cfg::STAGES) & 1, A.err))) break;
-      }
+      if (DKV) ok = ok && at_wait_warp(&full[s], (it / Cfg::STAGES) & 1, A.err);  // counts the rows' bulk copy
       if (BIAS == 1) bias.y = float(pos - (DKV ? off + c0 : c0) - h0) * bias.slope;
       const uint32_t xcol = tmem + lane_base + buf * 128;
       float sv[32], dp[32];
@@ -386,7 +384,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
         const int c = c0 + r % kAbCols, panel = half;
         const bool dead = DKV ? c < A.Lq && A.doc_q[(long long)b * A.Lq + c] < 0
                               : c >= n || (docs && A.doc_k[(long long)b * A.Lk + c] < 0);
-        if (dead && panel < Cfg::PANELS) {
+        if (ok && dead && panel < Cfg::PANELS) {
           uint8_t* d = strm + s * 2 * Cfg::STRM + (r / kAbCols) * Cfg::STRM + panel * kAbCols * 128 + (r % kAbCols) * 128;
 #pragma unroll
           for (int k = 0; k < 8; k++) *reinterpret_cast<uint4*>(d + k * 16) = make_uint4(0, 0, 0, 0);
@@ -396,7 +394,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) at_arrive(smem_u32(&ds_full[buf]));
+      if (lane == 0 && ok) at_arrive(smem_u32(&ds_full[buf]));
       tile++;
     }
     const bool any = it > 0;

@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         }
         named_bar_sync(1, kAfSoft);
       }
-      ok = at_wait(bar_s, it & 1, A.err);
+      ok = ok && at_wait(bar_s, it & 1, A.err);
       tc_fence_after();
       float top = -INFINITY;
       float x[N];
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         at_ld8(s_addr, x);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) at_arrive(bar_free);
+      if (lane == 0 && ok) at_arrive(bar_free);
       t = tiles.next(t);
       if (!idle) {
         uint32_t vis = 0xffffffffu;
@@ -410,7 +410,6 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
           l16 *= f;
         }
         if (ok && it > 0) ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err);  // the previous P·V is in O
-        if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
         for (int c = half * (DP / 2); it > 0 && c < (half + 1) * (DP / 2); c += 16) {
@@ -445,9 +444,9 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         l = s.x + s.y;
       }
       if (dirty) {  // V rows of keys that no query sees hold anything, NaN included: 0·NaN must not enter O
-        if (!(ok = at_wait_warp(&v_full[it % Cfg::STAGES], (it / Cfg::STAGES) & 1, A.err))) break;
+        ok = ok && at_wait_warp(&v_full[it % Cfg::STAGES], (it / Cfg::STAGES) & 1, A.err);
         const int key = tid % KEYS, j = j0 + key, panel = tid / KEYS;  // a thread per row and panel
-        if (panel < Cfg::PANELS && (j >= n || (docs && A.doc_k[(long long)b * A.Lk + j] < 0))) {
+        if (ok && panel < Cfg::PANELS && (j >= n || (docs && A.doc_k[(long long)b * A.Lk + j] < 0))) {
           uint8_t* v = smem + Cfg::QTILE + (Cfg::STAGES + it % Cfg::STAGES) * Cfg::TILE + panel * Cfg::KPANEL + key * 128;
 #pragma unroll
           for (int c = 0; c < 8; c++) *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0, 0, 0, 0);
@@ -457,23 +456,41 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) at_arrive(bar_p + (it & 1) * 8);
+      if (lane == 0 && ok) at_arrive(bar_p + (it & 1) * 8);
     }
     ok = ok && at_wait_warp(&o_done, 0, A.err);
-    if (ok) {
-      tc_fence_after();
-      pair_sum[half][row_of] = l;
+    tc_fence_after();
+    pair_sum[half][row_of] = l;
+    ok = !at_pair_any(pair_bar, !ok);
+    l += pair_sum[half ^ 1][row_of];
+    // few or nearly equal weights share their rounding to 16 bits; against the sum of the rounded weights it cancels (two
+    // tokens over 10860 keys, bf16: error 1.7e-3 instead of 1.9e-3, o's own rounding being 1.6e-3); lse keeps the exact sum
+    float fix = 1.f;
+    float w4[4] = {1.f, 0.f, 0.f, 0.f};  // the groups' weights
+    const int g = warp % 4;
+    if (SPREAD) {
+      pair_low[half][row_of] = l16;
       named_bar_sync(pair_bar, 64);
-      l += pair_sum[half ^ 1][row_of];
-      // few or nearly equal weights share their rounding to 16 bits; against the sum of the rounded weights it cancels (two
-      // tokens over 10860 keys, bf16: error 1.7e-3 instead of 1.9e-3, o's own rounding being 1.6e-3); lse keeps the exact sum
-      float fix = 1.f;
-      if (SPREAD) {
-        pair_low[half][row_of] = l16;
-        named_bar_sync(pair_bar, 64);
-        l16 += pair_low[half ^ 1][row_of];
-        if (l16 > 0.f) fix = l / l16;
+      l16 += pair_low[half ^ 1][row_of];
+      if (l16 > 0.f) fix = l / l16;
+      if (half == 0) {
+        pair_top[0][row_of] = m;
+        pair_top[1][row_of] = l;
       }
+      ok = !at_any(1, !ok, kAfSoft);
+      float M = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 4; k++) M = fmaxf(M, pair_top[0][k * 32 + lane]);
+      l = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float mk = pair_top[0][k * 32 + lane];
+        w4[k] = mk == -INFINITY ? 0.f : at_ex2(mk - M);
+        l = fmaf(w4[k], pair_top[1][k * 32 + lane], l);
+      }
+      m = M;
+    }
+    if (ok) {
       const long long row = ((long long)b * A.Hq + head) * A.Lq + qi;
       const long long part_row = (long long)split * A.B * A.Hq * A.Lq + row;
       T* o_ptr = static_cast<T*>(P.o.p) + b * P.o.sb + qi * P.o.st + head * P.o.sh;
@@ -490,27 +507,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
           d[1] = make_float4(v[4], v[5], v[6], v[7]);
         }
       };
-      float w4[4] = {1.f, 0.f, 0.f, 0.f};  // the groups' weights
       float* joined = reinterpret_cast<float*>(smem);  // [group][row][DP + 4]: the operands' room is free by now
-      const int g = warp % 4;
-      if (SPREAD) {
-        if (half == 0) {
-          pair_top[0][row_of] = m;
-          pair_top[1][row_of] = l;
-        }
-        named_bar_sync(1, kAfSoft);
-        float M = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < 4; k++) M = fmaxf(M, pair_top[0][k * 32 + lane]);
-        l = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const float mk = pair_top[0][k * 32 + lane];
-          w4[k] = mk == -INFINITY ? 0.f : at_ex2(mk - M);
-          l = fmaf(w4[k], pair_top[1][k * 32 + lane], l);
-        }
-        m = M;
-      }
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays one
 #pragma unroll
       for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 16) {

@@ -38,3 +38,35 @@ def test_dependents_start_after_tensor_memory_is_taken():
     for name, body in both:
         between = body[body.rindex("tmem_alloc"):body.index("grid_dep_launch")]
         assert body.rindex("tmem_alloc") < body.index("grid_dep_launch") and "__syncthreads" in between, name
+
+
+def block(text, start):
+    """The brace block that follows `start`."""
+    at = text.index("{", text.index(start))
+    depth = 0
+    for end in range(at, len(text)):
+        depth += (text[end] == "{") - (text[end] == "}")
+        if not depth:
+            return text[at:end + 1]
+
+
+@pytest.mark.parametrize("kernel,loop", [("attn_fwd.cuh:k_attn_fwd", "for (int t = tiles.first(); t < tiles.end; it++)"),
+                                         ("attn_bwd.cuh:k_attn_bwd", "for (; x.more(tiles, streams); x.step(tiles), it++)")])
+def test_warps_whose_wait_ran_out_stay_in_step(kernel, loop):
+    """The softmax warps share named barriers, which have no bound: none leaves the loop over the tiles early, waits again
+    after a failed wait, or arrives for others after one."""
+    body = dict(kernels())[kernel]
+    tiles = block(body, loop)
+    assert "named_bar_sync" in tiles and not re.search(r"\b(break|return|goto)\b", tiles)
+    for wait in re.finditer(r"[^;{}]*\bat_wait\w*\(", tiles):
+        assert re.search(r"\bok &&", wait.group(0)), wait.group(0)
+    for arrive in re.finditer(r"[^;{}]*\bat_arrive\(", tiles):
+        assert "&& ok" in arrive.group(0), arrive.group(0)
+
+
+def test_results_are_written_by_agreement():
+    """The forward's barriers behind its loop over the tiles: a failed wait is agreed on before any that only some pass."""
+    body = dict(kernels())["attn_fwd.cuh:k_attn_fwd"]
+    tail = body[body.index("at_wait_warp(&o_done, 0, A.err);\n    tc_fence_after"):]
+    head = tail[:tail.index("if (ok)")]
+    assert "at_pair_any(pair_bar, !ok)" in head and "at_any(1, !ok, kAfSoft)" in head
