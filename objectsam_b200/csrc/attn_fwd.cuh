@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     }
     const int tail = n < A.Lk ? n : INT_MAX;  // keys from here on hold anything
     bool ok = true;
-    int it = 0;
+    int it = 0, fills = 0;
     for (int t = tiles.first(); t < tiles.end; it++) {
       const int j0 = t * KEYS;
       bool by_doc = false, dirty = j0 + KEYS > tail;
@@ -330,17 +330,21 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         dirty |= at_bit(pad, t - tiles.begin);
       }
       const bool masked = by_doc || j0 + KEYS > lim_min;
-      if (by_doc || BIAS == 2) {  // per-key data of the tile, one key a thread
+      // Per-key data of the tile, one key a thread.  The buffer goes by the fills, not by the tiles: the barrier of the fill
+      // in between tells that all warps have read what this one overwrites (tiles without a fill have no barrier).
+      const int slot = fills & 1;
+      if (by_doc || BIAS == 2) {
+        fills++;
         if (tid < KEYS) {
           const int j = j0 + tid;
           if (docs) {
             const int id = j < n ? A.doc_k[(long long)b * A.Lk + j] : -1;
-            col_doc[it & 1][tid] = id < 0 ? -1 : id;
+            col_doc[slot][tid] = id < 0 ? -1 : id;
           }
           if (BIAS == 2) {
             const float2 cell = at_cell(A, j);
-            col_y[it & 1][tid] = cell.x;
-            col_x[it & 1][tid] = cell.y;
+            col_y[slot][tid] = cell.x;
+            col_x[slot][tid] = cell.y;
           }
         }
         named_bar_sync(1, kAfSoft);
@@ -361,7 +365,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         uint32_t vis = 0xffffffffu;
         if (masked) {
           vis = at_low_bits(lim - j0 - c1);
-          if (by_doc) vis &= at_same_doc<N>(&col_doc[it & 1][c1], my_doc);
+          if (by_doc) vis &= at_same_doc<N>(&col_doc[slot][c1], my_doc);
           if (CAP) at_mask(x, vis, 0.f);
         }
         if (CAP || BIAS) {
@@ -376,8 +380,8 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
             float2 s2[2] = {make_float2(x[c], x[c + 1]), make_float2(x[c + 2], x[c + 3])}, sig[2];
             float4 ky = {}, kx = {};
             if (BIAS == 2) {
-              ky = *reinterpret_cast<const float4*>(&col_y[it & 1][c1 + c]);
-              kx = *reinterpret_cast<const float4*>(&col_x[it & 1][c1 + c]);
+              ky = *reinterpret_cast<const float4*>(&col_y[slot][c1 + c]);
+              kx = *reinterpret_cast<const float4*>(&col_x[slot][c1 + c]);
             }
             at_scores4<CAP, BIAS, false>(bias, s2, none, line, ky, kx, sig);
             x[c] = s2[0].x;

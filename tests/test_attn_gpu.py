@@ -367,3 +367,19 @@ def test_long_rows_of_few_heads(cuda_lib, mask, D):
     doc = torch.arange(L, dtype=torch.int32, device=DEV).div(500, rounding_mode="floor").int()[None].contiguous()
     check(q, k, v, do, mask=mask, doc_q=doc, doc_k=doc,
           prefix=torch.tensor([600], dtype=torch.int32, device=DEV) if mask == "prefix" else None)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bias", ["none", "line", "grid"])
+@pytest.mark.parametrize("tiles", [2, 3, 4])
+def test_documents_of_a_few_tiles(cuda_lib, D, bias, tiles):
+    """Key tiles that compare ids alternate with tiles of one document: the same bits every time, and the masks' results."""
+    B, L = 2, 1000
+    q, k, v, do = make(B, L, L, 4, 2, D, seed=18)
+    doc = (torch.arange(L, device=DEV) + 32).div(64 * tiles, rounding_mode="floor").int().expand(B, -1).contiguous()
+    kw = dict(doc_q=doc, doc_k=doc, slopes=None if bias == "none" else slopes_of(4), grid_w=25 if bias == "grid" else 0)
+    first = check(q, k, v, do, **kw)
+    for _ in range(10):
+        again = run(q, k, v, do, **kw)
+        for n in first:
+            assert torch.equal(first[n], again[n]), n

@@ -70,3 +70,14 @@ def test_results_are_written_by_agreement():
     tail = body[body.index("at_wait_warp(&o_done, 0, A.err);\n    tc_fence_after"):]
     head = tail[:tail.index("if (ok)")]
     assert "at_pair_any(pair_bar, !ok)" in head and "at_any(1, !ok, kAfSoft)" in head
+
+
+def test_buffers_of_the_columns_go_by_their_barriers():
+    """The forward fills its two buffers of per-key data in some tiles only, with a barrier in those: a buffer chosen by the
+    tile's number could be filled again while a warp still reads what it held two tiles ago."""
+    tiles = block(dict(kernels())["attn_fwd.cuh:k_attn_fwd"], "for (int t = tiles.first(); t < tiles.end; it++)")
+    fill = block(tiles, "if (by_doc || BIAS == 2)")
+    assert "fills++;" in fill and "named_bar_sync(1, kAfSoft);" in fill and tiles.count("fills++") == 1
+    assert "const int slot = fills & 1;" in tiles[:tiles.index(fill)]
+    uses = re.findall(r"col_(?:doc|y|x)\[([^]]*)\]", tiles)
+    assert len(uses) == 6 and set(uses) == {"slot"}
