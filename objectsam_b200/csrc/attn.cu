@@ -1,5 +1,7 @@
 // Attention: the C entry points, argument checks and workspace layout, and the small kernels around the two main
 // ones (attn_fwd.cuh, attn_bwd.cuh): document summaries, the join of split keys, the backward's row terms.
+#include <float.h>
+
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -135,52 +137,70 @@ __global__ void __launch_bounds__(256) k_attn_sum(const float* part, int parts, 
 }
 
 // Row terms of the backward pass, per 64-query block (padded to whole blocks): (u − lse·log2 e, −δ), δ = do·o, u = log2
-// of the factor that the backward holds P times — (−∞, 0) for that see nothing and for the padding, whose P is then 0 — and the block's largest |dO|.  One CTA per
-// block, 16 lanes per row (a 16-byte vector each).
+// of the factor that the backward holds P times — (−∞, 0) for queries that see nothing and for the padding, whose P is
+// then 0 — and for fp16 the block's largest ‖dO_i‖ and, in CTAs behind the query blocks', the largest ‖v_j‖ of each
+// 64-key block, over rows that are finite (another one's gradients are not finite whatever dS is held times) and keys in
+// use.  One CTA per block, 16 lanes per row (a 16-byte vector each).
 template <typename T>
-__global__ void __launch_bounds__(256) k_attn_rows(const AtView o, const AtView dout, const float* lse, int Hq, int Lq,
-                                                   int D, float* rows, float* peak) {
+__global__ void __launch_bounds__(256) k_attn_rows(const __grid_constant__ AttnDev A, const AtView o, const AtView dout,
+                                                   const AtView v, const float* lse, float* rows, float* peak, float* vpeak) {
   __shared__ float top[8];
-  constexpr float up = Half16<T>::kBf16 ? 0.f : kAbUp;
-  const int nb = (Lq + kAbCols - 1) / kAbCols;
-  const int blk = blockIdx.x % nb, h = (blockIdx.x / nb) % Hq, b = blockIdx.x / nb / Hq;
-  const int c = threadIdx.x % 16;
-  const long long bh = (long long)b * Hq + h;
+  constexpr bool BF16 = Half16<T>::kBf16;
+  constexpr float up = BF16 ? 0.f : kAbUp;
+  const int nq = (A.Lq + kAbCols - 1) / kAbCols, nk = (A.Lk + kAbCols - 1) / kAbCols;
+  const int c = threadIdx.x % 16, D = A.D;
+  const bool keys = !BF16 && (int)blockIdx.x >= nq * A.Hq * A.B;
+  const int at = keys ? blockIdx.x - nq * A.Hq * A.B : blockIdx.x, nb = keys ? nk : nq, heads = keys ? A.Hk : A.Hq;
+  const int blk = at % nb, h = (at / nb) % heads, b = at / nb / heads;
+  const long long bh = (long long)b * heads + h;
   grid_dep_wait();
   grid_dep_launch();
-  float big = 0.f;
+  const int n = keys ? at_keys(A, b) : 0;
+  float big = 0.f;  // largest ‖·‖²
 #pragma unroll
   for (int k = 0; k < kAbCols; k += 16) {
     const int r = k + threadIdx.x / 16, i = blk * kAbCols + r;
-    const float L = i < Lq ? lse[bh * Lq + i] : -INFINITY;
-    const bool live = L != -INFINITY;
-    float d = 0.f;
+    float L = -INFINITY;
+    bool live;
+    if (keys) {
+      live = i < n && !(A.doc_k && A.doc_k[(long long)b * A.Lk + i] < 0);
+    } else {
+      if (i < A.Lq) L = lse[bh * A.Lq + i];
+      live = L != -INFINITY;
+    }
+    const AtView& t = keys ? v : dout;
+    float d = 0.f, s2 = 0.f;
     if (live && c * 8 < D) {
       float a[8], g[8];
-      unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(o.p) + b * o.sb + i * o.st + h * o.sh + c * 8), a);
-      unpack8<T>(
-          *reinterpret_cast<const uint4*>(static_cast<const T*>(dout.p) + b * dout.sb + i * dout.st + h * dout.sh + c * 8), g);
+      unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(t.p) + b * t.sb + i * t.st + h * t.sh + c * 8), g);
+      if (!keys) {
+        unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(o.p) + b * o.sb + i * o.st + h * o.sh + c * 8), a);
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        d = fmaf(a[e], g[e], d);
-        big = fmaxf(big, fabsf(g[e]));
+        for (int e = 0; e < 8; e++) d = fmaf(a[e], g[e], d);
       }
+      if (!BF16)
+#pragma unroll
+        for (int e = 0; e < 8; e++) s2 = fmaf(g[e], g[e], s2);
     }
 #pragma unroll
-    for (int s = 8; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
-    if (c == 0) {
+    for (int s = 8; s > 0; s >>= 1) {
+      d += __shfl_xor_sync(0xffffffffu, d, s);
+      if (!BF16) s2 += __shfl_xor_sync(0xffffffffu, s2, s);
+    }
+    if (s2 <= FLT_MAX) big = fmaxf(big, s2);  // neither infinite nor NaN
+    if (c == 0 && !keys) {
       float* out = rows + (bh * nb + blk) * 2 * kAbCols + r;
       out[0] = live ? up - L * kAtLog2e : -INFINITY;
       out[kAbCols] = live ? -d : 0.f;
     }
   }
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
+  if (BF16) return;
+  big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
   if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = big;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 8; w++) big = fmaxf(big, top[w]);
-    peak[bh * nb + blk] = big;
+    (keys ? vpeak : peak)[bh * nb + blk] = sqrtf(big);
   }
 }
 
@@ -303,7 +323,7 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Workspace: document summaries | split outputs and statistics (forward) or row terms (backward).
 struct AtLayout {
-  size_t sum_q = 0, sum_k = 0, part = 0, stats = 0, chunk = 0, rows = 0, peak = 0, grad = 0, bytes = 0;
+  size_t sum_q = 0, sum_k = 0, part = 0, stats = 0, chunk = 0, rows = 0, peak = 0, vpeak = 0, grad = 0, bytes = 0;
 };
 AtLayout at_layout(const osam_attn_desc& a) {
   AtLayout L;
@@ -327,7 +347,8 @@ AtLayout at_layout(const osam_attn_desc& a) {
   }
   const size_t blocks = (size_t)a.batch * a.heads_q * ((a.len_q + kAbCols - 1) / kAbCols);
   L.peak = at + up256(blocks * 2 * kAbCols * sizeof(float));
-  L.grad = L.peak + up256(blocks * sizeof(float));
+  L.vpeak = L.peak + up256(blocks * sizeof(float));
+  L.grad = L.vpeak + up256((size_t)a.batch * a.heads_k * ((a.len_k + kAbCols - 1) / kAbCols) * sizeof(float));
   const int pk = at_parts(a, true), pq = at_parts(a, false);
   const size_t nk = (size_t)a.batch * a.heads_k * a.len_k * a.dim, nq = rows * a.dim;
   const size_t grad = std::max(pk > 1 ? pk * 2 * nk : 0, pq > 1 ? pq * nq : 0) * sizeof(float);
@@ -444,15 +465,18 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   if ((rc = at_dev(*a, W, w, &L.d, st)) != OSAM_OK) return rc;
   float* rows = reinterpret_cast<float*>(w + W.rows);
   float* peak = reinterpret_cast<float*>(w + W.peak);
+  float* vpeak = reinterpret_cast<float*>(w + W.vpeak);
   const int blocks = a->batch * a->heads_q * ((a->len_q + kAbCols - 1) / kAbCols);
   if (blocks > 0) {
-    if ((rc = at_cuda(launch_dependent(bf16 ? k_attn_rows<__nv_bfloat16> : k_attn_rows<__half>, blocks, 256, 0, st, at_view(o),
-                                       at_view(dout), lse, a->heads_q, a->len_q, a->dim, rows, peak),
+    const unsigned grid = blocks + (bf16 ? 0u : (unsigned)a->batch * a->heads_k * ((a->len_k + kAbCols - 1) / kAbCols));
+    if ((rc = at_cuda(launch_dependent(bf16 ? k_attn_rows<__nv_bfloat16> : k_attn_rows<__half>, grid, 256, 0, st, L.d, at_view(o),
+                                       at_view(dout), at_view(v), lse, rows, peak, vpeak),
                       "row terms")) != OSAM_OK)
       return rc;
   }
   L.rows = rows;
   L.peak = peak;
+  L.vpeak = vpeak;
   // a side of length 0 is never visited: its maps only have to be valid
   const bool eq = a->len_q == 0, ek = a->len_k == 0;
   const osam_view &vq = eq ? k : q, &vdo = eq ? k : dout, &vk = ek ? q : k, &vv = ek ? q : v;

@@ -11,9 +11,11 @@
 //   two threads per row (32 columns each): p = 2^(x − lse), ds = p·(dp − δ)·(1 − t²), back to TMEM in 16 bits over
 //   X and Y
 //   acc2 += P·strm2 (DKV), acc1 += dS·strm1, P and dS as TMEM operands
-// fp16 keeps its precision over long rows and small gradients by powers of two: P is held times 2^8 and dS times
-// 2^8·F with F = 2^−e, e the exponent of the largest |dO| (of the key head's group for DKV, of the row's block for
-// DQ), both taken back in fp32 at the end; bf16 needs neither.
+// fp16 keeps its precision over long rows and gradients of any size by powers of two: P is held times 2^8 and dS times
+// 2^8·F, both taken back in fp32 at the end; bf16 needs neither.  F comes from a bound: with dP_ij = dO_i·v_j and
+// δ_i = Σ_k p_ik dP_ik, |dS_ij| = p_ij·|dP_ij − δ_i| ≤ 2·p_ij·(1 − p_ij)·max_k |dP_ik| ≤ ½·‖dO_i‖·max‖v‖.  F = 2^(7−e), e the
+// exponent of max‖dO‖·max‖v‖ (of the key head and its group for DKV, of the row's block and its key head for DQ),
+// keeps dS within 2^15 and leaves 2^29 below that to normal numbers.
 // Warps: 8 per buffer of (X, Y) for the element-wise part (warps w and w + 4 share rows), then the TMA producer and the
 // MMA issuer.  Up to 64 head dims one buffer and 256 TMEM columns, two CTAs per SM; above, two buffers in one CTA
 // with all 512 columns: the tensor cores work on one while the other is in the element-wise part.
@@ -257,19 +259,25 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     // DKV: queries from `from` on see the key; DQ: keys below `lim` are seen
     const int from = row >= n ? INT_MAX : (!causal || prefix > row ? 0 : row - off);
     const int lim = !DKV && valid ? at_limit(A, n, prefix, pos) : 0;
-    float F = 1.f;  // power of two that brings the largest |dO| to [1, 2)
+    float F = 1.f;
     if (!BF16) {
-      float peak = 0.f;
+      float peak = 0.f, vpeak = 0.f;
+      const float* vk = P.vpeak + ((long long)b * A.Hk + (DKV ? hd : hd / A.G)) * nk64;
+      for (int i = lane; i < nk64; i += 32) vpeak = fmaxf(vpeak, vk[i]);
       if (DKV) {
         const float* pk = P.peak + ((long long)b * A.Hq + hd * A.G) * nq64;
         for (int i = lane; i < A.G * nq64; i += 32) peak = fmaxf(peak, pk[i]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
       } else if (valid) {
         peak = P.peak[((long long)b * A.Hq + hd) * nq64 + row / kAbCols];
       }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        vpeak = fmaxf(vpeak, __shfl_xor_sync(0xffffffffu, vpeak, o));
+        if (DKV) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+      }
+      peak *= vpeak;  // at most 2^40: rows of 128 fp16 numbers
       const int e = (__float_as_int(peak) >> 23) & 255;
-      if (peak > 0.f && e < 255) F = __int_as_float(min(227, max(27, 254 - e)) << 23);  // at most 2^±100
+      if (peak > 0.f) F = __int_as_float(min(227, max(27, 127 + 7 + 127 - e)) << 23);  // at most 2^±100
     }
     float row_lse = 0.f, row_delta = 0.f;
     if (!DKV) {

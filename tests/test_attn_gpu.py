@@ -383,3 +383,28 @@ def test_documents_of_a_few_tiles(cuda_lib, D, bias, tiles):
         again = run(q, k, v, do, **kw)
         for n in first:
             assert torch.equal(first[n], again[n]), n
+
+
+# ---------------------------------------------------------------- sizes of v
+@pytest.mark.parametrize("mask", ["none", "causal"])
+def test_two_keys_of_opposite_values(cuda_lib, mask):
+    """p = ½ on v = +8 and −8 at 128 dims: dS = ±512 in fp16, twice what dO's size alone would leave room for."""
+    q, k, v, do = make(2, 3, 2, 2, 1, 128, seed=21)
+    q.zero_(), do.fill_(1.0)
+    v[:, 0], v[:, 1] = 8.0, -8.0
+    check(q, k, v, do, mask=mask)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", [2.0 ** -8, 256.0, 1024.0])
+@pytest.mark.parametrize("mask", ["none", "causal"])
+def test_size_of_v(cuda_lib, D, dtype, size, mask):
+    """dP and dS grow with v; a row of large values that nothing may see changes nothing.  dO brings the gradients of queries and
+    keys to one size, within fp16's normal numbers, where the bounds hold."""
+    q, k, v, do = make(1, 200, 230, 4, 2, D, dtype, seed=22)
+    doc_q, doc_k = (torch.zeros(1, n, dtype=torch.int32, device=DEV) for n in (200, 230))
+    doc_k[0, 100] = -1
+    v *= size
+    v[0, 100] = 60000.0
+    check(q, k, v, do * (16 if size < 1 else 1 / 64), mask=mask, doc_q=doc_q, doc_k=doc_k)
