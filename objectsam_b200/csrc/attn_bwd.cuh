@@ -163,6 +163,8 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
   if (warp == 8 * NB + 1) {
     tmem_alloc(&tmem_slot, Cfg::TMEM);
     tmem_relinquish();
+    // the CTA's one signal, given once TMEM is its own: the next kernel's CTAs may take columns and then wait for this one
+    grid_dep_launch();
   }
   if (docs) {
     const AtDocs* sq = A.sum_q + (long long)b * nq64;
@@ -171,7 +173,6 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     at_doc_bits(own, DKV ? sq : sk, DKV ? nq64 : nk64, 1, tiles.begin, tiles.end, warp, Cfg::THREADS / 32, live, mix, pad);
   }
   __syncthreads();
-  grid_dep_launch();  // not before TMEM is this CTA's: the next kernel's CTAs may take columns and then wait for this one
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 

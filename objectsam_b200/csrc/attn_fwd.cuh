@@ -181,6 +181,8 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   if (warp == 9) {
     tmem_alloc(&tmem_slot, 256);
     tmem_relinquish();
+    // the CTA's one signal, given once TMEM is its own: the next kernel's CTAs may take columns and then wait for this one
+    grid_dep_launch();
   }
   if (warp < 8) {
     // Q rows into the K-major swizzled panels; rows past the end and dims past D are zero
@@ -209,7 +211,6 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     }
   }
   __syncthreads();
-  grid_dep_launch();  // not before TMEM is this CTA's: the next kernel's CTAs may take columns and then wait for this one
   if (docs) {
     AtDocs own = own_docs[0];
     for (int w = 1; w < 4; w++) {
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       tmem_st16(tmem + lane_base + Cfg::COL_P + 32 + h0 / 2, zero);
     }
     const int tail = n < A.Lk ? n : INT_MAX;  // keys from here on hold anything
-    bool ok = true;
+    bool ok = true, lead = lane == 0;  // lead: arrives for the warp, until a wait of its own or its partner's has run out
     int it = 0, fills = 0;
     for (int t = tiles.first(); t < tiles.end; it++) {
       const int j0 = t * KEYS;
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         }
         named_bar_sync(1, kAfSoft);
       }
-      ok = ok && at_wait(bar_s, it & 1, A.err);
+      if (ok) ok = at_wait(bar_s, it & 1, A.err);
       tc_fence_after();
       float top = -INFINITY;
       float x[N];
@@ -359,7 +360,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         at_ld8(s_addr, x);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0 && ok) at_arrive(bar_free);
+      if (lead) at_arrive(bar_free);
       t = tiles.next(t);
       if (!idle) {
         uint32_t vis = 0xffffffffu;
@@ -414,6 +415,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
           l16 *= f;
         }
         if (ok && it > 0) ok = at_wait_warp(&pv_done, (it - 1) & 1, A.err);  // the previous P·V is in O
+        lead &= ok;
         tc_fence_after();
 #pragma unroll 1
         for (int c = half * (DP / 2); it > 0 && c < (half + 1) * (DP / 2); c += 16) {
@@ -448,7 +450,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         l = s.x + s.y;
       }
       if (dirty) {  // V rows of keys that no query sees hold anything, NaN included: 0·NaN must not enter O
-        ok = ok && at_wait_warp(&v_full[it % Cfg::STAGES], (it / Cfg::STAGES) & 1, A.err);
+        if (ok) lead &= ok = at_wait_warp(&v_full[it % Cfg::STAGES], (it / Cfg::STAGES) & 1, A.err);
         const int key = tid % KEYS, j = j0 + key, panel = tid / KEYS;  // a thread per row and panel
         if (ok && panel < Cfg::PANELS && (j >= n || (docs && A.doc_k[(long long)b * A.Lk + j] < 0))) {
           uint8_t* v = smem + Cfg::QTILE + (Cfg::STAGES + it % Cfg::STAGES) * Cfg::TILE + panel * Cfg::KPANEL + key * 128;
@@ -460,12 +462,17 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0 && ok) at_arrive(bar_p + (it & 1) * 8);
+      if (lead) at_arrive(bar_p + (it & 1) * 8);
     }
     ok = ok && at_wait_warp(&o_done, 0, A.err);
     tc_fence_after();
     pair_sum[half][row_of] = l;
-    ok = !at_pair_any(pair_bar, !ok);
+    if (SPREAD) {
+      pair_low[half][row_of] = l16;
+      named_bar_sync(pair_bar, 64);
+    } else {
+      ok = !at_pair_any(pair_bar, !ok);
+    }
     l += pair_sum[half ^ 1][row_of];
     // few or nearly equal weights share their rounding to 16 bits; against the sum of the rounded weights it cancels (two
     // tokens over 10860 keys, bf16: error 1.7e-3 instead of 1.9e-3, o's own rounding being 1.6e-3); lse keeps the exact sum
@@ -473,8 +480,6 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     float w4[4] = {1.f, 0.f, 0.f, 0.f};  // the groups' weights
     const int g = warp % 4;
     if (SPREAD) {
-      pair_low[half][row_of] = l16;
-      named_bar_sync(pair_bar, 64);
       l16 += pair_low[half ^ 1][row_of];
       if (l16 > 0.f) fix = l / l16;
       if (half == 0) {

@@ -37,7 +37,9 @@ def test_dependents_start_after_tensor_memory_is_taken():
     assert {"attn_fwd.cuh:k_attn_fwd", "attn_bwd.cuh:k_attn_bwd", "conv_fprop.cuh:k_conv_fprop"} <= {n for n, _ in both}
     for name, body in both:
         between = body[body.rindex("tmem_alloc"):body.index("grid_dep_launch")]
-        assert body.rindex("tmem_alloc") < body.index("grid_dep_launch") and "__syncthreads" in between, name
+        # the warp that has allocated signals, or the CTA has met since
+        assert body.rindex("tmem_alloc") < body.index("grid_dep_launch"), name
+        assert "__syncthreads" in between or not re.search(r"[{}]", between), name
 
 
 def block(text, start):
@@ -59,9 +61,11 @@ def test_warps_whose_wait_ran_out_stay_in_step(kernel, loop):
     tiles = block(body, loop)
     assert "named_bar_sync" in tiles and not re.search(r"\b(break|return|goto)\b", tiles)
     for wait in re.finditer(r"[^;{}]*\bat_wait\w*\(", tiles):
-        assert re.search(r"\bok &&", wait.group(0)), wait.group(0)
+        assert re.search(r"ok = ok && |\bif \([^=]*\bok\b[^=]*\) (lead &= )?ok = ", wait.group(0)), wait.group(0)
     for arrive in re.finditer(r"[^;{}]*\bat_arrive\(", tiles):
-        assert "&& ok" in arrive.group(0), arrive.group(0)
+        assert re.search(r"if \((lead|lane == 0 && ok)\)", arrive.group(0)), arrive.group(0)
+    if "if (lead)" in tiles:  # `lead` is what is agreed on in the tile in which a wait ran out
+        assert re.search(r"ok = !at_pair_any\(pair_bar, !ok\);.*?ok = at_wait_warp\(&pv_done[^;]*;\s*lead &= ok;", tiles, re.S)
 
 
 def test_results_are_written_by_agreement():
