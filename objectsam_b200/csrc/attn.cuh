@@ -171,13 +171,26 @@ __device__ __forceinline__ void at_sigmoid4(float2 (&u)[2]) {
   u[1] = mul2(make_float2(half.y, half.y), make_float2(a[1].y, a[1].x));
 }
 
-// Scores in log2 units: s ← cap·tanh(scale·s/cap)·log2 e (CAP) or s·scale·log2 e, minus slope·dist.
+// Scores in log2 units: s ← cap·tanh(scale·s/cap)·log2 e (CAP) or s·scale·log2 e, minus slope·dist.  tanh y is taken as
+// 1 − 2/(1 + e^2y), which is off by 2^-23 whatever y is: cap·tanh by 2e-7·cap, 2.6e-5 at kAtCapLarge, a tenth of fp16's
+// rounding of P.  Above it (CAP = 2) small y, |y| < ½, go by tanh's series to y^13, off by 9e-8 of the score (the other form by
+// 4e-7 beyond), at a price: 2 × 4096 causal tokens, 16/4 heads × 128, forward 255 → 347 us, backward 659 → 871.
+constexpr float kAtCapLarge = 128.f;
 struct AtBias {
   float mul;        // scale·log2 e, or with a cap 2·scale·log2 e / cap
   float cap2;       // cap·log2 e
+  float lin, arg;   // CAP = 2: scale·log2 e and scale / cap
   float slope;      // of the row's head, ·log2 e
   float y, x;       // the row's position on the map times the slope; line: y only, relative to the chunk's first column
 };
+// tanh(y)/y from z = y² < ¼: its Taylor series.
+__device__ __forceinline__ float2 at_tanh_ratio(float2 z) {
+  constexpr float c[7] = {1.f, -1.f / 3, 2.f / 15, -17.f / 315, 62.f / 2835, -1382.f / 155925, 21844.f / 6081075};
+  float2 r = make_float2(c[6], c[6]);
+#pragma unroll
+  for (int i = 5; i >= 0; i--) r = fma2(r, z, make_float2(c[i], c[i]));
+  return r;
+}
 // Distances along the line of four consecutive columns, carried from one group of four to the next.
 struct AtLine {
   float2 d[2], step;
@@ -193,7 +206,7 @@ struct AtLine {
 };
 // Four consecutive columns; `line` holds their distances (line), ky / kx their cells (grid).  out: the scores plus
 // `add` (ADD); with CAP, sig = 1/(1 + 2^u), from which 1 − tanh² = 4·sig·(1 − sig).
-template <bool CAP, int BIAS, bool ADD>
+template <int CAP, int BIAS, bool ADD>
 __device__ __forceinline__ void at_scores4(const AtBias& P, float2 (&s)[2], const float2 (&add)[2], AtLine& line,
                                            const float4& ky, const float4& kx, float2 (&sig)[2]) {
   const float2 mul = make_float2(P.mul, P.mul);
@@ -219,6 +232,16 @@ __device__ __forceinline__ void at_scores4(const AtBias& P, float2 (&s)[2], cons
     sig[1] = mul2(s[1], mul);
     at_sigmoid4(sig);
     const float2 m2 = make_float2(-2.f * P.cap2, -2.f * P.cap2), c2 = make_float2(P.cap2, P.cap2);
+    if (CAP == 2) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const float2 y = mul2(s[i], make_float2(P.arg, P.arg)), lin = mul2(s[i], make_float2(P.lin, P.lin)),
+                     far = fma2(m2, sig[i], c2), r = mul2(lin, at_tanh_ratio(mul2(y, y)));
+        s[i] = make_float2(fabsf(y.x) < 0.5f ? r.x : far.x, fabsf(y.y) < 0.5f ? r.y : far.y);
+        if (ADD || BIAS) s[i] = add2(s[i], b[i]);
+      }
+      return;
+    }
     s[0] = fma2(m2, sig[0], ADD || BIAS ? add2(c2, b[0]) : c2);
     s[1] = fma2(m2, sig[1], ADD || BIAS ? add2(c2, b[1]) : c2);
   } else if (ADD || BIAS) {

@@ -64,7 +64,7 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-template <typename T, int DP, bool DKV, bool CAP, int BIAS>
+template <typename T, int DP, bool DKV, int CAP, int BIAS>
 __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     k_attn_bwd(const __grid_constant__ AttnBwdLaunch P) {
   using Cfg = AbCfg<DP>;
@@ -289,6 +289,8 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
     AtBias bias;
     bias.mul = CAP ? 2.f * A.scale * kAtLog2e / A.cap : A.scale * kAtLog2e;
     bias.cap2 = A.cap * kAtLog2e;
+    bias.lin = A.scale * kAtLog2e;
+    bias.arg = A.scale / A.cap;
     bias.slope = bias.y = bias.x = 0.f;
     int slope_of = -1;
     AbIter x;
@@ -451,7 +453,7 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
   }
 }
 
-template <typename T, int DP, bool DKV, bool CAP, int BIAS>
+template <typename T, int DP, bool DKV, int CAP, int BIAS>
 cudaError_t attn_bwd_one(const AttnBwdLaunch& L, int grid, cudaStream_t st) {
   static bool set[64] = {};  // per device; a race only repeats the call
   int dev = 0;
@@ -466,16 +468,19 @@ cudaError_t attn_bwd_one(const AttnBwdLaunch& L, int grid, cudaStream_t st) {
   return launch_dependent(k, grid, AbCfg<DP>::THREADS, AbCfg<DP>::SMEM, st, L);
 }
 
+template <typename T, int DP, bool DKV, int CAP>
+cudaError_t attn_bwd_cap(const AttnBwdLaunch& L, int grid, cudaStream_t st) {
+  const int bias = !L.d.slopes ? 0 : L.d.grid_w > 0 ? 2 : 1;
+  return bias == 0   ? attn_bwd_one<T, DP, DKV, CAP, 0>(L, grid, st)
+         : bias == 1 ? attn_bwd_one<T, DP, DKV, CAP, 1>(L, grid, st)
+                     : attn_bwd_one<T, DP, DKV, CAP, 2>(L, grid, st);
+}
+
 template <typename T, int DP, bool DKV>
 cudaError_t attn_bwd_dp(const AttnBwdLaunch& L, int grid, cudaStream_t st) {
-  const int bias = !L.d.slopes ? 0 : L.d.grid_w > 0 ? 2 : 1;
-  if (L.d.cap > 0.f)
-    return bias == 0   ? attn_bwd_one<T, DP, DKV, true, 0>(L, grid, st)
-           : bias == 1 ? attn_bwd_one<T, DP, DKV, true, 1>(L, grid, st)
-                       : attn_bwd_one<T, DP, DKV, true, 2>(L, grid, st);
-  return bias == 0   ? attn_bwd_one<T, DP, DKV, false, 0>(L, grid, st)
-         : bias == 1 ? attn_bwd_one<T, DP, DKV, false, 1>(L, grid, st)
-                     : attn_bwd_one<T, DP, DKV, false, 2>(L, grid, st);
+  return L.d.cap == 0.f          ? attn_bwd_cap<T, DP, DKV, 0>(L, grid, st)
+         : L.d.cap <= kAtCapLarge ? attn_bwd_cap<T, DP, DKV, 1>(L, grid, st)
+                                  : attn_bwd_cap<T, DP, DKV, 2>(L, grid, st);
 }
 
 template <typename T, bool DKV>

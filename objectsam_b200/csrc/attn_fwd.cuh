@@ -86,7 +86,7 @@ static __device__ __noinline__ AtSplitCta at_split_cta(const AttnFwdLaunch& P, i
   return r;
 }
 
-template <typename T, int DP, bool CAP, int BIAS, bool SPREAD>
+template <typename T, int DP, int CAP, int BIAS, bool SPREAD>
 __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constant__ AttnFwdLaunch P) {
   using Cfg = AfCfg<DP>;
   constexpr bool BF16 = Half16<T>::kBf16;
@@ -301,6 +301,8 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     AtBias bias;
     bias.mul = CAP ? 2.f * A.scale * kAtLog2e / A.cap : A.scale * kAtLog2e;
     bias.cap2 = A.cap * kAtLog2e;
+    bias.lin = A.scale * kAtLog2e;
+    bias.arg = A.scale / A.cap;
     bias.slope = BIAS && valid ? A.slopes[head] * kAtLog2e : 0.f;
     bias.y = bias.x = 0.f;
     if (BIAS == 2) {
@@ -576,7 +578,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   }
 }
 
-template <typename T, int DP, bool CAP, int BIAS, bool SPREAD>
+template <typename T, int DP, int CAP, int BIAS, bool SPREAD>
 cudaError_t attn_fwd_one(const AttnFwdLaunch& L, cudaStream_t st) {
   static bool set[64] = {};  // per device; a race only repeats the call
   int dev = 0;
@@ -591,16 +593,19 @@ cudaError_t attn_fwd_one(const AttnFwdLaunch& L, cudaStream_t st) {
   return launch_dependent(k, L.grid, kAfThreads, AfCfg<DP>::SMEM, st, L);
 }
 
+template <typename T, int DP, int CAP, bool SPREAD>
+cudaError_t attn_fwd_cap(const AttnFwdLaunch& L, cudaStream_t st) {
+  const int bias = !L.d.slopes ? 0 : L.d.grid_w > 0 ? 2 : 1;
+  return bias == 0   ? attn_fwd_one<T, DP, CAP, 0, SPREAD>(L, st)
+         : bias == 1 ? attn_fwd_one<T, DP, CAP, 1, SPREAD>(L, st)
+                     : attn_fwd_one<T, DP, CAP, 2, SPREAD>(L, st);
+}
+
 template <typename T, int DP, bool SPREAD>
 cudaError_t attn_fwd_dp(const AttnFwdLaunch& L, cudaStream_t st) {
-  const int bias = !L.d.slopes ? 0 : L.d.grid_w > 0 ? 2 : 1;
-  if (L.d.cap > 0.f)
-    return bias == 0   ? attn_fwd_one<T, DP, true, 0, SPREAD>(L, st)
-           : bias == 1 ? attn_fwd_one<T, DP, true, 1, SPREAD>(L, st)
-                       : attn_fwd_one<T, DP, true, 2, SPREAD>(L, st);
-  return bias == 0   ? attn_fwd_one<T, DP, false, 0, SPREAD>(L, st)
-         : bias == 1 ? attn_fwd_one<T, DP, false, 1, SPREAD>(L, st)
-                     : attn_fwd_one<T, DP, false, 2, SPREAD>(L, st);
+  return L.d.cap == 0.f          ? attn_fwd_cap<T, DP, 0, SPREAD>(L, st)
+         : L.d.cap <= kAtCapLarge ? attn_fwd_cap<T, DP, 1, SPREAD>(L, st)
+                                  : attn_fwd_cap<T, DP, 2, SPREAD>(L, st);
 }
 
 template <typename T>

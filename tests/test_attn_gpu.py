@@ -408,3 +408,29 @@ def test_size_of_v(cuda_lib, D, dtype, size, mask):
     v *= size
     v[0, 100] = 60000.0
     check(q, k, v, do * (16 if size < 1 else 1 / 64), mask=mask, doc_q=doc_q, doc_k=doc_k)
+
+
+# ---------------------------------------------------------------- large caps
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("cap", [100.0, 150.0, 1e4, 1e7, 3e38])
+@pytest.mark.parametrize("bias", ["none", "line", "grid"])
+def test_large_caps(cuda_lib, D, dtype, cap, bias):
+    """A cap far above the scores leaves them as they are."""
+    H, W = 13, 15
+    q, k, v, do = make(1, H * W, H * W, 4, 2, D, dtype, seed=23)
+    check(q, k, v, do, cap=cap, mask="causal", slopes=None if bias == "none" else slopes_of(4), grid_w=W if bias == "grid" else 0)
+
+
+@pytest.mark.parametrize("cap", [50.0, 128.0, 129.0, 200.0, 1000.0])
+@pytest.mark.parametrize("Lq", [1, 90])
+def test_scores_near_a_large_cap(cuda_lib, cap, Lq):
+    """Scores up to twice the cap and a row's largest just below it: whole products, exact in fp32, so that only the cap's form
+    is in the error (4e-7 of a score of at most 1000: below the 0.3 of a rounding unit that `check` leaves for it with bf16)."""
+    g = torch.Generator().manual_seed(24)
+    Lk, D = 200, 64
+    q = torch.randint(1, 4, (1, Lq, 2, D), generator=g).to(torch.bfloat16).to(DEV)
+    k = torch.randint(-8, 9, (1, Lk, 2, D), generator=g).to(torch.bfloat16).to(DEV)
+    k[0, ::3] = k[0, ::3].abs()
+    v, do = (torch.randn(1, n, 2, D, generator=g).to(torch.bfloat16).to(DEV) for n in (Lk, Lq))
+    check(q, k, v, do, cap=cap, scale=2.0 ** round(math.log2(cap / 500)))
