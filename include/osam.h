@@ -556,7 +556,7 @@ int osam_adamw_destroy(osam_adamw* a);
  * same call serves single tokens over a long cache (few query rows: the keys are split over the GPU and joined).
  *   s_ij = cap·tanh(scale·q_i·k_j/cap)  (cap > 0, of any size: scores far below it stay as they are)   or
  *          scale·q_i·k_j  (cap = 0)
- *   x_ij = s_ij − slopes[head]·dist(i, j)           (slopes NULL: no bias; they get no gradient)
+ *   x_ij = s_ij − slopes[head]·dist(i, j)           (slopes of either sign; NULL: no bias; they get no gradient)
  *   o_i = Σ_j p_ij v_j,  p_ij = exp(x_ij − lse_i),  over the keys that i sees
  * n_b = lens[b] (clamped to 0 … len_k; lens NULL: len_k) keys are in use; query i stands at position
  * i + n_b − len_q, key j at j.  dist = |pos_i − j|, or with grid_w > 0, tokens laid row by row on a map grid_w

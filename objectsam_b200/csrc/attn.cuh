@@ -181,6 +181,7 @@ struct AtBias {
   float cap2;       // cap·log2 e
   float lin, arg;   // CAP = 2: scale·log2 e and scale / cap
   float slope;      // of the row's head, ·log2 e
+  float away;       // −1, or 1 where the slope is negative
   float y, x;       // the row's position on the map times the slope; line: y only, relative to the chunk's first column
 };
 // tanh(y)/y from z = y² < ¼: its Taylor series.
@@ -204,28 +205,38 @@ struct AtLine {
     d[1] = add2(d[1], step);
   }
 };
-// Four consecutive columns; `line` holds their distances (line), ky / kx their cells (grid).  out: the scores plus
-// `add` (ADD); with CAP, sig = 1/(1 + 2^u), from which 1 − tanh² = 4·sig·(1 − sig).
-template <int CAP, int BIAS, bool ADD>
-__device__ __forceinline__ void at_scores4(const AtBias& P, float2 (&s)[2], const float2 (&add)[2], AtLine& line,
-                                           const float4& ky, const float4& kx, float2 (&sig)[2]) {
-  const float2 mul = make_float2(P.mul, P.mul);
-  float2 b[2] = {add[0], add[1]};
+// Distances (times the slope's size) of four consecutive columns: `line` holds them signed, ky / kx the columns' cells (grid).
+template <int BIAS>
+__device__ __forceinline__ void at_far4(const AtBias& P, AtLine& line, const float4& ky, const float4& kx, float2 (&t)[2]) {
   if (BIAS == 1) {
-    const float2 t0 = make_float2(-fabsf(line.d[0].x), -fabsf(line.d[0].y)),
-                 t1 = make_float2(-fabsf(line.d[1].x), -fabsf(line.d[1].y));
-    b[0] = ADD ? make_float2(b[0].x + t0.x, b[0].y + t0.y) : t0;
-    b[1] = ADD ? make_float2(b[1].x + t1.x, b[1].y + t1.y) : t1;
+    t[0] = make_float2(fabsf(line.d[0].x), fabsf(line.d[0].y));
+    t[1] = make_float2(fabsf(line.d[1].x), fabsf(line.d[1].y));
     line.next();
   }
   if (BIAS == 2) {
     const float2 ns = make_float2(-P.slope, -P.slope), y = make_float2(P.y, P.y), x = make_float2(P.x, P.x);
     const float2 y0 = fma2(ns, make_float2(ky.x, ky.y), y), y1 = fma2(ns, make_float2(ky.z, ky.w), y);
     const float2 x0 = fma2(ns, make_float2(kx.x, kx.y), x), x1 = fma2(ns, make_float2(kx.z, kx.w), x);
-    const float2 t0 = make_float2(-fabsf(y0.x) - fabsf(x0.x), -fabsf(y0.y) - fabsf(x0.y)),
-                 t1 = make_float2(-fabsf(y1.x) - fabsf(x1.x), -fabsf(y1.y) - fabsf(x1.y));
-    b[0] = ADD ? add2(b[0], t0) : t0;
-    b[1] = ADD ? add2(b[1], t1) : t1;
+    t[0] = make_float2(fabsf(y0.x) + fabsf(x0.x), fabsf(y0.y) + fabsf(x0.y));
+    t[1] = make_float2(fabsf(y1.x) + fabsf(x1.x), fabsf(y1.y) + fabsf(x1.y));
+  }
+}
+// Four consecutive columns; out: the scores plus `add` (ADD); with CAP, sig = 1/(1 + 2^u), from which 1 − tanh² =
+// 4·sig·(1 − sig).  NEG: slopes may be negative; without, the sign rides on the operand.
+template <int CAP, int BIAS, bool ADD, bool NEG>
+__device__ __forceinline__ void at_scores4(const AtBias& P, float2 (&s)[2], const float2 (&add)[2], AtLine& line,
+                                           const float4& ky, const float4& kx, float2 (&sig)[2]) {
+  const float2 mul = make_float2(P.mul, P.mul);
+  float2 b[2] = {add[0], add[1]};
+  if (BIAS) {
+    float2 t[2];
+    at_far4<BIAS>(P, line, ky, kx, t);
+    const float2 away = make_float2(P.away, P.away);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const float2 a = NEG ? mul2(t[i], away) : make_float2(-t[i].x, -t[i].y);
+      b[i] = !ADD ? a : NEG ? fma2(t[i], away, b[i]) : add2(b[i], a);
+    }
   }
   if (CAP) {
     sig[0] = mul2(s[0], mul);

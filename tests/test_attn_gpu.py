@@ -434,3 +434,17 @@ def test_scores_near_a_large_cap(cuda_lib, cap, Lq):
     k[0, ::3] = k[0, ::3].abs()
     v, do = (torch.randn(1, n, 2, D, generator=g).to(torch.bfloat16).to(DEV) for n in (Lk, Lq))
     check(q, k, v, do, cap=cap, scale=2.0 ** round(math.log2(cap / 500)))
+
+
+# ---------------------------------------------------------------- slopes of either sign
+@pytest.mark.parametrize("cap", [0.0, 20.0, 1e4])
+@pytest.mark.parametrize("bias", ["line", "grid"])
+@pytest.mark.parametrize("mask", ["none", "prefix"])
+@pytest.mark.parametrize("Lq", [3, 195])
+def test_slopes_of_either_sign(cuda_lib, cap, bias, mask, Lq):
+    """A negative slope favours distant keys: s − slope·distance as it stands."""
+    H, W = 13, 15
+    q, k, v, do = make(2, Lq, H * W, 4, 2, 64, seed=25)
+    slopes = torch.tensor([-0.06, 0.11, 0.0, -0.01], device=DEV)
+    check(q, k, v, do, cap=cap, mask=mask, slopes=slopes, grid_w=W if bias == "grid" else 0,
+          prefix=torch.tensor([0, 150], dtype=torch.int32, device=DEV) if mask == "prefix" else None)
