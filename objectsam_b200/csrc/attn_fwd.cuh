@@ -6,7 +6,7 @@
 // Per 64-key tile:  S = Q·Kᵀ (tcgen05, fp32 in TMEM) → two threads per row read 32 scores each into registers, apply cap,
 // bias and masks, take p = 2^(x − m) against the row's reference maximum m and write P in 16 bits back to TMEM → O +=
 // P·V with P as the TMEM operand.  A row is a TMEM lane: its maximum and sum need no shuffles.  m follows the maximum
-// only when a tile exceeds it by more than 2^8 (P ≤ 2^8 keeps its relative precision in 16 bits, the sum is fp32):
+// only when a tile exceeds it by more than 2^8 (P, fp16's held times 2^7, stays in range, the sum is fp32):
 // then the row's two threads agree on it and O, which stays in TMEM, is rescaled; otherwise one flag barrier of the
 // two warps tells that nothing is to do.  Tiles are visited from the CTA's own positions outwards, so that with a
 // distance bias the largest scores come first and this stays rare.
@@ -29,6 +29,7 @@ namespace osam {
 constexpr int kAfSoft = 256;    // softmax threads
 constexpr int kAfThreads = kAfSoft + 64;
 constexpr float kAfGrow = 8.f;  // log2 growth over a row's reference maximum that forces a rescale
+constexpr float kAfUp = 7.f;    // fp16: P is held times 2^7 (at most 2^15), so weights down to 2^-31 of the reference enter O
 
 template <int DP>
 struct AfCfg {
@@ -93,6 +94,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
   using Cfg = AfCfg<DP>;
   constexpr bool BF16 = Half16<T>::kBf16;
   constexpr int KEYS = kAfKeys, N = SPREAD ? 8 : 32;  // N: columns of a thread
+  constexpr float up = BF16 ? 0.f : kAfUp;
   extern __shared__ uint8_t af_raw[];
   __shared__ __align__(8) uint64_t k_full[Cfg::STAGES], k_empty[Cfg::STAGES], v_full[Cfg::STAGES], v_empty[Cfg::STAGES];
   __shared__ __align__(8) uint64_t s_full, s_free, p_full[2], pv_done, o_done;
@@ -313,8 +315,8 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       bias.x = cell.y * bias.slope;
     }
     float m = -INFINITY;  // the row's reference maximum, log2 units (−∞: nothing seen yet)
-    float neg = 0.f;      // −m, or 0 while there is none
-    float l = 0.f;        // this thread's part of its sum
+    float neg = 0.f;      // up − m, or 0 while there is none
+    float l = 0.f;        // this thread's part of its sum (of P as it is held)
     float l16 = 0.f;      // SPREAD: the same of P as the tensor cores read it, rounded to 16 bits
     const uint32_t bar_s = smem_u32(&s_full), bar_free = smem_u32(&s_free), bar_p = smem_u32(&p_full[0]);
     const int c1 = h0 + (SPREAD ? 8 * (warp % 4) : 0);  // first column of this thread
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
         if (top > m + kAfGrow) {
           f = m == -INFINITY ? 0.f : at_ex2(m - top);
           m = top;
-          neg = -m;
+          neg = up - m;
           l *= f;
           l16 *= f;
         }
@@ -513,6 +515,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       m = M;
     }
     if (ok) {
+      m -= up;  // from here on l's reference
       const long long row = ((long long)b * A.Hq + head) * A.Lq + qi;
       const long long part_row = (long long)split * A.B * A.Hq * A.Lq + row;
       T* o_ptr = static_cast<T*>(P.o.p) + b * P.o.sb + qi * P.o.st + head * P.o.sh;

@@ -448,3 +448,18 @@ def test_slopes_of_either_sign(cuda_lib, cap, bias, mask, Lq):
     slopes = torch.tensor([-0.06, 0.11, 0.0, -0.01], device=DEV)
     check(q, k, v, do, cap=cap, mask=mask, slopes=slopes, grid_w=W if bias == "grid" else 0,
           prefix=torch.tensor([0, 150], dtype=torch.int32, device=DEV) if mask == "prefix" else None)
+
+
+@pytest.mark.parametrize("Lq", [1, 40, 200])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_many_small_weights(cuda_lib, Lq, dtype):
+    """One key of weight 1 with v = 0 and 700 of weight 2^-26 with v = 60000: o is what the small ones add up to.  The weights
+    are powers of two that fp16 holds with a shift of 2^2 and more, so o's rounding is the only one, and 2^-11 covers the
+    score's (−26·ln 2·log2 e, off by 2^-23 of 26)."""
+    D, N = 8, 700
+    q, k, v = (torch.zeros(1, n, 1, D, dtype=dtype, device=DEV) for n in (Lq, N + 1, N + 1))
+    q[..., 0], k[:, 1:, :, 0], v[:, 1:] = 1.0, -26.0, 60000.0
+    out = run(q, k, v, None, train=False, scale=math.log(2.0))
+    want = float(v[0, 1, 0, 0]) * N * 2.0 ** -26 / (1 + N * 2.0 ** -26)
+    assert ((out["o"].double() - want).abs() <= (UNIT[dtype] + 2.0 ** -11) * want).all(), (out["o"].double().mean().item(), want)
+    assert (out["lse"].double() - math.log(1 + N * 2.0 ** -26)).abs().max() <= 2.0 ** -20
