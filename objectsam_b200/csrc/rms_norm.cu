@@ -150,6 +150,13 @@ __global__ void __launch_bounds__(kRmsThreads) k_rms_fwd(const RmsFwd P) {
         const float other = __shfl_xor_sync(0xffffffffu, top, o);
         top = (top != top || other != other) ? __int_as_float(0x7fffffff) : fmaxf(top, other);
       }
+      // 448/top is not finite below 2^-119: such a group is brought up by a power of two first, its scale left as it is
+      const float scale = top / kE4m3Max;
+      if (top < 0x1p-100f) {
+        top *= 0x1p100f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] *= 0x1p100f;
+      }
       const float inv = top > 0.f ? kE4m3Max / top : (top == 0.f ? 0.f : top);
       if (live && v < C8) {
         uint2 u;
@@ -158,7 +165,7 @@ __global__ void __launch_bounds__(kRmsThreads) k_rms_fwd(const RmsFwd P) {
         for (int i = 0; i < 4; i++)
           q[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i] * inv, y[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(P.y) + row * P.ldy + v * 8) = u;
-        if (v % 16 == 0) P.qscale[row * P.groups + v / 16] = top / kE4m3Max;
+        if (v % 16 == 0) P.qscale[row * P.groups + v / 16] = scale;
       }
     }
   }

@@ -169,3 +169,24 @@ def test_empty_and_many(cuda_lib):
     norm.rms_norm_fwd(x, torch.ones(C, device=DEV), EPS, x)
     tail = x[-3:].double()
     assert ((tail * tail).mean(1) - 1).abs().max() < 1e-2 and not x[:8].any()
+
+
+@pytest.mark.parametrize("C", [128, 264, 2048])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_vanishing_groups(cuda_lib, C, dtype):
+    """A group whose largest |y| is near fp32's smallest normal number keeps its values' proportions, and its zeros; y there is
+    ±2^-125·rstd and halves of it, normal numbers, so q is off by e4m3's half step and the scale by its own subnormal step."""
+    from objectsam_b200 import norm
+    x = torch.randn(5, C, device=DEV).to(dtype)
+    w = torch.ones(C, device=DEV)
+    part = torch.tensor([1.0, 0.0, -0.5, 0.25], device=DEV).repeat(32)
+    x[:, :128] = part.to(dtype)
+    x[:, 128:] *= 0.25
+    w[:128] = 2.0 ** -124
+    q, qs = torch.empty(5, C, dtype=torch.float8_e4m3fn, device=DEV), torch.empty(5, -(-C // 128), device=DEV)
+    norm.rms_norm_fwd_q8(x, w, EPS, q, qs)
+    assert torch.isfinite(q.float()).all()
+    got, want = q[:, :128].double(), 448.0 * part.double()
+    assert ((got - want).abs() <= 2.0 ** -4 * want.abs()).all()
+    rstd = torch.rsqrt(x.double().square().mean(1) + EPS)
+    assert ((qs[:, 0].double() - 2.0 ** -124 * rstd / 448).abs() <= 2.0 ** -149).all()
