@@ -563,8 +563,8 @@ int osam_adamw_destroy(osam_adamw* a);
  * wide, |y_i − y_j| + |x_i − x_j|.  i sees j < n_b when, by `mask`, OSAM_ATTN_NONE: always; CAUSAL: j ≤ pos_i;
  * PREFIX: j ≤ pos_i or j < prefix[b]; and with documents (doc_q [batch][len_q] and doc_k [batch][len_k], both or
  * neither) doc_q[i] = doc_k[j] ≥ 0: a token with a negative id sees nothing and is seen by none.  A query that
- * sees nothing gets o = 0, lse = −∞ and gives no gradient.  Contents of K and V rows past n_b or of tokens without
- * a document do not matter (NaN included).
+ * sees nothing gets o = 0, lse = −∞ and gives no gradient.  Contents of K and V rows past n_b, of tokens without a
+ * document, and of q and dO rows that see nothing do not matter (NaN included).
  * Query head h reads key head h / (heads_q / heads_k).  Tensors are dtype (OSAM_F16 / OSAM_BF16), [batch][token]
  * [head][dim] by element strides with dim contiguous; strides multiples of 8 and not 0 (where the extent is
  * above 1), 16-byte aligned; dim a multiple of 8, 8 … 128.  With documents len_q and len_k ≤ 1048576.

@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(256) k_attn_sum(const float* part, int parts, 
 // use.  One CTA per block, 16 lanes per row (a 16-byte vector each).
 template <typename T>
 __global__ void __launch_bounds__(256) k_attn_rows(const __grid_constant__ AttnDev A, const AtView o, const AtView dout,
-                                                   const AtView v, const float* lse, float* rows, float* peak, float* vpeak) {
+                                                   const AtView v, const float* lse, float* rows, float* peak, float* vpeak,
+                                                   AtDocs* sum_q) {
   __shared__ float top[8];
   constexpr bool BF16 = Half16<T>::kBf16;
   constexpr float up = BF16 ? 0.f : kAbUp;
@@ -156,7 +157,8 @@ __global__ void __launch_bounds__(256) k_attn_rows(const __grid_constant__ AttnD
   grid_dep_wait();
   grid_dep_launch();
   const int n = keys ? at_keys(A, b) : 0;
-  float big = 0.f;  // largest ‖·‖²
+  float big = 0.f;     // largest ‖·‖²
+  bool blind = false;  // a query that sees nothing: the same in all heads
 #pragma unroll
   for (int k = 0; k < kAbCols; k += 16) {
     const int r = k + threadIdx.x / 16, i = blk * kAbCols + r;
@@ -167,6 +169,7 @@ __global__ void __launch_bounds__(256) k_attn_rows(const __grid_constant__ AttnD
     } else {
       if (i < A.Lq) L = lse[bh * A.Lq + i];
       live = L != -INFINITY;
+      blind |= i < A.Lq && !live;
     }
     const AtView& t = keys ? v : dout;
     float d = 0.f, s2 = 0.f;
@@ -194,6 +197,7 @@ __global__ void __launch_bounds__(256) k_attn_rows(const __grid_constant__ AttnD
       out[kAbCols] = live ? -d : 0.f;
     }
   }
+  if (sum_q && !keys && h == 0 && blind && c == 0) sum_q[(long long)b * nq + blk].pad = 1;
   if (BF16) return;
   big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
   if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = big;
@@ -470,7 +474,8 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   if (blocks > 0) {
     const unsigned grid = blocks + (bf16 ? 0u : (unsigned)a->batch * a->heads_k * ((a->len_k + kAbCols - 1) / kAbCols));
     if ((rc = at_cuda(launch_dependent(bf16 ? k_attn_rows<__nv_bfloat16> : k_attn_rows<__half>, grid, 256, 0, st, L.d, at_view(o),
-                                       at_view(dout), at_view(v), lse, rows, peak, vpeak),
+                                       at_view(dout), at_view(v), lse, rows, peak, vpeak,
+                                       a->doc_q ? reinterpret_cast<AtDocs*>(w + W.sum_q) : (AtDocs*)nullptr),
                       "row terms")) != OSAM_OK)
       return rc;
   }

@@ -32,7 +32,8 @@ struct AtView {
   long long sb, st, sh;
 };
 
-// Documents of 64 tokens: the smallest and largest id ≥ 0 (lo > hi: none) and whether a token has none (id < 0).
+// Documents of 64 tokens: the smallest and largest id ≥ 0 (lo > hi: none) and whether a token has none (id < 0) or, for the
+// backward's queries, sees nothing.
 struct AtDocs {
   int lo, hi, pad, unused;
 };

@@ -395,10 +395,9 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
       if (DKV) tmem_st16(xcol + h0, pp);  // over the scores that this thread has read
       tmem_st16(xcol + 64 + h0, dd);
       // streamed rows that nothing sees hold anything, NaN included: 0·NaN must not enter the sums
-      if (has_pad || (!DKV && n < A.Lk && c0 + kAbCols > n)) {
+      if (has_pad || (DKV ? causal && c0 < -off : n < A.Lk && c0 + kAbCols > n)) {
         const int c = c0 + r % kAbCols, panel = half;
-        const bool dead = DKV ? c < A.Lq && A.doc_q[(long long)b * A.Lq + c] < 0
-                              : c >= n || (docs && A.doc_k[(long long)b * A.Lk + c] < 0);
+        const bool dead = DKV ? rows[r % kAbCols - h0] == -INFINITY : c >= n || (docs && A.doc_k[(long long)b * A.Lk + c] < 0);
         if (ok && dead && panel < Cfg::PANELS) {
           uint8_t* d = strm + s * 2 * Cfg::STRM + (r / kAbCols) * Cfg::STRM + panel * kAbCols * 128 + (r % kAbCols) * 128;
 #pragma unroll

@@ -463,3 +463,23 @@ def test_many_small_weights(cuda_lib, Lq, dtype):
     want = float(v[0, 1, 0, 0]) * N * 2.0 ** -26 / (1 + N * 2.0 ** -26)
     assert ((out["o"].double() - want).abs() <= (UNIT[dtype] + 2.0 ** -11) * want).all(), (out["o"].double().mean().item(), want)
     assert (out["lse"].double() - math.log(1 + N * 2.0 ** -26)).abs().max() <= 2.0 ** -20
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("mask", ["causal", "prefix"])
+def test_contents_of_queries_that_see_nothing(cuda_lib, D, dtype, mask):
+    """Queries in front of the first key (fewer keys than queries), or of a document that no key has: q and dO may hold NaN or
+    infinities there, and the keys' gradients are those of the other queries."""
+    lens = torch.tensor([150, 3, 0, 90], dtype=torch.int32, device=DEV)
+    B, Lq, Lk = len(lens), 150, 160
+    q, k, v, do = make(B, Lq, Lk, 4, 2, D, dtype, seed=26)
+    for b, n in enumerate(lens.tolist()):
+        q[b, :Lq - n] = float("nan")
+        do[b, :Lq - n] = float("inf")
+    check(q, k, v, do, mask=mask, lens=lens, prefix=torch.zeros(B, dtype=torch.int32, device=DEV) if mask == "prefix" else None)
+    q, k, v, do = make(1, Lq, Lk, 4, 2, D, dtype, seed=27)
+    dq, dk = (torch.arange(n, dtype=torch.int32, device=DEV).div(40, rounding_mode="floor").int()[None].contiguous() for n in (Lq, Lk))
+    dq[0, 20:30], dq[0, 70:100] = 77, 78
+    q[0, 20:30], do[0, 70:100] = float("nan"), float("nan")
+    check(q, k, v, do, doc_q=dq, doc_k=dk)
