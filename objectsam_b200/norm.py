@@ -31,17 +31,19 @@ def _rows(t, shape, dtype, name: str):
     stride = t.stride()
     if stride[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name}: channels are contiguous")
-    ld = n = 0
+    ld, n = None, 1
     for size, step in zip(shape[-2::-1], stride[-2::-1]):
         if size == 1:
             continue
-        if not ld:
+        if ld is None:
             ld, n = step, size
+            if ld < shape[-1]:  # a row repeated by broadcasting, too: stride 0
+                raise ValueError(f"{name}: rows do not overlap")
         elif step != ld * n:
             raise ValueError(f"{name}: rows are equally spaced")
         else:
             n *= size
-    return t.data_ptr(), ld or shape[-1]
+    return t.data_ptr(), shape[-1] if ld is None else ld
 
 
 def _f32(t, n: int, name: str):

@@ -152,3 +152,34 @@ def test_reference_rms_gradients():
     up, down = token_ref.rms_norm(x + eps * dx, w + eps * dw, 1e-5)["y"], token_ref.rms_norm(x - eps * dx, w - eps * dw, 1e-5)["y"]
     got = ((up - down) * dy).sum() / (2 * eps)
     assert abs(got - (out["dx"] * dx).sum() - (out["dw"] * dw).sum()) < 1e-7
+
+
+class Strided:
+    """A CUDA tensor's shape and strides, as the argument checks see them."""
+    dtype, is_cuda = torch.float16, True
+
+    def __init__(self, t):
+        self.t, self.shape = t, t.shape
+
+    def is_contiguous(self):
+        return self.t.is_contiguous()
+
+    def stride(self):
+        return self.t.stride()
+
+    def data_ptr(self):
+        return 4096
+
+
+def test_rows_of_a_norm():
+    """Rows are taken by one distance from row to row; a row that broadcasting repeats has none."""
+    from objectsam_b200 import norm
+    base = torch.zeros(6, 10, 96, dtype=torch.float16)
+    rows = lambda t: norm._rows(Strided(t), t.shape, torch.float16, "x")  # noqa: E731
+    assert rows(base) == (4096, 96) and rows(base[..., 16:80]) == (4096, 96) and rows(base[:, 3:4, :32]) == (4096, 960)
+    assert rows(base[:1, :1]) == (4096, 96) and rows(base[:, ::2, :64]) == (4096, 192)
+    row = torch.zeros(1, 64, dtype=torch.float16)
+    for bad in (row.expand(8, 64), base[:, :1].expand(6, 10, 96), base[:1].expand(6, 10, 96), base[:, :5], base[..., :64].as_strided((5, 64), (32, 1)),
+                base.transpose(1, 2)):
+        with pytest.raises(ValueError):
+            rows(bad)
