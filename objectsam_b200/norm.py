@@ -83,15 +83,16 @@ def rms_norm_fwd_q8(x, w, eps: float, q, qscale, res=None, total=None, rstd=None
 
 
 def workspace(C: int, device, stream=None) -> torch.Tensor:
-    """The backward's workspace for C channels, one per (device, stream)."""
+    """The backward's workspace for C channels, one per (device, stream, size).  None is ever replaced: a captured graph may
+    hold its address."""
     dev = torch.device(device)
     s = stream if stream is not None else torch.cuda.current_stream(dev)
-    nbytes = int(lib().osam_rms_bwd_workspace_size(C))
-    key = (dev.index, s.cuda_stream)
+    nbytes = max(int(lib().osam_rms_bwd_workspace_size(C)), 1 << 20)
+    key = (dev.index, s.cuda_stream, nbytes)
     buf = _ws_cache.get(key)
-    if buf is None or buf.numel() < nbytes:
+    if buf is None:
         with torch.cuda.stream(s):
-            buf = _ws_cache[key] = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=dev)
+            buf = _ws_cache[key] = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     return buf
 
 

@@ -190,3 +190,32 @@ def test_vanishing_groups(cuda_lib, C, dtype):
     assert ((got - want).abs() <= 2.0 ** -4 * want.abs()).all()
     rstd = torch.rsqrt(x.double().square().mean(1) + EPS)
     assert ((qs[:, 0].double() - 2.0 ** -124 * rstd / 448).abs() <= 2.0 ** -149).all()
+
+
+def test_captured_backward_keeps_its_workspace(cuda_lib):
+    """A graph holds the address of the workspace that the norm keeps for its stream: wider calls on that stream take others."""
+    from objectsam_b200 import norm
+    g = torch.Generator(device=DEV).manual_seed(6)
+    s = torch.cuda.Stream()
+
+    def case(C):
+        dy, x = (torch.randn(700, C, generator=g, device=DEV).half() for _ in range(2))
+        return dy, x, torch.ones(C, device=DEV), torch.rand(700, device=DEV), torch.empty_like(x), torch.empty(C, device=DEV)
+
+    small, large = case(64), case(8192)
+    norm.rms_norm_bwd(*small)
+    want = small[4].clone(), small[5].clone()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        norm.rms_norm_bwd(*small)
+        held = norm.workspace(64, DEV)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            norm.rms_norm_bwd(*small)
+        for _ in range(2):
+            norm.rms_norm_bwd(*large)
+            assert norm.workspace(64, DEV) is held and norm.workspace(8192, DEV) is not held
+            small[4].zero_(), small[5].zero_()
+            graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(small[4], want[0]) and torch.equal(small[5], want[1])
