@@ -9,7 +9,7 @@ backward, and single tokens over a long cache (osam_attn_fwd / osam_attn_bwd in 
 Tensors are (batch, tokens, heads, dim) CUDA tensors of the plan's type with dim contiguous: slices of a fused
 projection (batch, tokens, (q, k, v) heads, dim) and of a cache are taken as they lie.  slopes, lens, prefix and
 the document ids are device tensors that the plan keeps and every call reads anew.  Without `ws` the plan makes
-one per stream and keeps it.
+one per device and stream and keeps it.
 """
 from __future__ import annotations
 
@@ -92,11 +92,11 @@ class AttnOp:
     def _workspace(self, ws, stream):
         if ws is None:
             s = stream if stream is not None else torch.cuda.current_stream()
-            ws = self._ws.get(s.cuda_stream)
+            key = s.device.index, s.cuda_stream  # the default stream's handle is 0 on every device
+            ws = self._ws.get(key)
             if ws is None:
                 with torch.cuda.stream(s):
-                    ws = self._ws[s.cuda_stream] = torch.empty(max(self._ws_bytes, 256), dtype=torch.uint8,
-                                                               device=torch.device("cuda", torch.cuda.current_device()))
+                    ws = self._ws[key] = torch.empty(max(self._ws_bytes, 256), dtype=torch.uint8, device=s.device)
         return ws.data_ptr(), ws.numel() * ws.element_size()
 
     def _lse(self, lse):

@@ -483,3 +483,20 @@ def test_contents_of_queries_that_see_nothing(cuda_lib, D, dtype, mask):
     dq[0, 20:30], dq[0, 70:100] = 77, 78
     q[0, 20:30], do[0, 70:100] = float("nan"), float("nan")
     check(q, k, v, do, doc_q=dq, doc_k=dk)
+
+
+def test_without_a_workspace(cuda_lib):
+    """The plan's own workspace, on the current stream and on another, forward and backward."""
+    from objectsam_b200.attn import AttnGeom, AttnOp
+    q, k, v, do = make(2, 40, 900, 4, 2, 64, seed=28)
+    want = run(q, k, v, do, mask="causal")
+    op = AttnOp().init(AttnGeom(2, 40, 900, 4, 2, 64), mask="causal")
+    for s in (None, torch.cuda.Stream()):
+        out = {n: torch.full_like(t, float("nan")) for n, t in want.items()}
+        torch.cuda.synchronize()
+        op.fwd(q, k, v, out["o"], out["lse"], stream=s)
+        op.bwd(q, k, v, out["o"], out["lse"], do, out["dq"], out["dk"], out["dv"], stream=s)
+        torch.cuda.synchronize()
+        for n in want:
+            assert torch.equal(out[n], want[n]), n
+    assert len(op._ws) == 2

@@ -183,3 +183,20 @@ def test_rows_of_a_norm():
                 base.transpose(1, 2)):
         with pytest.raises(ValueError):
             rows(bad)
+
+
+def test_kept_workspaces_go_by_device_and_stream(monkeypatch):
+    """The default stream has the same handle on every device."""
+    import contextlib
+    from types import SimpleNamespace
+
+    from objectsam_b200.attn import AttnGeom, AttnOp
+    op = AttnOp().init(AttnGeom(1, 4, 4, 1, 1, 64))
+    made = []
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch, "empty", lambda n, dtype, device: made.append(device) or
+                        SimpleNamespace(data_ptr=lambda at=len(made): at, numel=lambda: n, element_size=lambda: 1))
+    streams = [SimpleNamespace(device=torch.device("cuda", d), cuda_stream=h) for d, h in ((0, 0), (1, 0), (1, 7))]
+    got = [op._workspace(None, s) for s in streams + streams]
+    assert [p for p, _ in got] == [1, 2, 3] * 2 and [d.index for d in made] == [0, 1, 1]
