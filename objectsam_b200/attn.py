@@ -97,6 +97,8 @@ class AttnOp:
             if ws is None:
                 with torch.cuda.stream(s):
                     ws = self._ws[key] = torch.empty(max(self._ws_bytes, 256), dtype=torch.uint8, device=s.device)
+        elif not ws.is_cuda or not ws.is_contiguous():
+            raise ValueError("workspace: a contiguous CUDA tensor expected")
         return ws.data_ptr(), ws.numel() * ws.element_size()
 
     def _lse(self, lse):

@@ -101,7 +101,10 @@ def rms_norm_bwd(dy, h, w, rstd, dx, dw, dtotal=None, ws=None, stream=None) -> N
     residual path."""
     code, dtype, shape, C, rows = _in(dy)
     d = (None, 0) if dtotal is None else _rows(dtotal, shape, dtype, "dtotal")
-    ws = ws if ws is not None else workspace(C, dy.device, stream)
+    if ws is None:
+        ws = workspace(C, dy.device, stream)
+    elif not ws.is_cuda or not ws.is_contiguous():
+        raise ValueError("ws: a contiguous CUDA tensor expected")
     check(lib().osam_rms_bwd(code, *_rows(dy, shape, dtype, "dy"), *_rows(h, shape, dtype, "h"), _f32(w, C, "w"),
                              _f32(rstd, rows, "rstd"), *d, rows, C, *_rows(dx, shape, dtype, "dx"), _f32(dw, C, "dw"),
                              ws.data_ptr(), ws.numel() * ws.element_size(), stream_ptr(stream)))

@@ -200,3 +200,22 @@ def test_kept_workspaces_go_by_device_and_stream(monkeypatch):
     streams = [SimpleNamespace(device=torch.device("cuda", d), cuda_stream=h) for d, h in ((0, 0), (1, 0), (1, 7))]
     got = [op._workspace(None, s) for s in streams + streams]
     assert [p for p, _ in got] == [1, 2, 3] * 2 and [d.index for d in made] == [0, 1, 1]
+
+
+def test_workspaces_are_looked_at():
+    """A workspace in host memory, or one with gaps, is refused before anything is launched."""
+    from types import SimpleNamespace
+
+    from objectsam_b200 import norm
+    from objectsam_b200.attn import AttnGeom, AttnOp
+    op = AttnOp().init(AttnGeom(1, 4, 4, 1, 1, 64))
+    flat = torch.zeros(op.workspace_size() * 2, dtype=torch.uint8)
+    gaps = SimpleNamespace(is_cuda=True, is_contiguous=lambda: False)
+    dy = torch.zeros(4, 64, dtype=torch.float16)
+    for ws in (flat, gaps):
+        with pytest.raises(ValueError, match="workspace"):
+            op.fwd(None, None, None, None, ws=ws)
+        with pytest.raises(ValueError, match="workspace"):
+            op.bwd(None, None, None, None, None, None, None, None, None, ws=ws)
+        with pytest.raises(ValueError, match="ws"):
+            norm.rms_norm_bwd(dy, dy, None, None, dy, None, ws=ws)
