@@ -577,7 +577,7 @@ typedef struct osam_attn_desc {
   int dtype, batch, len_q, len_k, heads_q, heads_k, dim;
   int mask;             /* OSAM_ATTN_* */
   float scale, cap;     /* scale > 0; cap 0: uncapped */
-  int grid_w;           /* 0: distance along the sequence */
+  int grid_w;           /* 0: distance along the sequence; at most 2^30 */
   const float* slopes;  /* [heads_q], device */
   const int* lens;      /* [batch], device */
   const int* prefix;    /* [batch], device; needed by OSAM_ATTN_PREFIX */

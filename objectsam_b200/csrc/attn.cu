@@ -231,11 +231,12 @@ int at_check(const osam_attn_desc* a) {
   if (a->mask == OSAM_ATTN_PREFIX && !a->prefix) return at_fail(OSAM_ERR_INVALID, "a prefix mask needs prefix lengths");
   if ((a->doc_q == nullptr) != (a->doc_k == nullptr)) return at_fail(OSAM_ERR_INVALID, "doc_q and doc_k come together");
   if (a->grid_w < 0) return at_fail(OSAM_ERR_INVALID, "grid_w is not negative");
-  const long long most = 1LL << 30;
-  if ((long long)a->len_q * (a->heads_q / a->heads_k) > most || a->len_k > most ||
-      (long long)a->batch * a->heads_q * ((a->len_q + 63) / 64) > most ||
-      (long long)a->batch * a->heads_k * ((a->len_k + 63) / 64) > most)
+  // in doubles: exact up to here, and products of any descriptions stay in range
+  const double most = 1 << 30, B = a->batch, q64 = std::ceil(a->len_q / 64.), k64 = std::ceil(a->len_k / 64.);
+  if ((double)a->len_q * (a->heads_q / a->heads_k) > most || a->len_k > most || B * a->heads_q * q64 > most ||
+      B * a->heads_k * k64 > most)
     return at_fail(OSAM_ERR_INVALID, "too many tokens");
+  if (a->grid_w > most) return at_fail(OSAM_ERR_INVALID, "grid_w is at most 2^30");
   if (a->doc_q && (a->len_q > 1048576 || a->len_k > 1048576))
     return at_fail(OSAM_ERR_INVALID, "with documents at most 1048576 tokens");
   return OSAM_OK;

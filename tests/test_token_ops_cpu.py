@@ -219,3 +219,16 @@ def test_workspaces_are_looked_at():
             op.bwd(None, None, None, None, None, None, None, None, None, ws=ws)
         with pytest.raises(ValueError, match="ws"):
             norm.rms_norm_bwd(dy, dy, None, None, dy, None, ws=ws)
+
+
+@pytest.mark.parametrize("kw", [dict(batch=1 << 30, heads_q=1 << 30, heads_k=1 << 30, len_q=1 << 10, len_k=1 << 10),
+                                dict(batch=1 << 16, heads_q=1 << 16, heads_k=1 << 16, len_q=1, len_k=1 << 30),
+                                dict(batch=(1 << 31) - 1, heads_q=(1 << 31) - 1, heads_k=(1 << 31) - 1, len_q=1, len_k=1),
+                                dict(batch=1 << 20, heads_q=1 << 20, heads_k=1 << 20, len_q=1 << 30, len_k=0),
+                                dict(grid_w=(1 << 30) + 1), dict(grid_w=(1 << 31) - 1)])
+def test_descriptions_past_any_size(kw):
+    """Products that wrap in 64 bits are too large, not small."""
+    import ctypes
+    d = desc(**kw)
+    assert lib().osam_attn_workspace_size(ctypes.byref(d)) == 0
+    assert fwd(d) == INVALID and (b"too many tokens" in lib().osam_last_error() or b"grid_w" in lib().osam_last_error())
