@@ -42,6 +42,7 @@ namespace {
 constexpr int kAdThreads = 256;
 constexpr int kAdChunk = kAdThreads * 8;  // elements per CTA
 constexpr int kAdBlock = 256;             // elements per quantisation scale (one warp)
+constexpr long long kAdMaxElems = 0x7fffffffLL * kAdChunk;  // of a grid's CTAs; below, the layouts' sums stay in range
 constexpr int kAdNormCtas = 148 * 8;
 constexpr float kE4m3Max = 448.f;
 constexpr float kTiny = 1e-30f;           // a block whose maximum is below this is stored as zeros
@@ -427,6 +428,7 @@ int ad_check(const osam_adamw_tensor* t, int n, int bits) {
   if (n < 0 || (n > 0 && !t)) return ad_fail(OSAM_ERR_INVALID, "adamw: no tensors");
   long long chunks = 0;
   for (int i = 0; i < n; i++) {
+    if (t[i].n > kAdMaxElems) return ad_fail(OSAM_ERR_INVALID, "adamw: too many elements");
     if (t[i].n < 0 || (t[i].n > 0 && (!t[i].p || !t[i].g)))
       return ad_fail(OSAM_ERR_INVALID, "adamw: null parameter or gradient");
     if (t[i].grad_type != OSAM_F32 && t[i].grad_type != OSAM_F16 && t[i].grad_type != OSAM_BF16)

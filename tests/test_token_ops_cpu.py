@@ -232,3 +232,15 @@ def test_descriptions_past_any_size(kw):
     d = desc(**kw)
     assert lib().osam_attn_workspace_size(ctypes.byref(d)) == 0
     assert fwd(d) == INVALID and (b"too many tokens" in lib().osam_last_error() or b"grid_w" in lib().osam_last_error())
+
+
+@pytest.mark.parametrize("sizes", [[(1 << 63) - 1], [1 << 62] * 3, [(1 << 63) - 2000] * 2, [1 << 43], [1 << 41] * 4])
+def test_adamw_over_any_number_of_elements(sizes):
+    """Sizes whose layout would wrap are refused, by the sizes' call and by the plan's, which would else ask for memory by them."""
+    import ctypes
+    L, tab = lib(), (AdamWTensor * len(sizes))(*(AdamWTensor(4096, 4096, None, n, _lib.F32, _lib.F16, 1) for n in sizes))
+    nbytes, elems, plan = ctypes.c_size_t(7), ctypes.c_int64(7), ctypes.c_void_p()
+    assert L.osam_adamw_sizes(tab, len(sizes), 8, ctypes.byref(nbytes), ctypes.byref(elems)) == INVALID
+    assert b"too many" in L.osam_last_error() and nbytes.value == 7
+    assert L.osam_adamw_create(tab, len(sizes), 8, 4096, (1 << 64) - 1, None, ctypes.byref(plan)) == INVALID and not plan
+    assert b"too many" in L.osam_last_error()
