@@ -576,7 +576,7 @@ enum { OSAM_ATTN_NONE = 0, OSAM_ATTN_CAUSAL = 1, OSAM_ATTN_PREFIX = 2 };
 typedef struct osam_attn_desc {
   int dtype, batch, len_q, len_k, heads_q, heads_k, dim;
   int mask;             /* OSAM_ATTN_* */
-  float scale, cap;     /* scale > 0; cap 0: uncapped */
+  float scale, cap;     /* scale > 0; cap 0: uncapped, else scale/cap < 1e38 */
   int grid_w;           /* 0: distance along the sequence; at most 2^30 */
   const float* slopes;  /* [heads_q], device */
   const int* lens;      /* [batch], device */

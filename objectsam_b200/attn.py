@@ -50,6 +50,8 @@ class AttnOp:
         and doc_k (batch, len_k): int32."""
         if g.dtype not in _DTYPE:
             raise ValueError("attention takes float16 or bfloat16")
+        if cap > 0 and not ctypes.c_float(cap).value:
+            raise ValueError("cap is below float32's range: it would be taken as none")
         if mask not in _MASK:
             raise ValueError(f"mask is one of {sorted(_MASK)}")
         for name, t, dtype, shape in (("slopes", slopes, torch.float32, (g.heads_q,)),

@@ -226,6 +226,8 @@ int at_check(const osam_attn_desc* a) {
   if (a->dim < 8 || a->dim > 128 || a->dim % 8) return at_fail(OSAM_ERR_INVALID, "dim is a multiple of 8 up to 128");
   if (!(a->scale > 0.f) || std::isinf(a->scale)) return at_fail(OSAM_ERR_INVALID, "scale is positive and finite");
   if (!(a->cap >= 0.f) || std::isinf(a->cap)) return at_fail(OSAM_ERR_INVALID, "cap is 0 or positive and finite");
+  if (a->cap > 0.f && std::isinf(2.f * a->scale * kAtLog2e / a->cap))  // a score of 0 would be 0·∞
+    return at_fail(OSAM_ERR_INVALID, "cap is too small beside the scale");
   if (a->mask != OSAM_ATTN_NONE && a->mask != OSAM_ATTN_CAUSAL && a->mask != OSAM_ATTN_PREFIX)
     return at_fail(OSAM_ERR_INVALID, "unknown mask");
   if (a->mask == OSAM_ATTN_PREFIX && !a->prefix) return at_fail(OSAM_ERR_INVALID, "a prefix mask needs prefix lengths");

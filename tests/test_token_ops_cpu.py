@@ -244,3 +244,15 @@ def test_adamw_over_any_number_of_elements(sizes):
     assert b"too many" in L.osam_last_error() and nbytes.value == 7
     assert L.osam_adamw_create(tab, len(sizes), 8, 4096, (1 << 64) - 1, None, ctypes.byref(plan)) == INVALID and not plan
     assert b"too many" in L.osam_last_error()
+
+
+def test_vanishing_caps():
+    """cap·tanh(s/cap) needs s/cap: a cap that fp32 cannot divide by is refused, and one that it rounds to 0 is not `none`."""
+    import ctypes
+
+    from objectsam_b200.attn import AttnGeom, AttnOp
+    for kw in (dict(cap=1e-39), dict(cap=1e-10, scale=1e30)):
+        assert fwd(desc(**kw)) == INVALID and b"cap is too small" in lib().osam_last_error(), kw
+    assert lib().osam_attn_workspace_size(ctypes.byref(desc(cap=1e-37))) > 0
+    with pytest.raises(ValueError):
+        AttnOp().init(AttnGeom(1, 4, 4, 1, 1, 64), cap=1e-50)
