@@ -63,6 +63,7 @@ class AdamW:
         check(lib().osam_adamw_create(tab, n, bits, self._table.data_ptr(), nbytes.value, s.cuda_stream,
                                       ctypes.byref(self._plan)))
         self._scales = (None, None) if bits == 32 else (self.m_scale.data_ptr(), self.v_scale.data_ptr())
+        self._streams = {s.cuda_stream}  # that the allocator knows to use the optimizer's own tensors
 
     def close(self) -> None:
         if self._plan:
@@ -93,8 +94,14 @@ class AdamW:
         not finite leaves everything but the step count as it was."""
         if max_norm is not None and not max_norm > 0:
             raise ValueError("max_norm is positive")
+        st = stream_ptr(stream)
+        if st not in self._streams:
+            s = stream if stream is not None else torch.cuda.current_stream()
+            for t in (self._table, self.m, self.v, self.m_scale, self.v_scale, self.norm):
+                if t is not None:
+                    t.record_stream(s)
+            self._streams.add(st)
         check(lib().osam_adamw_step(self._plan, self.m.data_ptr(), self.v.data_ptr(), *self._scales, self.steps + 1,
                                     self.lr if lr is None else lr, self.betas[0], self.betas[1], self.eps,
-                                    self.weight_decay, grad_scale, max_norm or 0.0, self.norm.data_ptr(),
-                                    stream_ptr(stream)))
+                                    self.weight_decay, grad_scale, max_norm or 0.0, self.norm.data_ptr(), st))
         self.steps += 1

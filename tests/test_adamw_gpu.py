@@ -185,3 +185,24 @@ def test_same_bits_every_time(cuda_lib):
             opt.step(max_norm=0.3)
         got.append([t.clone() for t in (*p, opt.norm, opt.m.view(torch.uint8))])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_states_outlive_steps_on_another_stream(cuda_lib):
+    """An optimizer that is let go while its step still waits on another stream than the one it was made on: the allocator
+    does not hand its states out before that step is through."""
+    from objectsam_b200.optim import AdamW
+    p, g, _ = tensors([3_000_001], copy=None)
+    opt = AdamW(p, g)
+    s, big = torch.cuda.Stream(), torch.randn(8192, 8192, device=DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(200):  # a few hundred milliseconds
+            big = big @ big * 1e-2
+    opt.step(stream=s)
+    held, n = {t.data_ptr() for t in (opt.m, opt.v)}, opt.m.numel()
+    del opt
+    again = [torch.empty(n, device=DEV) for _ in range(2)]
+    busy = not s.query()
+    assert not held & {t.data_ptr() for t in again} or not busy
+    assert busy, "the step was through too early for this test"
+    torch.cuda.synchronize()
