@@ -206,3 +206,27 @@ def test_states_outlive_steps_on_another_stream(cuda_lib):
     assert not held & {t.data_ptr() for t in again} or not busy
     assert busy, "the step was through too early for this test"
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_graph_capture(cuda_lib, bits):
+    """A captured step replays with its capture's step count and rate, over gradients read anew."""
+    from objectsam_b200.optim import AdamW
+    p, g, c = tensors([5000, 77])
+    p2, c2 = [t.clone() for t in p], [t.clone() for t in c]
+    a, b = AdamW(p, g, copies=c, bits=bits), AdamW(p2, g, copies=c2, bits=bits)
+    for o in (a, b):
+        o.step(max_norm=1.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step(max_norm=1.0)
+    for by in (1.0, 3.0):
+        for t in g:
+            t.mul_(by)
+        graph.replay()
+        b.step(max_norm=1.0)
+        b.steps -= 1
+    torch.cuda.synchronize()
+    for x, y in zip((*p, *c, a.m.view(torch.uint8), a.v.view(torch.uint8), a.norm), (*p2, *c2, b.m.view(torch.uint8), b.v.view(torch.uint8), b.norm)):
+        assert torch.equal(x, y)

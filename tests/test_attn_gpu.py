@@ -500,3 +500,56 @@ def test_without_a_workspace(cuda_lib):
         for n in want:
             assert torch.equal(out[n], want[n]), n
     assert len(op._ws) == 2
+
+
+def test_graph_capture_of_a_training_step(cuda_lib):
+    """Forward and backward in one graph, over documents that the plan reads anew, on the plan's own workspace."""
+    from objectsam_b200.attn import AttnGeom, AttnOp
+    q, k, v, do = make(2, 300, 300, 4, 2, 64, seed=29)
+    doc = torch.zeros(2, 300, dtype=torch.int32, device=DEV)
+    op = AttnOp().init(AttnGeom(2, 300, 300, 4, 2, 64), mask="causal", doc_q=doc, doc_k=doc)
+    out = {"o": torch.empty_like(q), "lse": torch.empty(2, 4, 300, device=DEV), "dq": torch.empty_like(q),
+           "dk": torch.empty_like(k), "dv": torch.empty_like(v)}
+
+    def step():
+        op.fwd(q, k, v, out["o"], out["lse"])
+        op.bwd(q, k, v, out["o"], out["lse"], do, out["dq"], out["dk"], out["dv"])
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for cut in (300, 130, 1):
+        doc[:, cut:] = 1
+        for t in out.values():
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        want = run(q, k, v, do, mask="causal", doc_q=doc, doc_k=doc)
+        for n in out:
+            assert torch.equal(out[n], want[n]), (cut, n)
+
+
+def test_offsets_past_32_bits(cuda_lib):
+    """A cache whose second sequence lies past 2^31 elements, one of whose heads and tokens are spread as far: the same bits
+    as over a small copy of the rows in use."""
+    Lk, Hk, D, n = 40_000, 448, 128, 130
+    cache = torch.empty(2, Lk, Hk, D, dtype=torch.bfloat16, device=DEV)  # 4.6e9 elements
+    assert cache.stride(0) > 2 ** 31
+    g = torch.Generator(device=DEV).manual_seed(30)
+    q, do = (torch.randn(2, 3, 4, D, generator=g, device=DEV).bfloat16() for _ in range(2))
+    k, v = cache[:, :, 5:9:2], cache[:, :, Hk - 2:]
+    for t in (k, v):
+        t[:, :n] = torch.randn(2, n, 2, D, generator=g, device=DEV).bfloat16()
+        t[1, Lk - 900:] = torch.randn(900, 2, D, generator=g, device=DEV).bfloat16()
+    lens = torch.tensor([n, n], dtype=torch.int32, device=DEV)
+    big = run(q, k, v, do, train=False, mask="causal", lens=lens)
+    small = run(q, k[:, :n].contiguous(), v[:, :n].contiguous(), do, train=False, mask="causal", lens=lens)
+    assert (big["o"].double() - small["o"].double()).abs().max() <= 2.0 ** -7 * small["o"].double().abs().max()
+    assert (big["lse"] - small["lse"]).abs().max() <= 2.0 ** -17
+    # forward and backward over a window at the far end, whose gradients go to views as wide
+    k, v = k[1:, Lk - 900:], v[1:, Lk - 900:]
+    got, want = run(q[1:], k, v, do[1:]), run(q[1:], k.contiguous(), v.contiguous(), do[1:])
+    for x in want:
+        assert torch.equal(got[x], want[x]), x

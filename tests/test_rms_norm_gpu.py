@@ -219,3 +219,34 @@ def test_captured_backward_keeps_its_workspace(cuda_lib):
             graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(small[4], want[0]) and torch.equal(small[5], want[1])
+
+
+def test_graph_capture(cuda_lib):
+    """Forward, e4m3 form and backward in one graph that reads its inputs anew."""
+    from objectsam_b200 import norm
+    g = torch.Generator(device=DEV).manual_seed(7)
+    R, C = 300, 264
+    x, r, dy = (torch.randn(R, C, generator=g, device=DEV).half() for _ in range(3))
+    w = torch.rand(C, generator=g, device=DEV)
+    new = lambda: dict(y=torch.zeros_like(x), h=torch.zeros_like(x), rstd=torch.zeros(R, device=DEV), dx=torch.zeros_like(x),  # noqa: E731
+                       dw=torch.zeros(C, device=DEV), q=torch.zeros(R, C, device=DEV).to(torch.float8_e4m3fn), qs=torch.zeros(R, 3, device=DEV))
+
+    def step(o):
+        norm.rms_norm_fwd(x, w, EPS, o["y"], res=r, total=o["h"], rstd=o["rstd"])
+        norm.rms_norm_fwd_q8(x, w, EPS, o["q"], o["qs"], res=r)
+        norm.rms_norm_bwd(dy, o["h"], w, o["rstd"], o["dx"], o["dw"])
+
+    got = new()
+    step(got)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(got)
+    for by in (1.0, 0.5):
+        x.mul_(by)
+        graph.replay()
+        want = new()
+        step(want)
+        torch.cuda.synchronize()
+        for n in got:
+            assert torch.equal(got[n].view(torch.uint8), want[n].view(torch.uint8)), n
