@@ -530,8 +530,9 @@ int osam_adamw_step(const osam_adamw* a, void* m, void* v, float* m_scale, float
     return OSAM_OK;
   }
   if (!m || !v || (a->bits == 8 && (!m_scale || !v_scale)) ||
-      ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15))
-    return ad_fail(OSAM_ERR_INVALID, "adamw: null or misaligned (16 bytes) states");
+      ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15) ||
+      ((reinterpret_cast<uintptr_t>(m_scale) | reinterpret_cast<uintptr_t>(v_scale) | reinterpret_cast<uintptr_t>(norm)) & 3))
+    return ad_fail(OSAM_ERR_INVALID, "adamw: null or misaligned (16 bytes, scales and norm 4) states");
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const AdChunk* chunks = reinterpret_cast<const AdChunk*>(a->table + a->chunks_at);
   AdNorm* ns = reinterpret_cast<AdNorm*>(a->table);

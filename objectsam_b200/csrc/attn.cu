@@ -218,6 +218,8 @@ int at_cuda(cudaError_t e, const char* what) {
   return OSAM_ERR_CUDA;
 }
 
+bool at_misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 3; }
+
 int at_check(const osam_attn_desc* a) {
   if (!a) return at_fail(OSAM_ERR_INVALID, "null description");
   if (a->dtype != OSAM_F16 && a->dtype != OSAM_BF16) return at_fail(OSAM_ERR_INVALID, "dtype is OSAM_F16 or OSAM_BF16");
@@ -232,6 +234,9 @@ int at_check(const osam_attn_desc* a) {
     return at_fail(OSAM_ERR_INVALID, "unknown mask");
   if (a->mask == OSAM_ATTN_PREFIX && !a->prefix) return at_fail(OSAM_ERR_INVALID, "a prefix mask needs prefix lengths");
   if ((a->doc_q == nullptr) != (a->doc_k == nullptr)) return at_fail(OSAM_ERR_INVALID, "doc_q and doc_k come together");
+  if (at_misaligned(a->slopes) || at_misaligned(a->lens) || at_misaligned(a->prefix) || at_misaligned(a->doc_q) ||
+      at_misaligned(a->doc_k))
+    return at_fail(OSAM_ERR_INVALID, "slopes, lens, prefix and documents are 4-byte aligned");
   if (a->grid_w < 0) return at_fail(OSAM_ERR_INVALID, "grid_w is not negative");
   // in doubles: exact up to here, and products of any descriptions stay in range
   const double most = 1 << 30, B = a->batch, q64 = std::ceil(a->len_q / 64.), k64 = std::ceil(a->len_k / 64.);
@@ -403,6 +408,7 @@ int osam_attn_fwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
   if ((rc = at_view_check(q, a->batch, a->len_q, a->heads_q, "q")) != OSAM_OK ||
       (rc = at_view_check(o, a->batch, a->len_q, a->heads_q, "o")) != OSAM_OK)
     return rc;
+  if (at_misaligned(lse)) return at_fail(OSAM_ERR_INVALID, "lse is 4-byte aligned");
   if (a->len_k > 0 && ((rc = at_view_check(k, a->batch, a->len_k, a->heads_k, "k")) != OSAM_OK ||
                        (rc = at_view_check(v, a->batch, a->len_k, a->heads_k, "v")) != OSAM_OK))
     return rc;
@@ -454,7 +460,7 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
     const char* name[] = {"q", "o", "dout", "dq"};
     for (int i = 0; i < 4; i++)
       if ((rc = at_view_check(*t[i], a->batch, a->len_q, a->heads_q, name[i])) != OSAM_OK) return rc;
-    if (!lse) return at_fail(OSAM_ERR_INVALID, "the backward pass needs the forward's lse");
+    if (!lse || at_misaligned(lse)) return at_fail(OSAM_ERR_INVALID, "the backward pass needs the forward's lse, 4-byte aligned");
   }
   if (a->len_k > 0) {
     const osam_view* t[] = {&k, &v, &dk, &dv};

@@ -299,6 +299,8 @@ bool rms_view(const void* p, long long ld, int C, int bytes_per_8) {  // 8-chann
   return p && ld >= C && ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & (bytes_per_8 - 1)) == 0;
 }
 
+bool rms_f32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
 // Calls f(TPR, NV) as compile-time constants for a row of C channels.
 template <typename F>
 void rms_shape(int C, F f) {
@@ -338,6 +340,8 @@ int rms_fwd(int dtype, RmsFwd P, bool q8, cudaStream_t st, const char* name) {
   if (!P.w || !rms_view(P.x, P.ldx, P.C, 16) || !rms_view(P.y, P.ldy, P.C, q8 ? 8 : 16) ||
       (P.r && !rms_view(P.r, P.ldr, P.C, 16)) || (P.sum && !rms_view(P.sum, P.lds, P.C, 16)) || (q8 && !P.qscale))
     return rms_fail(OSAM_ERR_INVALID, "rms: null, misaligned (16 bytes; 8 for e4m3) or overlapping rows");
+  if (!rms_f32(P.w) || !rms_f32(P.rstd) || !rms_f32(P.qscale))
+    return rms_fail(OSAM_ERR_INVALID, "rms: w, rstd and scales are 4-byte aligned");
   P.inv_c = 1.f / P.C;
   P.groups = (P.C + kRmsGroup - 1) / kRmsGroup;
   const cudaError_t e =
@@ -407,11 +411,12 @@ int osam_rms_bwd(int dtype, const void* dy, int64_t lddy, const void* h, int64_t
   if (dtype != OSAM_F16 && dtype != OSAM_BF16) return rms_fail(OSAM_ERR_INVALID, "rms: dtype is OSAM_F16 or OSAM_BF16");
   if (rows < 0 || C < 8 || C % 8 || C > kRmsMaxC)
     return rms_fail(OSAM_ERR_INVALID, "rms: channels are a multiple of 8, at most 8192");
-  if (!dw) return rms_fail(OSAM_ERR_INVALID, "rms: null dw");
+  if (!dw || !rms_f32(dw)) return rms_fail(OSAM_ERR_INVALID, "rms: null or misaligned dw");
   if (rows == 0) return rms_cuda(cudaMemsetAsync(dw, 0, (size_t)C * sizeof(float), st), "osam_rms_bwd memset");
   if (!w || !rstd || !rms_view(dy, lddy, C, 16) || !rms_view(h, ldh, C, 16) || !rms_view(dx, lddx, C, 16) ||
       (dsum && !rms_view(dsum, lddsum, C, 16)))
     return rms_fail(OSAM_ERR_INVALID, "rms: null, misaligned (16 bytes) or overlapping rows");
+  if (!rms_f32(w) || !rms_f32(rstd)) return rms_fail(OSAM_ERR_INVALID, "rms: w and rstd are 4-byte aligned");
   if (!ws || ws_bytes < osam_rms_bwd_workspace_size(C) || (reinterpret_cast<uintptr_t>(ws) & 15))
     return rms_fail(OSAM_ERR_INVALID, "rms: workspace (osam_rms_bwd_workspace_size, 16-byte aligned)");
   RmsBwd P{};

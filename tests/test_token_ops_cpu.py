@@ -256,3 +256,27 @@ def test_vanishing_caps():
     assert lib().osam_attn_workspace_size(ctypes.byref(desc(cap=1e-37))) > 0
     with pytest.raises(ValueError):
         AttnOp().init(AttnGeom(1, 4, 4, 1, 1, 64), cap=1e-50)
+
+
+def test_pointers_off_their_types():
+    """fp32 and int32 arrays at odd addresses, which a kernel's loads would fault on."""
+    import ctypes
+    L, good = lib(), View(4096, 512, 128, 64)
+    for kw in (dict(slopes=4097), dict(lens=4098), dict(prefix=4099, mask=_lib.ATTN_PREFIX), dict(doc_q=4098, doc_k=4096),
+               dict(doc_q=4096, doc_k=4097)):
+        assert fwd(desc(**kw)) == INVALID and b"aligned" in L.osam_last_error() and b"workspace" not in L.osam_last_error(), kw
+        assert L.osam_attn_workspace_size(ctypes.byref(desc(**kw))) == 0
+    d = ctypes.byref(desc())
+    assert L.osam_attn_fwd(d, good, good, good, good, 4098, None, 0, None) == INVALID and b"lse" in L.osam_last_error()
+    assert L.osam_attn_bwd(d, good, good, good, good, 4098, good, good, good, good, None, 0, None) == INVALID
+    assert b"lse" in L.osam_last_error()
+
+    def rms(w=4096, rstd=4096, qs=None, dw=4096):
+        if qs is not None:
+            return L.osam_rms_fwd_q8(_lib.F16, 4096, 64, None, 0, w, 3, 64, 1e-5, None, 0, 8192, 64, qs, rstd, None)
+        a = L.osam_rms_fwd(_lib.F16, 4096, 64, None, 0, w, 3, 64, 1e-5, None, 0, 8192, 64, rstd, None) if dw == 4096 else INVALID
+        b = L.osam_rms_bwd(_lib.F16, 4096, 64, 4096, 64, w, rstd, None, 0, 3, 64, 8192, 64, dw, 4096, 1 << 30, None)
+        return INVALID if a == b == INVALID else 0
+
+    for kw in (dict(w=4097), dict(rstd=4098), dict(qs=4099), dict(dw=4098)):
+        assert rms(**kw) == INVALID and b"aligned" in L.osam_last_error(), kw
