@@ -533,7 +533,8 @@ int osam_rms_bwd(int dtype, const void* dy, int64_t lddy, const void* h, int64_t
  * from then on.  Steps of one plan run in stream order (they share the table's scratch).
  *   osam_adamw_sizes    bytes of the table and elements of the states
  *   osam_adamw_create   fills `table` (256-byte aligned, kept by the caller) on `stream`
- *   osam_adamw_step     t counts from 1; m, v 16-byte aligned */
+ *   osam_adamw_step     t counts from 1; m, v 16-byte aligned.  t, lr and the other numbers are launch arguments: a captured
+ *                       step replays with those of its capture */
 typedef struct osam_adamw_tensor {
   float* p;        /* parameters, fp32 */
   const void* g;   /* gradients of grad_type */
@@ -571,6 +572,7 @@ int osam_adamw_destroy(osam_adamw* a);
  * lse [batch][heads_q][len_q] fp32 (natural log), or NULL in the forward.  Scores, softmax statistics and sums
  * are fp32; P (and dS in the backward) are rounded to dtype as operands of the second products.  No atomics:
  * results do not depend on scheduling.
+ * Outputs do not overlap each other or the inputs.
  * Workspace osam_attn_workspace_size(desc) bytes (both directions), 256-byte aligned, any contents. */
 enum { OSAM_ATTN_NONE = 0, OSAM_ATTN_CAUSAL = 1, OSAM_ATTN_PREFIX = 2 };
 typedef struct osam_attn_desc {

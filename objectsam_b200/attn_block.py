@@ -86,6 +86,7 @@ class AttnBlock:
         self.conv.dgrad(self.dhid, w["out"], self.da, ws, stream=stream)
         self.attn.bwd(*map(self._heads, self.qkv), self._heads(self.a), self.lse, self._heads(self.da),
                       *map(self._heads, self.dqkv), ws=ws, stream=stream)
+        # dn1 is summed in fp16 over the three projections (dgrad's beta): two roundings beside those of its terms, of one size
         for i, (n, d) in enumerate(zip(self.PROJ, self.dqkv)):
             self.conv.wgrad(self.n1, d, g[n], ws, stream=stream)
             self.conv.dgrad(d, w[n], self.dn1, ws, beta=float(i > 0), stream=stream)

@@ -4,11 +4,11 @@
 //   g' = g·mul;  m = β1·m + (1−β1)·g';  v = β2·v + (1−β2)·g'²
 //   p = p·(1 − lr·wd) − lr/(1−β1ᵗ)·m / (√v/√(1−β2ᵗ) + eps)          (wd = 0 for tensors marked so)
 // 8-bit states, per block of 256 elements: m = e4m3·s_m with s_m = max|m|/448, and the ROOT of v likewise
-// (√v = e4m3·s_v): the root halves the exponent range, so e4m3's 2^18 covers 2^36 in v.  A v above zero is never
+// (√v = e4m3·s_v; the scales by a product with 1/448, values by 448·(1/max), each within a rounding of the quotient): the root halves the exponent range, so e4m3's 2^18 covers 2^36 in v.  A v above zero is never
 // stored as zero (it takes the smallest e4m3 value): a moment that survives beside a vanished v would make its
 // step m/eps.  The step uses the new moments before they are rounded.
 //
-// Bound by HBM: 28 bytes an element with 32-bit states (14 + 1/32 with 8 bits and 32-bit gradients) and 2 more for a
+// Bound by HBM: 28 bytes an element with 32-bit states (16 + 1/16 with 8 bits and 32-bit gradients) and 2 more for a
 // 16-bit weight copy; with 8-bit states the arithmetic (one IEEE square root an element, e4m3 both ways) is close
 // behind, so it runs on pairs (two fp32 operations an instruction, rounded as the single ones are).  A table in
 // device memory, written once, has a record for every chunk of 2048 elements with all that the chunk needs, so

@@ -66,8 +66,8 @@ __device__ __forceinline__ int at_seq_splits(const AttnDev& A, int b, int chunk)
 }
 // Tiles of a split at most, `count(chunk)` being the splits of all B sequences: the smallest chunk with which they fit
 // one or two rounds of the GPU's places, `per` CTAs each, whichever takes less (a CTA's start and end cost about five
-// tiles).  So sequences of any lengths take their share of the CTAs (16 caches of 8192–32768 keys: 233 us, with one
-// number of splits for all 255; 16 caches of 8192 keys: 88 and 108).
+// tiles).  So sequences of any lengths take their share of the CTAs (back to back, 16 caches of 8192–32768 keys:
+// 233 us, with one number of splits for all 255; 16 caches of 8192 keys: 88 and 108).
 template <typename Count>
 __host__ __device__ __forceinline__ int at_best_chunk(int B, int per, int min_tiles, int max_tiles, int total, Count count) {
   int best = 0, least = INT_MAX;

@@ -3,8 +3,9 @@
 //   DKV: 128 keys of a key head stay (K, V), the queries of every head of the group stream (Q, dO):
 //        dV += Pᵀ·dO, dK += dSᵀ·Q — the sum over a shared key head's query heads is this accumulation
 //   DQ : 128 queries of one head stay (Q, dO), the keys stream (K, V):  dQ += dS·K
-// Two passes compute S and dP twice (7 products instead of 5) but every sum is taken by one CTA in one order: no
-// atomics, no fp32 copy of dQ, results that do not depend on scheduling.
+// Two passes compute S and dP twice (7 products instead of 5) but every sum is taken in one order: no atomics, results that
+// do not depend on scheduling.  One CTA takes it whole, without an fp32 copy; or, with few tiles (`parts`), up to eight share
+// the streamed side and k_attn_sum adds their fp32 parts in order.
 //
 // Per tile, rows = the stationary side (TMEM lanes), columns = the streamed side:
 //   X = stat1·strm1ᵀ (scores), Y = stat2·strm2ᵀ (dP), both fp32 in TMEM

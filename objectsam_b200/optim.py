@@ -4,10 +4,10 @@
     opt.step(max_norm=10.0, grad_scale=1 / loss_scale)
 
 params: contiguous float32 CUDA tensors; grads: float32, float16 or bfloat16, one per parameter (views of a gradient
-arena will do, unaligned ones too); copies: 16-bit tensors that receive the new parameters (the operands that the
-convs read), None where a parameter has none.  The tensors' memory is read at every step and must stay in place.
+arena will do, unaligned ones too); copies: 16-bit tensors that receive the new parameters (operands of convs that
+take their weights from the caller, as attn_block.py's do), None where a parameter has none.  The tensors' memory is read at every step and must stay in place.
 States: opt.m, opt.v (float32, or float8_e4m3fn with opt.m_scale, opt.v_scale per 256 elements, where v holds √v).
-opt.norm: the gradients' norm of the last step with max_norm.
+opt.norm: the gradients' norm of the last step with max_norm.  A captured step replays with its capture's count and rate.
 """
 from __future__ import annotations
 
