@@ -484,7 +484,8 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     pair_sum[half][row_of] = l;
     if (SPREAD) {
       pair_low[half][row_of] = l16;
-      named_bar_sync(pair_bar, 64);
+      if (half == 0) pair_top[0][row_of] = m;
+      ok = !at_any(1, !ok, kAfSoft);
     } else {
       ok = !at_pair_any(pair_bar, !ok);
     }
@@ -497,11 +498,6 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
     if (SPREAD) {
       l16 += pair_low[half ^ 1][row_of];
       if (l16 > 0.f) fix = l / l16;
-      if (half == 0) {
-        pair_top[0][row_of] = m;
-        pair_top[1][row_of] = l;
-      }
-      ok = !at_any(1, !ok, kAfSoft);
       float M = -INFINITY;
 #pragma unroll
       for (int k = 0; k < 4; k++) M = fmaxf(M, pair_top[0][k * 32 + lane]);
@@ -510,7 +506,7 @@ __global__ void __launch_bounds__(kAfThreads, 2) k_attn_fwd(const __grid_constan
       for (int k = 0; k < 4; k++) {
         const float mk = pair_top[0][k * 32 + lane];
         w4[k] = mk == -INFINITY ? 0.f : at_ex2(mk - M);
-        l = fmaf(w4[k], pair_top[1][k * 32 + lane], l);
+        l = fmaf(w4[k], pair_sum[0][k * 32 + lane] + pair_sum[1][k * 32 + lane], l);
       }
       m = M;
     }
