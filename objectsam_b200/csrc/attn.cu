@@ -156,48 +156,61 @@ __global__ void __launch_bounds__(256) k_attn_rows(const __grid_constant__ AttnD
   const long long bh = (long long)b * heads + h;
   grid_dep_wait();
   grid_dep_launch();
-  const int n = keys ? at_keys(A, b) : 0;
   float big = 0.f;     // largest ‖·‖²
   bool blind = false;  // a query that sees nothing: the same in all heads
+  auto norm2 = [](const float (&g)[8]) {
+    float s = 0.f;
 #pragma unroll
-  for (int k = 0; k < kAbCols; k += 16) {
-    const int r = k + threadIdx.x / 16, i = blk * kAbCols + r;
-    float L = -INFINITY;
-    bool live;
-    if (keys) {
-      live = i < n && !(A.doc_k && A.doc_k[(long long)b * A.Lk + i] < 0);
-    } else {
-      if (i < A.Lq) L = lse[bh * A.Lq + i];
-      live = L != -INFINITY;
+    for (int e = 0; e < 8; e++) s = fmaf(g[e], g[e], s);
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    return s <= FLT_MAX ? s : 0.f;  // neither infinite nor NaN
+  };
+  if (keys) {
+    const int n = at_keys(A, b);
+    int id[kAbCols / 16];
+    uint4 u[kAbCols / 16];
+#pragma unroll
+    for (int k = 0; k < kAbCols / 16; k++) {  // all loads first
+      const int i = blk * kAbCols + k * 16 + threadIdx.x / 16;
+      id[k] = i < n ? (A.doc_k ? A.doc_k[(long long)b * A.Lk + i] : 0) : -1;
+      u[k] = make_uint4(0, 0, 0, 0);
+      if (i < n && c * 8 < D) u[k] = *reinterpret_cast<const uint4*>(static_cast<const T*>(v.p) + b * v.sb + i * v.st + h * v.sh + c * 8);
+    }
+#pragma unroll
+    for (int k = 0; k < kAbCols / 16; k++) {
+      float g[8];
+      unpack8<T>(u[k], g);
+      const float s = norm2(g);
+      if (id[k] >= 0) big = fmaxf(big, s);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kAbCols; k += 16) {
+      const int r = k + threadIdx.x / 16, i = blk * kAbCols + r;
+      const float L = i < A.Lq ? lse[bh * A.Lq + i] : -INFINITY;
+      const bool live = L != -INFINITY;
       blind |= i < A.Lq && !live;
-    }
-    const AtView& t = keys ? v : dout;
-    float d = 0.f, s2 = 0.f;
-    if (live && c * 8 < D) {
-      float a[8], g[8];
-      unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(t.p) + b * t.sb + i * t.st + h * t.sh + c * 8), g);
-      if (!keys) {
+      float a[8] = {}, g[8] = {};
+      if (live && c * 8 < D) {
         unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(o.p) + b * o.sb + i * o.st + h * o.sh + c * 8), a);
-#pragma unroll
-        for (int e = 0; e < 8; e++) d = fmaf(a[e], g[e], d);
+        unpack8<T>(
+            *reinterpret_cast<const uint4*>(static_cast<const T*>(dout.p) + b * dout.sb + i * dout.st + h * dout.sh + c * 8), g);
       }
-      if (!BF16)
+      float d = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) s2 = fmaf(g[e], g[e], s2);
-    }
+      for (int e = 0; e < 8; e++) d = fmaf(a[e], g[e], d);
 #pragma unroll
-    for (int s = 8; s > 0; s >>= 1) {
-      d += __shfl_xor_sync(0xffffffffu, d, s);
-      if (!BF16) s2 += __shfl_xor_sync(0xffffffffu, s2, s);
-    }
-    if (s2 <= FLT_MAX) big = fmaxf(big, s2);  // neither infinite nor NaN
-    if (c == 0 && !keys) {
-      float* out = rows + (bh * nb + blk) * 2 * kAbCols + r;
-      out[0] = live ? up - L * kAtLog2e : -INFINITY;
-      out[kAbCols] = live ? -d : 0.f;
+      for (int s = 8; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
+      if (!BF16) big = fmaxf(big, norm2(g));
+      if (c == 0) {
+        float* out = rows + (bh * nb + blk) * 2 * kAbCols + r;
+        out[0] = live ? up - L * kAtLog2e : -INFINITY;
+        out[kAbCols] = live ? -d : 0.f;
+      }
     }
   }
-  if (sum_q && !keys && h == 0 && blind && c == 0) sum_q[(long long)b * nq + blk].pad = 1;
+  if (sum_q && h == 0 && blind && c == 0) sum_q[(long long)b * nq + blk].pad = 1;
   if (BF16) return;
   big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
   if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = big;
@@ -507,7 +520,13 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
                    "sum launch");
   };
   const int g = a->heads_q / a->heads_k;
+  const auto ctas = [&](bool dkv) {
+    return (double)(((dkv ? a->len_k : a->len_q) + kAbRows - 1) / kAbRows) * a->batch * (dkv ? a->heads_k : a->heads_q) *
+           at_parts(*a, dkv);
+  };
+  const double nkv = ctas(true), nq = ctas(false);
   if (!ek) {
+    L.alone = nkv + std::ceil(nq / 2) <= kAtSms;  // the longer pass; dQ's CTAs then have the other SMs, two each
     L.parts = at_parts(*a, true);
     L.group = at_group(*a, (a->len_k + kAbRows - 1) / kAbRows, (long long)a->batch * a->heads_k * L.parts,
                        4.0 * a->len_q * a->dim * g / L.parts);
@@ -522,6 +541,7 @@ int osam_attn_bwd(const osam_attn_desc* a, osam_view q, osam_view k, osam_view v
       return rc;
   }
   if (!eq) {
+    L.alone = nkv + nq <= kAtSms;
     L.parts = at_parts(*a, false);
     L.group = at_group(*a, (a->len_q + kAbRows - 1) / kAbRows, (long long)a->batch * a->heads_q * L.parts,
                        4.0 * a->len_k * a->dim / g / L.parts);

@@ -537,6 +537,7 @@ struct AttnBwdLaunch {
   const float* rows;      // [B][Hq][⌈Lq/64⌉][2][64]: log2 of P's factor − lse·log2 e (−∞ where the query is empty), −δ
   const float* peak;      // fp16: [B][Hq][⌈Lq/64⌉] max ‖dO_i‖ of the block
   const float* vpeak;     // fp16: [B][Hk][⌈Lk/64⌉] max ‖v_j‖ of the block
+  int alone;              // has its SMs to itself, one CTA each
   int late;               // DQ behind DKV, which it does not depend on: waits for that kernel's end only at its own end
   int group;              // at_order
   int parts;              // CTAs that share a tile's streamed side (few tiles: to fill the GPU); above 1 they write

@@ -21,6 +21,7 @@
 // MMA issuer.  Up to 64 head dims one buffer and 256 TMEM columns, two CTAs per SM; above, two buffers in one CTA
 // with all 512 columns: the tensor cores work on one while the other is in the element-wise part.
 #pragma once
+#include <algorithm>
 #include <type_traits>
 
 #include "attn.cuh"
@@ -335,11 +336,12 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
         }
         named_bar_sync(1 + buf, 256);
       }
-      ok = ok && at_wait_warp(&xy_full[buf], (it / NB) & 1, A.err);
+      // DKV: full counts the rows' bulk copy
+      ok = ok && at_wait_warp(&xy_full[buf], (it / NB) & 1, A.err) &&
+           (!DKV || at_wait_warp(&full[it % Cfg::STAGES], (it / Cfg::STAGES) & 1, A.err));
       tc_fence_after();
       const int s = it % Cfg::STAGES;
       const float* rows = reinterpret_cast<const float*>(srows + s * Cfg::ROWS) + h0;
-      if (DKV) ok = ok && at_wait_warp(&full[s], (it / Cfg::STAGES) & 1, A.err);  // counts the rows' bulk copy
       if (BIAS == 1) bias.y = float(pos - (DKV ? off + c0 : c0) - h0) * bias.slope;
       const uint32_t xcol = tmem + lane_base + buf * 128;
       float sv[32], dp[32];
@@ -467,6 +469,11 @@ __global__ void __launch_bounds__(AbCfg<DP>::THREADS, AbCfg<DP>::CTAS)
   }
 }
 
+// Shared memory of which an SM has room for one CTA only.  The passes run side by side, and where the GPU holds both at once,
+// dQ's CTAs were at times put on the SMs of dK's and dV's all the same, beside idle ones (297 tokens, 4 heads × 64: the
+// backward in 26.9 us, so 21.0; 2 × 605 tokens, 16/4 × 64: 66.6 and 64.5).
+constexpr int kAbAlone = 116 * 1024;
+
 template <typename T, int DP, bool DKV, int CAP, int BIAS>
 cudaError_t attn_bwd_one(const AttnBwdLaunch& L, int grid, cudaStream_t st) {
   static bool set[64] = {};  // per device; a race only repeats the call
@@ -475,11 +482,11 @@ cudaError_t attn_bwd_one(const AttnBwdLaunch& L, int grid, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   auto* k = k_attn_bwd<T, DP, DKV, CAP, BIAS>;
   if (dev >= 64 || !set[dev]) {
-    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, AbCfg<DP>::SMEM);
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(AbCfg<DP>::SMEM, kAbAlone));
     if (e != cudaSuccess) return e;
     if (dev < 64) set[dev] = true;
   }
-  return launch_dependent(k, grid, AbCfg<DP>::THREADS, AbCfg<DP>::SMEM, st, L);
+  return launch_dependent(k, grid, AbCfg<DP>::THREADS, L.alone ? std::max(AbCfg<DP>::SMEM, kAbAlone) : AbCfg<DP>::SMEM, st, L);
 }
 
 template <typename T, int DP, bool DKV, int CAP>
