@@ -553,3 +553,14 @@ def test_offsets_past_32_bits(cuda_lib):
     got, want = run(q[1:], k, v, do[1:]), run(q[1:], k.contiguous(), v.contiguous(), do[1:])
     for x in want:
         assert torch.equal(got[x], want[x]), x
+
+
+@pytest.mark.parametrize("bias", ["line", "grid"])
+@pytest.mark.parametrize("docs", [False, True])
+def test_slopes_of_either_sign_in_one_tile(cuda_lib, bias, docs):
+    """More heads to a key head than a warp has rows: warps of one tile with and without a negative slope keep step."""
+    q, k, v, do = make(1, 5, 300, 130, 1, 32, seed=31)
+    slopes = torch.full((130,), 0.02, device=DEV)
+    slopes[40:45], slopes[100:] = -0.03, -0.01
+    dq, dk = (torch.arange(n, dtype=torch.int32, device=DEV).div(n // 2, rounding_mode="floor").int()[None].contiguous() for n in (5, 300))
+    check(q, k, v, do, slopes=slopes, grid_w=20 if bias == "grid" else 0, doc_q=dq if docs else None, doc_k=dk if docs else None)
